@@ -75,9 +75,11 @@ def build_kernels(force=False, jobs=8, verbose=False):
         o = os.path.join(BUILD, os.path.basename(s) + '.o')
         objs.append(o)
         if force or _newer(o, [s] + hdrs):
+            # no packed fp32 instructions (v_pk_{add,mul,fma}_f32): some of their forms have given
+            # wrong results on this hardware; the host pass warns that it does not know the feature
             jobs_list.append([HIPCC, '--offload-arch=' + ARCH, '-O3', '-std=c++17', '-fPIC', '-c', s, '-o', o,
                               '-I' + os.path.join(CSRC, 'include'), '-munsafe-fp-atomics',
-                              '-Wno-unused-result'])
+                              '-Wno-unused-result', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops'])
     # host-only TUs against the torch / ROCm headers: the bindings and the native
     # gradient reducer (c10d process groups, autograd hooks, HIP events)
     for b_src in (os.path.join(CSRC, 'bindings.cpp'), os.path.join(CSRC, 'native', 'reducer.cpp')):
