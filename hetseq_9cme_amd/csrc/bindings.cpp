@@ -736,6 +736,200 @@ std::vector<Tensor> gemm_f16_dgelu(Tensor a, Tensor a_amax, Tensor b, Tensor b_a
   return {t, rm, cm, db};
 }
 
+// ------------------------------------------------------------------ 8-bit blocks (quant8.hip, gemm_fp8.hip)
+inline bool rows_vec(const Tensor& t, int64_t ld) {   // 16-B accesses of 8 consecutive elements of a row
+  return aligned16(t.data_ptr()) && ld % (t.scalar_type() == torch::kFloat32 ? 4 : 8) == 0;
+}
+inline int64_t blocks128(int64_t n) { return (n + 127) / 128; }
+inline void check_bias8(const OptT& b, int64_t N, const Tensor& like, const char* what) {
+  if (!has(b)) return;
+  check_f32(*b, what);
+  TORCH_CHECK(b->numel() == N && b->device() == like.device(), what, ": fp32 [N] on the tensor's device");
+}
+inline void check_rows8(const Tensor& x, const char* what) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.stride(1) == 1 || x.size(1) == 1) && (x.stride(0) >= x.size(1) || x.size(0) <= 1),
+              what, ": a 2-D GPU tensor with unit column stride");
+  act_bf16(x);
+  TORCH_CHECK(x.size(0) < (1LL << 31) - 128 && x.size(1) >= 1 && x.size(1) <= (1LL << 22) &&
+                  blocks128(x.size(0)) * blocks128(x.size(1)) < (1LL << 31),
+              what, ": fewer than 2^31 rows of 1 .. 2^22 columns");
+}
+inline Tensor scale_words(int64_t rows, int64_t cols, const Tensor& like) {
+  // one byte per row and block of 128; four blocks of a row to a word, rows rounded up to 4
+  return torch::empty({(blocks128(cols) + 3) / 4, (rows + 3) / 4 * 4, 4}, like.options().dtype(torch::kUInt8));
+}
+
+// x [R, C] -> (q, s, qt, st, sum): its e4m3 codes blocked along the columns (by_rows) and transposed,
+// blocked along the rows (by_cols), and its fp32 column sums (sum_out / want_sum); undefined where
+// not wanted
+std::vector<OptT> split8(Tensor x, bool by_rows, bool by_cols, bool want_sum, OptT sum_out) {
+  check_rows8(x, "split8");
+  const int64_t R = x.size(0), C = x.size(1);
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  auto u8 = x.options().dtype(torch::kUInt8);
+  auto f32 = x.options().dtype(torch::kFloat32);
+  OptT q, s, qt, st, sum;
+  if (by_rows) {
+    q = torch::empty({R, blocks128(C) * 128}, u8);
+    s = scale_words(R, C, x);
+  }
+  if (by_cols) {
+    TORCH_CHECK(R <= (1LL << 22), "split8: at most 2^22 rows blocked along the rows");
+    qt = torch::empty({C, blocks128(R) * 128}, u8);
+    st = scale_words(C, R, x);
+  }
+  Tensor part;
+  if (want_sum) {
+    sum = has(sum_out) ? *sum_out : torch::empty({C}, f32);
+    check_f32(*sum, "split8 column sums");
+    TORCH_CHECK(sum->numel() == C && sum->device() == x.device(), "split8: column sums [C]");
+    if (R == 0) sum->zero_();
+    else part = torch::empty({hx_split8_row_tiles(R), C}, f32);
+  }
+  if (R > 0 && (by_rows || by_cols || want_sum))
+    hx_split8(act_bf16(x), x.data_ptr(), R > 1 ? x.stride(0) : C, (int)R, (int)C, ptr_or_null<uint8_t>(q),
+              ptr_or_null<uint8_t>(s), ptr_or_null<uint8_t>(qt), ptr_or_null<uint8_t>(st),
+              want_sum ? part.data_ptr<float>() : nullptr, ptr_or_null<float>(sum), rows_vec(x, R > 1 ? x.stride(0) : C),
+              cur_stream(x));
+  return {q, s, qt, st, sum};
+}
+
+// C [M, N] (+)= A . B^T (+ bias) on split8's codes: A (q, s) of an [M, K] operand, B of an [N, K] one.
+// bf16 results on the scaled e4m3 instructions, fp32 results on decoded bf16 ones (gemm_fp8.hip).
+Tensor gemm_fp8(Tensor a, Tensor as, Tensor b, Tensor bs, int64_t K, bool out_bf16, OptT out_, bool beta, OptT bias) {
+  const int64_t M = a.size(0), N = b.size(0), nkb = blocks128(K);
+  auto operand = [&](const Tensor& q, const Tensor& s, const char* what) {
+    TORCH_CHECK(q.is_cuda() && q.scalar_type() == torch::kUInt8 && q.dim() == 2 && q.is_contiguous() && aligned16(q.data_ptr()) &&
+                    q.size(1) == nkb * 128 && q.size(0) < (1LL << 31) - 256 && q.size(1) <= (1LL << 22) && q.device() == a.device(), what,
+                ": codes [rows, K rounded up to 128] on one device");
+    TORCH_CHECK(s.is_cuda() && s.scalar_type() == torch::kUInt8 && s.is_contiguous() && aligned16(s.data_ptr()) && s.device() == a.device() &&
+                    s.numel() == (nkb + 3) / 4 * ((q.size(0) + 3) / 4 * 4) * 4 && s.numel() < (1LL << 31), what, ": scale words");
+  };
+  TORCH_CHECK(K >= 1, "gemm_fp8: an empty reduction");
+  operand(a, as, "gemm_fp8 a");
+  operand(b, bs, "gemm_fp8 b");
+  check_bias8(bias, N, a, "gemm_fp8 bias");
+  TORCH_CHECK(!beta || has(out_), "gemm_fp8: beta needs an output to accumulate into");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
+  const auto dt = out_bf16 ? torch::kBFloat16 : torch::kFloat32;
+  Tensor out = has(out_) ? *out_ : torch::empty({M, N}, a.options().dtype(dt));
+  TORCH_CHECK(out.scalar_type() == dt && out.device() == a.device() && out.dim() == 2 && out.size(0) == M && out.size(1) == N &&
+                  (out.stride(1) == 1 || N == 1) && (M <= 1 || out.stride(0) >= N),
+              "gemm_fp8: out must be [M, N] of the result type with unit column stride");
+  if (M == 0 || N == 0) return out;
+  const int es = out_bf16 ? 2 : 4;
+  HxGemm8 g{};
+  g.A = a.data_ptr<uint8_t>();
+  g.lda = a.size(1);
+  g.sa = reinterpret_cast<const uint32_t*>(as.data_ptr());
+  g.B = b.data_ptr<uint8_t>();
+  g.ldb = b.size(1);
+  g.sb = reinterpret_cast<const uint32_t*>(bs.data_ptr());
+  g.C = out.data_ptr();
+  g.ldc = M > 1 ? out.stride(0) : N;
+  g.bias = ptr_or_null<float>(bias);
+  g.M = (int)M;
+  g.N = (int)N;
+  g.nkb = (int)nkb;
+  g.beta = beta ? 1 : 0;
+  const int cfg = hx_gemm_fp8_plan(g.M, g.N);
+  g.ks = hx_gemm_fp8_ks(g.M, g.N, g.nkb, cfg);
+  g.vec = aligned16(g.C) && g.ldc * es % 16 == 0 && N * es % 16 == 0;
+  Tensor part;
+  if (g.ks > 1) {
+    part = torch::empty({g.ks, M, N}, a.options().dtype(torch::kFloat32));
+    HxGemm8 p = g;
+    p.C = part.data_ptr();
+    p.ldc = N;
+    p.c_zs = M * N;
+    p.bias = nullptr;
+    p.beta = 0;
+    p.vec = N % 4 == 0;
+    TORCH_CHECK(hx_gemm_fp8(p, cfg, out_bf16 ? 0 : 1, 0, cur_stream(a)) == 0, "gemm_fp8: split-K launch failed");
+    hx_gemm_fp8_slabs(part.data_ptr<float>(), g.C, out_bf16, g.ldc, g.M, g.N, g.ks, g.bias, g.beta,
+                      N % 4 == 0 && aligned16(g.C) && g.ldc % 4 == 0 && (!out_bf16 || g.ldc % 8 == 0), cur_stream(a));
+  } else {
+    TORCH_CHECK(hx_gemm_fp8(g, cfg, out_bf16 ? 0 : 1, out_bf16 ? 1 : 0, cur_stream(a)) == 0, "gemm_fp8: launch failed");
+  }
+  dbg_finite(out, "gemm_fp8");
+  return out;
+}
+
+// ---- int8 blocks along the last dimension (contiguous rows): codes [rows, nb, 128], scale bytes [rows, nb]
+inline void check_kept(const Tensor& q, const Tensor& s, const Tensor& like, int64_t rows, int64_t N, const char* what) {
+  TORCH_CHECK(q.is_cuda() && q.scalar_type() == torch::kUInt8 && q.is_contiguous() && aligned16(q.data_ptr()) &&
+                  q.numel() == rows * blocks128(N) * 128 && s.is_cuda() && s.scalar_type() == torch::kUInt8 && s.is_contiguous() &&
+                  s.numel() == rows * blocks128(N) && q.device() == like.device() && s.device() == like.device(),
+              what, ": int8 codes [rows, blocks, 128] and scale bytes [rows, blocks] on the tensor's device");
+}
+inline std::pair<int64_t, int64_t> rows_cols8(const Tensor& x, const char* what) {
+  check_cuda(x, what);
+  act_bf16(x);
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) < (1LL << 30), what, ": a last dimension of 1 .. 2^30");
+  const int64_t rows = x.numel() / x.size(-1);
+  TORCH_CHECK(blocks128(x.size(-1)) * ((rows + 63) / 64) < (1LL << 31), what, ": too many rows");
+  return {rows, x.size(-1)};
+}
+
+std::vector<Tensor> gelu8_fwd(Tensor y, OptT b) {
+  const auto [rows, N] = rows_cols8(y, "gelu8_fwd y");
+  check_bias8(b, N, y, "gelu8_fwd bias");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(y.device());
+  Tensor out = torch::empty_like(y);
+  Tensor q = torch::empty({rows, blocks128(N), 128}, y.options().dtype(torch::kUInt8));
+  Tensor s = torch::empty({rows, blocks128(N)}, y.options().dtype(torch::kUInt8));
+  const bool vec = rows_vec(y, N) && aligned16(out.data_ptr()) && (!has(b) || aligned16(b->data_ptr()));
+  if (rows > 0)
+    hx_gelu8_fwd(act_bf16(y), y.data_ptr(), ptr_or_null<float>(b), out.data_ptr(), q.data_ptr<uint8_t>(),
+                 s.data_ptr<uint8_t>(), rows, (int)N, vec, cur_stream(y));
+  dbg_finite(out, "gelu8_fwd");
+  return {out, q, s};
+}
+
+std::vector<OptT> gelu8_bwd(Tensor dout, Tensor q, Tensor s, OptT b, bool want_db, OptT db_out) {
+  const auto [rows, N] = rows_cols8(dout, "gelu8_bwd dout");
+  check_kept(q, s, dout, rows, N, "gelu8_bwd");
+  check_bias8(b, N, dout, "gelu8_bwd bias");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dout.device());
+  auto f32 = dout.options().dtype(torch::kFloat32);
+  Tensor dy = torch::empty_like(dout), part;
+  OptT db;
+  if (want_db) {
+    db = has(db_out) ? *db_out : torch::empty({N}, f32);
+    check_bias8(db, N, dout, "gelu8_bwd bias gradient");
+    if (rows == 0) db->zero_();
+    else part = torch::empty({hx_gelu8_chunks(rows), N}, f32);
+  }
+  const bool vec = rows_vec(dout, N) && aligned16(dy.data_ptr()) && (!has(b) || aligned16(b->data_ptr()));
+  if (rows > 0)
+    hx_gelu8_bwd(act_bf16(dout), dout.data_ptr(), q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), ptr_or_null<float>(b),
+                 dy.data_ptr(), want_db ? part.data_ptr<float>() : nullptr, ptr_or_null<float>(db), rows, (int)N, vec,
+                 cur_stream(dout));
+  dbg_finite(dy, "gelu8_bwd");
+  return {dy, db};
+}
+
+std::vector<Tensor> pack8(Tensor x) {
+  const auto [rows, N] = rows_cols8(x, "pack8 x");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  Tensor q = torch::empty({rows, blocks128(N), 128}, x.options().dtype(torch::kUInt8));
+  Tensor s = torch::empty({rows, blocks128(N)}, x.options().dtype(torch::kUInt8));
+  if (rows > 0)
+    hx_pack8(act_bf16(x), x.data_ptr(), q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), rows, (int)N, rows_vec(x, N), cur_stream(x));
+  return {q, s};
+}
+
+Tensor unpack8(Tensor q, Tensor s, int64_t N, bool bf16) {
+  TORCH_CHECK(q.dim() == 3 && N >= 1 && q.size(1) == blocks128(N) && q.size(2) == 128, "unpack8: codes [rows, ceil(N / 128), 128]");
+  const int64_t rows = q.size(0);
+  check_kept(q, s, q, rows, N, "unpack8");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  Tensor x = torch::empty({rows, N}, q.options().dtype(bf16 ? torch::kBFloat16 : torch::kFloat32));
+  if (rows > 0)
+    hx_unpack8(bf16, q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), x.data_ptr(), rows, (int)N, rows_vec(x, N), cur_stream(q));
+  return x;
+}
+
 // the per-column scale source of a weight-gradient operand: 1-D = partials of the whole tensor (a
 // per-tensor bound), 2-D [P, cols] = P partials per column; with aff = (gamma, beta) the
 // LayerNorm-output bound (|gamma| z + |beta|) mul instead (t unused)
@@ -1105,6 +1299,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("dbias_out") = py::none(), py::arg("bias") = py::none(), py::arg("dmode") = 1);
   m.def("gemm_bf16", &gemm_bf16, py::arg("a"), py::arg("b"), py::arg("out") = py::none(), py::arg("beta") = false,
         py::arg("bias") = py::none(), py::arg("out_bf16") = true);
+  m.def("split8", &split8, py::arg("x"), py::arg("by_rows"), py::arg("by_cols"), py::arg("want_sum") = false,
+        py::arg("sum_out") = py::none());
+  m.def("gemm_fp8", &gemm_fp8, py::arg("a"), py::arg("as"), py::arg("b"), py::arg("bs"), py::arg("K"), py::arg("out_bf16"),
+        py::arg("out") = py::none(), py::arg("beta") = false, py::arg("bias") = py::none());
+  m.def("gelu8_fwd", &gelu8_fwd);
+  m.def("gelu8_bwd", &gelu8_bwd, py::arg("dout"), py::arg("q"), py::arg("s"), py::arg("bias"), py::arg("want_db"),
+        py::arg("db_out") = py::none());
+  m.def("pack8", &pack8);
+  m.def("unpack8", &unpack8);
   m.def("weight_bf16_t", &weight_bf16_t);
 
   m.def("gemm_f16_plan", &hx_gemm_f16_plan);

@@ -233,3 +233,40 @@ hipStream_t hx_priority_stream(int prio);
 void hx_stream_priority_range(int* least, int* greatest);
 void hx_destroy_stream(hipStream_t s);
 void hx_spin(int blocks, double us, int lds_bytes, uint32_t* sink, hipStream_t s);
+
+// quant8.hip -- 8-bit blocks of 128 (hx_quant.h).  vec: rows allow 16-B accesses.
+// split8: x [R, C] (row stride ld) -> e4m3 codes q [R, 128 ceil(C / 128)] blocked along the columns and
+// / or qt [C, 128 ceil(R / 128)] blocked along the rows (either may be null), with their scale bytes s /
+// st (block b of row r at ((b / 4) Rs + r) 4 + b % 4, Rs = rows rounded up to 4), and / or the column
+// sums (colpart: [row tiles][C] fp32 workspace, with colsum [C])
+int hx_split8_row_tiles(int64_t R);
+void hx_split8(int bf16, const void* x, int64_t ld, int R, int C, uint8_t* q, uint8_t* s, uint8_t* qt, uint8_t* st,
+               float* colpart, float* colsum, int vec, hipStream_t stream);
+// int8 blocks along contiguous rows of N: codes [rows][nb][128], scale bytes [rows][nb], nb = ceil(N / 128)
+void hx_gelu8_fwd(int bf16, const void* y, const float* b, void* out, uint8_t* q, uint8_t* s, int64_t rows, int N,
+                  int vec, hipStream_t stream);
+int hx_gelu8_chunks(int64_t rows);
+void hx_gelu8_bwd(int bf16, const void* dout, const uint8_t* q, const uint8_t* s, const float* b, void* dy,
+                  float* partial, float* db, int64_t rows, int N, int vec, hipStream_t stream);
+void hx_pack8(int bf16, const void* x, uint8_t* q, uint8_t* s, int64_t rows, int N, int vec, hipStream_t stream);
+void hx_unpack8(int bf16, const uint8_t* q, const uint8_t* s, void* x, int64_t rows, int N, int vec, hipStream_t stream);
+
+// gemm_fp8.hip -- C[M][N] (+)= A . B^T (+ bias) on split8's codes (lda / ldb = padded row lengths,
+// multiples of 128; nkb = k blocks); sa / sb: their scale words
+struct HxGemm8 {
+  const uint8_t* A;
+  int64_t lda;
+  const uint32_t* sa;
+  const uint8_t* B;
+  int64_t ldb;
+  const uint32_t* sb;
+  void* C;          // fp32 or bf16; slab z of a split reduction at C + z c_zs (fp32)
+  int64_t ldc, c_zs;
+  const float* bias;
+  int M, N, nkb, beta, ks, vec;   // vec: C rows allow 16-B stores and N is a whole number of them
+};
+int hx_gemm_fp8_plan(int M, int N);
+int hx_gemm_fp8_ks(int M, int N, int nkb, int cfg);
+int hx_gemm_fp8(const HxGemm8& g, int cfg, int exact, int out_bf16, hipStream_t s);
+void hx_gemm_fp8_slabs(const float* part, void* out, int out_bf16, int64_t ldc, int M, int N, int ks, const float* bias,
+                       int beta, int vec, hipStream_t s);

@@ -1,0 +1,124 @@
+// 8-bit blocks: 128 consecutive entries share one power-of-two scale 2^e.
+//
+//   e4m3 : e = the smallest integer with max |x| <= 448 2^e,  code = e4m3(x 2^-e), nearest even
+//   int8 : e = the smallest integer with max |x| <= 127 2^e,  code = rint(x 2^-e)
+//
+// over the block's finite entries (all zero: e = 0), e >= -126 so that 2^e and 2^-e are normal fp32
+// numbers.  Scaling by a power of two is exact, so the only rounding is the code's own and any
+// order of the same arithmetic gives the same bits; and 2^e is one byte (e + 127), the form the
+// scaled matrix instructions take.  A general scale max / 448 would keep at most one bit more of
+// range and cost that rounding.  Entries that are not finite: e4m3 NaN, int8 -128.
+#pragma once
+#include "hx_common.h"
+
+namespace hx {
+namespace q8 {
+
+constexpr int kBlock = 128;
+
+// (exponent of the largest code, mantissa bits of the largest code): 448 = 1.75 2^8, 127 = 1.984375 2^6
+struct E4M3 {
+  static constexpr int top_exp = 8;
+  static constexpr uint32_t top_man = 0x600000u;
+};
+struct Int8 {
+  static constexpr int top_exp = 6;
+  static constexpr uint32_t top_man = 0x7E0000u;
+};
+
+// the block exponent from its largest finite magnitude
+template <typename F>
+__device__ __forceinline__ int block_exp(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const int e = (int)(u >> 23) - 127 - F::top_exp + ((u & 0x7fffffu) > F::top_man ? 1 : 0);
+  return u == 0 ? 0 : (e < -126 ? -126 : e);   // (a subnormal maximum clamps too)
+}
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 .. 127
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;   // inf / NaN do not take part in the maximum
+}
+
+// 4 scaled values -> 4 e4m3 codes in one word (v_cvt_pk_fp8_f32: nearest even; |x| <= 448 or not finite)
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+// one scaled value -> its int8 code in the low byte
+__device__ __forceinline__ uint32_t int8_of(float v) {
+  const float r = rintf(v);
+  return fabsf(r) <= 127.f ? (uint32_t)(int)r & 0xffu : 0x80u;
+}
+__device__ __forceinline__ uint32_t int8x4(float a, float b, float c, float d) {
+  return int8_of(a) | (int8_of(b) << 8) | (int8_of(c) << 16) | (int8_of(d) << 24);
+}
+// byte j of a word of int8 codes -> its value times s
+__device__ __forceinline__ float int8_val(uint32_t w, int j, float s) {
+  const int c = (int)(w << (24 - 8 * j)) >> 24;
+  return c == -128 ? __uint_as_float(0x7fc00000u) : (float)c * s;
+}
+
+// ---- typed access of 8 consecutive elements as fp32
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8<uint16_t>(const uint16_t* p, float (&v)[8]) {
+  const uint4 x = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[2 * k] = __uint_as_float(w[k] << 16);
+    v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint32_t bf16x2(float a, float b) { return f2bf(a) | ((uint32_t)f2bf(b) << 16); }
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]);
+template <>
+__device__ __forceinline__ void store8<float>(float* p, const float (&v)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <>
+__device__ __forceinline__ void store8<uint16_t>(uint16_t* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]), bf16x2(v[4], v[5]), bf16x2(v[6], v[7]));
+}
+// 8 elements of a row of which n (<= 0: none) are inside; vec: the row allows one wide access
+template <typename T>
+__device__ __forceinline__ void load_upto(const T* p, int n, bool vec, float (&v)[8]) {
+  if (vec && n >= 8) {
+    load8<T>(p, v);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = k < n ? io<T>::ld(p + k) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void store_upto(T* p, int n, bool vec, const float (&v)[8]) {
+  if (vec && n >= 8) {
+    store8<T>(p, v);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (k < n) io<T>::st(p + k, v[k]);
+}
+
+// max over the 16 lanes that hold one block's row
+__device__ __forceinline__ float max16(float m) {
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  return m;
+}
+
+}  // namespace q8
+}  // namespace hx

@@ -11,6 +11,9 @@ from .fused import (  # noqa: F401
     decoder_xent, masked_rows, gelu_ref, layer_norm_ref, linear, grad_slot, ResidualGrad,
     set_side_stream, active_side_stream, side_join, ffn, ffn_fusable, qkv_weight_view, weight_pieces_scope,
 )
+from .fp8 import (  # noqa: F401
+    linear_fp8, linear3_fp8, Fp8Weight, fp8_scope, pack8, unpack8, Packed8, checkpoint8,
+)
 
 
 def flat_grad_norm_clip(grad_flat, gscale, out_norm, clipped, max_norm):

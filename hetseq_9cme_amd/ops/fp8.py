@@ -1,0 +1,399 @@
+"""8-bit training: linear layers on e4m3 operands, activations kept in 8 bits for the backward.
+
+A block is 128 consecutive entries sharing one power-of-two scale 2^e (csrc/include/hx_quant.h):
+
+* e4m3 (operands of products): e the smallest integer with max |x| <= 448 2^e, code = e4m3(x 2^-e);
+* int8 (kept activations):     e the smallest integer with max |x| <= 127 2^e, code = rint(x 2^-e),
+
+both rounded to nearest even; e = 0 for a block of zeros, e >= -126.  Entries that are not finite do
+not take part in the maximum and come back as NaN, so an overflow still reaches the loss and the
+gradient norm.  A power of two costs at most one bit of a block's range and rounds nothing itself,
+so codes are the same bits whatever computes them.
+
+``linear_fp8`` blocks every operand along the dimension its product sums over:
+
+    y  = Q(x)  Q(W)^T + b      blocks along the input features
+    dx = Q(dy) Q(W^T)^T        blocks along the output features
+    dW = Q(dy^T) Q(x^T)^T      blocks along the tokens
+    db = sum of dy's rows      (not rounded)
+
+What it keeps for the backward is Q(x^T): one byte per element (and 1 / 128) instead of two or four.
+Results in bf16 come from the matrix cores' scaled e4m3 instructions, results in fp32 (dW, and y / dx
+of fp32 activations) from exact bf16 copies of the codes (csrc/kernels/gemm_fp8.hip).
+
+int8 keeps what is used element by element (``bias_act(bits=8)``, ``pack8``): its error is a fixed
+fraction of the block's largest entry, 1/4 of e4m3's on normal data.
+
+Sites of the reference model: hetseq/bert_modeling.py:104-116 (bias_gelu), :334-336, :383, :409, :419
+(linear layers), :428-446 (checkpointed segments).
+"""
+import torch
+
+from . import fused
+from ._ext import C, use_kernels
+
+BLOCK = 128
+_DTYPES = (torch.float32, torch.bfloat16)
+
+
+def _check_act(x, what):
+    if not torch.is_tensor(x) or x.dtype not in _DTYPES:
+        raise TypeError('{}: an fp32 or bf16 tensor, got {}'.format(what, getattr(x, 'dtype', type(x).__name__)))
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError('{}: needs a last dimension of at least 1, got shape {}'.format(what, tuple(x.shape)))
+
+
+def _check_bias(b, n, like, what):
+    if b is None:
+        return
+    if b.dtype != torch.float32 or tuple(b.shape) != (n,) or b.device != like.device:
+        raise ValueError('{}: the bias must be fp32 [{}] on {}, got {} {} on {}'.format(
+            what, n, like.device, b.dtype, tuple(b.shape), b.device))
+
+
+# ---------------------------------------------------------------- references (CPU, and the numerics oracle)
+def _blocks_ref(x, largest):
+    """x / 2^e per block of the last dimension, and 2^e, as [..., blocks, 128] fp32."""
+    x = torch.nn.functional.pad(x.float(), (0, -x.shape[-1] % BLOCK)).unflatten(-1, (-1, BLOCK))
+    a = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x)).amax(-1, keepdim=True)
+    m, e = torch.frexp(a)   # a = m 2^e, m in [1/2, 1)
+    mt, et = torch.frexp(torch.tensor(float(largest)))
+    e = torch.where(a > 0, e - int(et) + (m > float(mt)).to(e.dtype), torch.zeros_like(e)).clamp(min=-126)
+    s = ((e + 127) << 23).view(torch.float32)
+    return x * ((127 - e) << 23).view(torch.float32), s
+
+
+def e4m3_ref(x):
+    """The values of x's e4m3 codes (blocks along the last dimension), fp32."""
+    v, s = _blocks_ref(x, 448.0)
+    q = torch.where(torch.isfinite(v), v, torch.zeros_like(v)).to(torch.float8_e4m3fn).float()
+    return torch.where(torch.isfinite(v), q * s, torch.full_like(v, float('nan'))).flatten(-2)[..., :x.shape[-1]]
+
+
+def int8_ref(x):
+    """The values of x's int8 codes (blocks along the last dimension), fp32."""
+    v, s = _blocks_ref(x, 127.0)
+    return torch.where(torch.isfinite(v), torch.round(v) * s, torch.full_like(v, float('nan'))).flatten(-2)[..., :x.shape[-1]]
+
+
+def _gelu_grad_ref(u):
+    c = 1.41421
+    return 0.5 * (1.0 + torch.erf(u / c)) + u * torch.exp(-(u / c) ** 2) / (c * 3.141592653589793 ** 0.5)
+
+
+# ---------------------------------------------------------------- operands
+class Fp8Weight(object):
+    """A weight's e4m3 codes for ``linear_fp8``: of W [N, K] blocked along K (the forward) and of W^T
+    blocked along N (the data gradient; ``grad=False`` leaves it out: inference).  A served model
+    builds it once; training builds it per forward (``fp8_scope`` does, for a whole encoder)."""
+    __slots__ = ('shape', 'dtype', 'device', 'q', 's', 'qt', 'st', 'ref')
+
+    def __init__(self, W, grad=True):
+        _check_act(W, 'Fp8Weight')
+        if W.dim() != 2 or W.shape[0] < 1:
+            raise ValueError('Fp8Weight: a non-empty [out, in] weight, got shape {}'.format(tuple(W.shape)))
+        W = W.detach()
+        self.shape, self.dtype, self.device = tuple(W.shape), W.dtype, W.device
+        self.q = self.s = self.qt = self.st = self.ref = None
+        if use_kernels(W):
+            self.q, self.s, self.qt, self.st, _ = C().split8(_rows2(W), True, bool(grad))
+        else:
+            self.ref = (e4m3_ref(W), e4m3_ref(W.t()) if grad else None)
+
+    @property
+    def has_grad(self):
+        return self.qt is not None or (self.ref is not None and self.ref[1] is not None)
+
+
+class _Scope(object):
+    weights = None      # {(data_ptr, shape): Fp8Weight} of the running forward
+
+
+class fp8_scope(object):
+    """``Fp8Weight`` copies of every weight in ``Ws`` for the running forward: ``linear_fp8`` finds
+    them by the weight; a recompute outside the scope builds its own."""
+
+    def __init__(self, Ws):
+        self.Ws = [W for W in Ws if W is not None]
+
+    def __enter__(self):
+        self.prev = _Scope.weights
+        _Scope.weights = {(W.data_ptr(), tuple(W.shape)): Fp8Weight(W) for W in self.Ws if use_kernels(W)}
+        return self
+
+    def __exit__(self, *exc):
+        _Scope.weights = self.prev
+        return False
+
+
+def _weight(W, grad):
+    if isinstance(W, Fp8Weight):
+        return W
+    if _Scope.weights is not None:
+        w = _Scope.weights.get((W.data_ptr(), tuple(W.shape)))
+        if w is not None:
+            return w
+    return Fp8Weight(W, grad)
+
+
+def _rows2(x):
+    """[.., K] as a 2-D operand with unit column stride (a contiguous copy if it has none)."""
+    x2 = x.reshape(-1, x.shape[-1])
+    ok = (x2.stride(1) == 1 or x2.shape[1] == 1) and (x2.stride(0) >= x2.shape[1] or x2.shape[0] <= 1)
+    return x2 if ok else x2.contiguous()
+
+
+# ---------------------------------------------------------------- linear
+class _LinearFp8Fn(torch.autograd.Function):
+    """One product over one weight, or over several stacked along the output features (Q / K / V).
+    ``params``: the n weights (or none: frozen), then their n biases (or none).  ``bias``: the
+    stacked bias added here; ``bgrad=False``: its gradient comes from the consumer."""
+
+    @staticmethod
+    def forward(ctx, x, w8, bias, mbox, bgrad, n, *params):
+        N, K = w8.shape
+        x2 = _rows2(x)
+        ctx.w8, ctx.mbox, ctx.xshape, ctx.n, ctx.bgrad = w8, mbox, x.shape, n, bgrad
+        ctx.Ws, ctx.bs = params[:n], params[n:]
+        # the weight gradient reads the 8-bit copy of x blocked along the tokens
+        keep = any(ctx.needs_input_grad[6:6 + n])
+        if use_kernels(x):
+            q, s, qt, st, _ = C().split8(x2, True, keep)
+            y = C().gemm_fp8(q, s, w8.q, w8.s, K, x.dtype == torch.bfloat16, bias=bias)
+        else:
+            y = e4m3_ref(x2) @ w8.ref[0].t()
+            y = (y if bias is None else y + bias).to(x.dtype)
+            qt, st = (e4m3_ref(x2.t()), None) if keep else (None, None)
+        ctx.save_for_backward(qt, st)
+        return y.view(*x.shape[:-1], N)
+
+    @staticmethod
+    def backward(ctx, dy):
+        xt, xs = ctx.saved_tensors
+        w8, n, Ws, bs = ctx.w8, ctx.n, ctx.Ws, ctx.bs
+        N, K = w8.shape
+        need_x = ctx.needs_input_grad[0]
+        need_w = any(ctx.needs_input_grad[6:6 + n])
+        need_b = ctx.bgrad and any(ctx.needs_input_grad[6 + n:])
+        dy2 = _rows2(dy)
+        M = dy2.shape[0]
+        if not use_kernels(dy):
+            dx = (e4m3_ref(dy2) @ w8.ref[1].t()).to(dy.dtype).view(ctx.xshape) if need_x else None
+            dW = e4m3_ref(dy2.t()) @ xt.t() if need_w else None
+            db = dy2.float().sum(0) if need_b else None
+            return (_residual(dx, ctx.mbox), None, None, None, None, None,
+                    *_parts(dW, Ws, None), *_parts(db, bs, None))
+        bslots, bview = _slots(bs) if need_b else (None, None)
+        q, s, qt, st, db = C().split8(dy2, need_x, need_w and M > 0, need_b, bview)
+        gW = (None,) * len(Ws)
+        if need_w:
+            slots, view = _slots(Ws)
+            side = fused.side_begin(dy2.device, M) if view is not None and M > 0 else None
+            with fused.side_ctx(side):
+                if M == 0:
+                    dW = view.zero_() if view is not None else torch.zeros(N, K, device=dy.device)
+                else:
+                    dW = C().gemm_fp8(qt, st, xt, xs, M, False, out=view)
+                gW = _parts(dW, Ws, slots, view is not None)
+            fused._record(side, qt, st, xt, xs)
+        dx = None
+        if need_x:
+            acc = other = None
+            if ctx.mbox is not None:
+                acc, other = ctx.mbox.take(dy.dtype)
+            acc = acc.view(M, K) if acc is not None else None
+            dx = C().gemm_fp8(q, s, w8.qt, w8.st, N, dy.dtype == torch.bfloat16, out=acc, beta=acc is not None).view(ctx.xshape)
+            if other is not None:
+                dx = dx + other.view(ctx.xshape).to(dx.dtype)
+        return (dx, None, None, None, None, None, *gW, *_parts(db, bs, bslots, bview is not None))
+
+
+def _slots(params):
+    """The parameters' flat gradient slots and, if all have one and they lie back to back, the one
+    view over them that a product writes directly."""
+    slots = [fused.grad_slot(p) for p in params]
+    if any(t is None for t in slots):
+        return slots, None
+    return slots, slots[0] if len(slots) == 1 else fused._adjacent_view(slots)
+
+
+def _parts(g, params, slots, direct=False):
+    """The stacked gradient ``g`` as one gradient per parameter (in its slot, where it has one)."""
+    if g is None:
+        return (None,) * len(params)
+    if direct:
+        return tuple(slots)
+    out, o = [], 0
+    for i, p in enumerate(params):
+        t = g[o:o + p.shape[0]].to(p.dtype)
+        o += p.shape[0]
+        if slots is not None and slots[i] is not None:
+            t = slots[i].copy_(t)
+        out.append(t)
+    return tuple(out)
+
+
+def _residual(dx, mbox):
+    if mbox is None or dx is None:
+        return dx
+    g, other = mbox.take(dx.dtype)
+    g = g if g is not None else other
+    return dx if g is None else dx + g.view(dx.shape).to(dx.dtype)
+
+
+def linear_fp8(x, W, b=None, res_grad=None):
+    """x W^T (+ b) with e4m3 operands (one power-of-two scale per block of 128; see the module's
+    formulas).  ``x`` [.., K] fp32 or bf16 (the result has its type); ``W`` [N, K] a parameter, or an
+    ``Fp8Weight`` (then it gets no gradient: inference, frozen layers); ``b`` fp32 [N].
+    ``res_grad``: see ``ResidualGrad``."""
+    _check_act(x, 'linear_fp8')
+    if not isinstance(W, Fp8Weight):
+        _check_act(W, 'linear_fp8 weight')
+        if W.dim() != 2 or W.shape[0] < 1:
+            raise ValueError('linear_fp8: a non-empty [out, in] weight, got shape {}'.format(tuple(W.shape)))
+    N, K = W.shape
+    if x.shape[-1] != K:
+        raise ValueError('linear_fp8: x has {} features, the weight takes {}'.format(x.shape[-1], K))
+    if x.device != W.device:
+        raise ValueError('linear_fp8: x on {}, the weight on {}'.format(x.device, W.device))
+    _check_bias(b, N, x, 'linear_fp8')
+    grad = torch.is_grad_enabled() and x.requires_grad
+    w8 = _weight(W, grad)
+    if grad and not w8.has_grad:
+        raise ValueError('linear_fp8: x needs a gradient, the Fp8Weight was built with grad=False')
+    if isinstance(W, Fp8Weight):
+        return _LinearFp8Fn.apply(x, w8, b, res_grad, True, 0, *(() if b is None else (b,)))
+    return _LinearFp8Fn.apply(x, w8, b, res_grad, True, 1, W, *(() if b is None else (b,)))
+
+
+def linear3_fp8(x, wq, wk, wv, bq, bk, bv, res_grad=None, bias_grad=True):
+    """``linear3`` on e4m3 operands: the Q / K / V projections as one product (N = 3H)."""
+    _check_act(x, 'linear3_fp8')
+    W = fused._adjacent_view([wq, wk, wv])
+    W = W if W is not None else torch.cat([wq.detach(), wk.detach(), wv.detach()], 0)
+    bs, bias = (), None
+    if bq is not None:
+        bs, bias = (bq, bk, bv), fused._adjacent_view([bq, bk, bv])
+        bias = bias if bias is not None else torch.cat([t.detach() for t in bs], 0)
+    _check_bias(bias, W.shape[0], x, 'linear3_fp8')
+    w8 = _weight(W, torch.is_grad_enabled() and x.requires_grad)
+    return _LinearFp8Fn.apply(x, w8, bias, res_grad, bool(bias_grad), 3, wq, wk, wv, *bs)
+
+
+# ---------------------------------------------------------------- bias + GELU with an int8 checkpoint
+class _BiasGelu8Fn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, b):
+        ctx.b = b
+        if use_kernels(y):
+            out, q, s = C().gelu8_fwd(y, b)
+            ctx.save_for_backward(q, s)
+        else:
+            u = y.float() if b is None else y.float() + b
+            out = fused.gelu_ref(u).to(y.dtype)
+            ctx.save_for_backward(int8_ref(y), None)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, s = ctx.saved_tensors
+        b, need_b = ctx.b, ctx.needs_input_grad[1]
+        if use_kernels(dout):
+            dy, db = C().gelu8_bwd(dout.contiguous(), q, s, b, need_b, fused.grad_slot(b) if need_b else None)
+            return dy, db
+        dy = dout.float() * _gelu_grad_ref(q if b is None else q + b)
+        return dy.to(dout.dtype), dy.reshape(-1, dy.shape[-1]).sum(0) if need_b else None
+
+
+def bias_gelu8(y, b):
+    """gelu(y + b); the backward reads y from int8 blocks (``bias_act(y, b, 'gelu', bits=8)``)."""
+    _check_act(y, 'bias_act(bits=8)')
+    _check_bias(b, y.shape[-1], y, 'bias_act(bits=8)')
+    return _BiasGelu8Fn.apply(y.contiguous(), b)
+
+
+# ---------------------------------------------------------------- kept activations
+class Packed8(object):
+    """A tensor kept as int8 blocks (``pack8``): codes [rows, blocks, 128], scale bytes [rows, blocks]."""
+    __slots__ = ('q', 's', 'shape', 'dtype')
+
+    def __init__(self, q, s, shape, dtype):
+        self.q, self.s, self.shape, self.dtype = q, s, tuple(shape), dtype
+
+    @property
+    def nbytes(self):
+        return self.q.numel() * self.q.element_size() + (self.s.numel() if self.s is not None else 0)
+
+
+def pack8(x):
+    """``x`` (fp32 or bf16) as int8 blocks along its last dimension: 1 + 1/128 bytes per element."""
+    _check_act(x, 'pack8')
+    x = x.detach()
+    if use_kernels(x):
+        q, s = C().pack8(x.contiguous())
+    else:
+        q, s = _pack8_ref(x)
+    return Packed8(q, s, x.shape, x.dtype)
+
+
+def _pack8_ref(x):
+    v, s = _blocks_ref(x.reshape(-1, x.shape[-1]), 127.0)
+    q = torch.where(torch.isfinite(v), torch.round(v), torch.full_like(v, -128.0))
+    return q.to(torch.int8).view(torch.uint8), (s.view(torch.int32) >> 23).to(torch.uint8).squeeze(-1)
+
+
+def unpack8(p):
+    """The values of a ``Packed8``, in its tensor's shape and type."""
+    if not isinstance(p, Packed8):
+        raise TypeError('unpack8: a Packed8 (ops.pack8), got {}'.format(type(p).__name__))
+    if use_kernels(p.q):
+        return C().unpack8(p.q, p.s, p.shape[-1], p.dtype == torch.bfloat16).view(p.shape)
+    c = p.q.view(torch.int8).float()
+    v = c * (p.s.to(torch.int32) << 23).view(torch.float32).unsqueeze(-1)
+    v = torch.where(c == -128, torch.full_like(v, float('nan')), v)
+    return v.flatten(-2)[..., :p.shape[-1]].to(p.dtype).view(p.shape)
+
+
+class _Anchor(torch.autograd.Function):
+    """A stand-in for x in the graph: its shape, type and gradient, one element of storage."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.new_zeros(()).expand(x.shape)
+
+    @staticmethod
+    def backward(ctx, g):
+        return g
+
+
+class _Restore8(torch.autograd.Function):
+    """x while the segment first runs, its decoded 8-bit copy when it is recomputed."""
+
+    @staticmethod
+    def forward(ctx, anchor, box):
+        return box.x.view_as(box.x) if box.x is not None else unpack8(box.kept)
+
+    @staticmethod
+    def backward(ctx, g):
+        return g, None
+
+
+class _Box(object):
+    __slots__ = ('x', 'kept')
+
+
+def checkpoint8(fn, x, *rest):
+    """``fn(x, *rest)`` keeping only ``x`` in 8 bits (``pack8``) and ``rest`` as it is: the forward runs
+    on ``x`` itself; the backward recomputes the segment from the decoded copy and passes x's
+    gradient straight through the rounding.  ``fn`` returns a tensor or a tuple of them."""
+    _check_act(x, 'checkpoint8')
+    if not torch.is_grad_enabled():
+        return fn(x, *rest)
+    from torch.utils.checkpoint import checkpoint
+    box = _Box()
+    box.x, box.kept = x.detach(), pack8(x)
+    try:
+        return checkpoint(lambda anchor, *r: fn(_Restore8.apply(anchor, box), *r), _Anchor.apply(x), *rest,
+                          use_reentrant=False)
+    finally:
+        box.x = None

@@ -447,8 +447,15 @@ class _BiasActFn(torch.autograd.Function):
         return dy, (dbias if has_bias else None), None
 
 
-def bias_act(y, bias, act):
-    """act(y + bias) -- LinearActivation's fused bias_gelu / bias_tanh (bert_modeling.py:104-116)."""
+def bias_act(y, bias, act, bits=None):
+    """act(y + bias) -- LinearActivation's fused bias_gelu / bias_tanh (bert_modeling.py:104-116).
+    ``bits=8`` (gelu): what the backward keeps of ``y`` is int8 with one power-of-two scale per 128
+    entries of a row (ops/fp8.py); the result is the same."""
+    if bits is not None:
+        if bits != 8 or act != 'gelu':
+            raise ValueError("bias_act: bits=8 goes with 'gelu', got bits={!r}, act={!r}".format(bits, act))
+        from .fp8 import bias_gelu8
+        return bias_gelu8(y, bias)
     if use_kernels(y) and y.shape[-1] % 4 == 0:
         return _BiasActFn.apply(y.contiguous(), bias, act)
     x = y if bias is None else y + bias

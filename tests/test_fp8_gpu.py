@@ -1,0 +1,389 @@
+"""8-bit operators on the GPU kernels against 64-bit formulas: e4m3 linear layers (forward, both
+gradient products, bias gradient), bias + GELU with an int8 checkpoint, kept activations."""
+import math
+
+import pytest
+import torch
+
+from hetseq_9cme_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+DT = {'fp32': torch.float32, 'bf16': torch.bfloat16}
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}   # half a rounding step, relative
+
+
+# ---------------------------------------------------------------- the formats, in 64 bits
+def pow2(e):
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def exponents(x, largest):
+    """[rows, blocks] block exponents of x [rows, n]."""
+    rows, n = x.shape
+    xp = torch.zeros(rows, -(-n // 128) * 128, dtype=torch.float64, device=x.device)
+    xp[:, :n] = torch.where(torch.isfinite(x), x.double().abs(), 0.0)
+    a = xp.view(rows, -1, 128).amax(-1)
+    m, e = torch.frexp(a / largest)
+    return torch.where(a > 0, e - (m == 0.5).to(e.dtype), torch.zeros_like(e)).clamp(min=-126)
+
+
+def scaled(x, largest):
+    e = exponents(x, largest)
+    s = pow2(e).repeat_interleave(128, 1)[:, :x.shape[1]]
+    return x.double() / s, s
+
+
+def e4m3(x):
+    v, s = scaled(x, 448.0)
+    step = pow2(torch.frexp(v.abs().clamp(min=2.0 ** -6))[1] - 4)
+    return torch.where(torch.isfinite(v), torch.round(v / step) * step * s, float('nan'))
+
+
+def int8(x):
+    v, s = scaled(x, 127.0)
+    return torch.where(torch.isfinite(v), torch.round(v) * s, float('nan'))
+
+
+def code_values(q, s, rows, n):
+    """The values of split8's codes q [rows, padded] with scale words s."""
+    sc = s.permute(1, 0, 2).reshape(s.shape[1], -1)[:rows, :-(-n // 128)]
+    v = q.view(torch.float8_e4m3fn).double() * pow2(sc.int() - 127).repeat_interleave(128, 1)
+    return v[:, :n], v[:, n:]
+
+
+def rand(shape, dtype, seed, spread=1.0):
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    x = torch.randn(*shape, generator=g, device='cuda') * torch.exp(spread * torch.randn(shape[-1], generator=g, device='cuda'))
+    return x.to(dtype)
+
+
+def assert_product(got, a, b, extra=None, bias=None):
+    """got = a b^T (+ bias) (+ extra) for exact operand values a, b (64 bits).
+
+    fp32 results: bf16 matrix products of exact copies, 16 products per step, each step's sum rounded
+    to fp32 and one rounding per slab / epilogue term: (K / 16 + 8) steps of 2^-23 (truncation counts
+    double) of sum |a||b|.  bf16 results: half a bf16 step of the value, and the e4m3 instruction's
+    own 2^-11 of sum |a||b| (it keeps about 12 bits below the largest product of a group)."""
+    ref, mag = a @ b.t(), a.abs() @ b.abs().t()
+    if bias is not None:
+        ref, mag = ref + bias.double(), mag + bias.double().abs()
+    if extra is not None:
+        ref, mag = ref + extra.double(), mag + extra.double().abs()
+    K = a.shape[1]
+    if got.dtype == torch.float32:
+        tol = (K / 16 + 8) * 2.0 ** -23 * mag
+    else:
+        tol = HALF[got.dtype] * ref.abs() + 2.0 ** -11 * mag * (1 + 2.0 ** -8)
+    err = (got.double() - ref).abs()
+    bad = err > tol + 1e-37
+    assert not bad.any(), 'off by {:.3g} where {:.3g} is allowed, at {}'.format(
+        (err - tol).max().item(), tol.flatten()[(err - tol).argmax()].item(), bad.nonzero()[:4].tolist())
+
+
+# ---------------------------------------------------------------- operand copies
+@pytest.mark.parametrize('dt', ['fp32', 'bf16'])
+@pytest.mark.parametrize('R,C', [(1, 1), (1, 128), (3, 130), (127, 129), (128, 128), (130, 1000), (513, 777), (7, 4096)])
+def test_split8_codes_exact(dev, R, C, dt):
+    x = rand((R, C), DT[dt], R * 7 + C, 2.0)
+    x[0, 0] = 0.0
+    if R > 2:
+        x[1] = 0.0            # whole blocks of zeros
+        x[2, : C // 2] *= 2.0 ** -40
+    q, s, qt, st, sm = ops.C().split8(x, True, True, True)
+    v, pad = code_values(q, s, R, C)
+    assert torch.equal(v, e4m3(x)) and not pad.any()
+    v, pad = code_values(qt, st, C, R)
+    assert torch.equal(v, e4m3(x.t().contiguous())) and not pad.any()
+    ref = x.double().sum(0)
+    assert ((sm.double() - ref).abs() <= (R + 8) * 2.0 ** -24 * x.double().abs().sum(0)).all()
+
+
+@pytest.mark.parametrize('dt', ['fp32', 'bf16'])
+def test_split8_border_values(dev, dt):
+    top = torch.finfo(DT[dt]).max
+    tiny = torch.finfo(DT[dt]).tiny
+    vals = [[448.0], [449.0 if dt == 'fp32' else 450.0], [447.0, 1e-3], [0.0], [top, 1.0], [tiny, -tiny / 2], [tiny / 8],
+            [1.0, 2.0 ** -9, 2.0 ** -10, 1.5 * 2.0 ** -10], [-448.0 * 2.0 ** -30, 2.0 ** -33]]
+    x = torch.zeros(len(vals), 130, device=dev)
+    for i, v in enumerate(vals):
+        x[i, :len(v)] = torch.tensor(v)
+    x = x.to(DT[dt])
+    q, s, _, _, _ = ops.C().split8(x, True, False)
+    assert torch.equal(code_values(q, s, x.shape[0], 130)[0], e4m3(x))
+
+
+@pytest.mark.parametrize('dt', ['fp32', 'bf16'])
+def test_split8_nonfinite(dev, dt):
+    x = rand((130, 260), DT[dt], 3)
+    x[5, 7], x[5, 200], x[9, 0], x[129, 259] = float('inf'), float('nan'), float('-inf'), float('nan')
+    q, s, qt, st, _ = ops.C().split8(x, True, True)
+    for got, ref in ((code_values(q, s, 130, 260)[0], e4m3(x)), (code_values(qt, st, 260, 130)[0], e4m3(x.t().contiguous()))):
+        assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.isnan(ref).sum() == 4
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(ref))
+
+
+def test_split8_row_stride(dev):
+    x = rand((200, 600), torch.bfloat16, 11)
+    for v in (x[:, 8:390], x[:, 3:131], x[::3, :257]):
+        q, s, qt, st, sm = ops.C().split8(v, True, True, True)
+        r = ops.C().split8(v.contiguous(), True, True, True)
+        for a, b in ((code_values(q, s, *v.shape), code_values(r[0], r[1], *v.shape)),
+                     (code_values(qt, st, *v.t().shape), code_values(r[2], r[3], *v.t().shape))):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[0], a[0].nan_to_num())
+        assert torch.equal(sm, r[4])
+
+
+# ---------------------------------------------------------------- linear layers
+SHAPES = [(1, 1, 1), (1, 768, 130), (2, 127, 64), (17, 129, 33), (41, 1024, 96), (64, 128, 128), (65, 384, 257),
+          (130, 513, 1001), (300, 640, 128), (1312, 256, 768), (2100, 300, 100), (700, 2304, 520), (4100, 128, 1030)]
+
+
+@pytest.mark.parametrize('dt', ['fp32', 'bf16'])
+@pytest.mark.parametrize('M,K,N', SHAPES)
+def test_linear_fp8(dev, M, K, N, dt):
+    x = rand((M, K), DT[dt], M + K, 0.8).requires_grad_(True)
+    W = (rand((N, K), torch.float32, N) * 0.02).requires_grad_(True)
+    b = rand((N,), torch.float32, 5).requires_grad_(True)
+    dy = rand((M, N), DT[dt], 9, 1.0) * 1e-3
+    y = ops.linear_fp8(x, W, b)
+    dx, dW, db = torch.autograd.grad(y, (x, W, b), dy)
+    assert (y.dtype, dx.dtype, dW.dtype, db.dtype) == (x.dtype, x.dtype, torch.float32, torch.float32)
+    with torch.no_grad():
+        assert_product(y, e4m3(x), e4m3(W), bias=b)
+        assert_product(dx, e4m3(dy), e4m3(W.t().contiguous()))
+        assert_product(dW, e4m3(dy.t().contiguous()), e4m3(x.t().contiguous()))
+        assert ((db.double() - dy.double().sum(0)).abs() <= (M + 8) * 2.0 ** -24 * dy.double().abs().sum(0)).all()
+
+
+@pytest.mark.parametrize('dt', ['fp32', 'bf16'])
+@pytest.mark.parametrize('M,K,N', [(1, 768, 2304), (5, 130, 33), (33, 1024, 1001), (64, 4096, 128), (129, 96, 64), (3000, 256, 512)])
+def test_linear_fp8_kept_weight(dev, M, K, N, dt):
+    x, W, b = rand((M, K), DT[dt], 1), rand((N, K), torch.float32, 2) * 0.02, rand((N,), torch.float32, 3)
+    w8 = ops.Fp8Weight(W, grad=False)
+    with torch.no_grad():
+        assert_product(ops.linear_fp8(x, w8, b), e4m3(x), e4m3(W), bias=b)
+        assert_product(ops.linear_fp8(x, w8), e4m3(x), e4m3(W))
+
+
+def test_linear_fp8_shapes_and_strides(dev):
+    x = rand((6, 40, 256), torch.bfloat16, 1)
+    W = rand((192, 256), torch.float32, 2) * 0.02
+    y = ops.linear_fp8(x, W)
+    assert y.shape == (6, 40, 192)
+    assert torch.equal(ops.linear_fp8(x[2, 3], W), y[2, 3])
+    assert torch.equal(ops.linear_fp8(x[:, 3], W), y[:, 3])
+    assert torch.equal(ops.linear_fp8(x.transpose(0, 1), W), y.transpose(0, 1))
+    wide = torch.cat([x, x], -1)
+    assert torch.equal(ops.linear_fp8(wide[..., 256:], W), y)
+    # a broadcast output gradient, and a transposed one
+    xg = x.clone().requires_grad_(True)
+    one = torch.full((), 0.5, dtype=torch.bfloat16, device=dev)
+    g1, = torch.autograd.grad(ops.linear_fp8(xg, W), xg, one.expand(6, 40, 192))
+    g2, = torch.autograd.grad(ops.linear_fp8(xg, W), xg, torch.full((6, 40, 192), 0.5, dtype=torch.bfloat16, device=dev))
+    assert torch.equal(g1, g2)
+    d = rand((40, 6, 192), torch.bfloat16, 4).transpose(0, 1)
+    g1, = torch.autograd.grad(ops.linear_fp8(xg, W), xg, d)
+    g2, = torch.autograd.grad(ops.linear_fp8(xg, W), xg, d.contiguous())
+    assert torch.equal(g1, g2)
+
+
+def test_linear_fp8_no_tokens(dev):
+    x = torch.zeros(0, 256, device=dev, dtype=torch.bfloat16, requires_grad=True)
+    W = torch.randn(64, 256, device=dev, requires_grad=True)
+    b = torch.randn(64, device=dev, requires_grad=True)
+    y = ops.linear_fp8(x, W, b)
+    assert y.shape == (0, 64)
+    dx, dW, db = torch.autograd.grad(y, (x, W, b), torch.zeros(0, 64, device=dev, dtype=torch.bfloat16))
+    assert dx.shape == (0, 256) and not dW.any() and not db.any()
+
+
+def test_linear_fp8_residual_gradient(dev):
+    for dt in (torch.float32, torch.bfloat16):
+        x = rand((130, 256), dt, 1).requires_grad_(True)
+        W = rand((192, 256), torch.float32, 2) * 0.02
+        dy, res = rand((130, 192), dt, 3), rand((130, 256), dt, 4)
+        mbox = ops.ResidualGrad()
+        y = ops.linear_fp8(x, W, res_grad=mbox)
+        assert mbox.deposit(res.clone())
+        dx, = torch.autograd.grad(y, x, dy)
+        assert_product(dx, e4m3(dy), e4m3(W.t().contiguous()), extra=res)
+
+
+def test_linear_fp8_nonfinite_reaches_the_rows_that_read_it(dev):
+    x = rand((200, 256), torch.bfloat16, 1)
+    W = (rand((192, 256), torch.float32, 2) * 0.02).requires_grad_(True)
+    x[7, 3], x[150, 200] = float('inf'), float('nan')
+    x.requires_grad_(True)
+    y = ops.linear_fp8(x, W)
+    bad = torch.zeros(200, dtype=torch.bool, device=dev)
+    bad[[7, 150]] = True
+    assert torch.equal(torch.isnan(y).any(1), bad) and torch.isnan(y[7]).all()
+    dW, = torch.autograd.grad(y, W, torch.ones_like(y))
+    cols = torch.zeros(256, dtype=torch.bool, device=dev)
+    cols[[3, 200]] = True
+    assert torch.equal(torch.isnan(dW).all(0), cols) and torch.equal(torch.isnan(dW).any(0), cols)
+
+
+def test_linear3_fp8(dev):
+    x = rand((150, 128), torch.bfloat16, 1).requires_grad_(True)
+    ws = [(rand((128, 128), torch.float32, 2 + i) * 0.02).requires_grad_(True) for i in range(3)]
+    bs = [rand((128,), torch.float32, 7 + i).requires_grad_(True) for i in range(3)]
+    dy = rand((150, 384), torch.bfloat16, 20)
+    y = ops.linear3_fp8(x, *ws, *bs)
+    gs = torch.autograd.grad(y, [x] + ws + bs, dy)
+    x1, W, b = x.detach().clone().requires_grad_(True), torch.cat(ws).detach().requires_grad_(True), torch.cat(bs).detach().requires_grad_(True)
+    y1 = ops.linear_fp8(x1, W, b)
+    r = torch.autograd.grad(y1, (x1, W, b), dy)
+    assert torch.equal(y, y1) and torch.equal(gs[0], r[0])
+    assert torch.equal(torch.cat(gs[1:4]), r[1]) and torch.equal(torch.cat(gs[4:]), r[2])
+
+
+# ---------------------------------------------------------------- bias + GELU
+def gelu64(u):
+    return u * 0.5 * (1 + torch.special.erf(u / 1.41421))
+
+
+def gelu_slope64(u):
+    c = 1.41421
+    return 0.5 * (1 + torch.special.erf(u / c)) + u * torch.exp(-(u / c) ** 2) / (c * math.sqrt(math.pi))
+
+
+@pytest.mark.parametrize('bias', [True, False])
+@pytest.mark.parametrize('dt', ['fp32', 'bf16'])
+@pytest.mark.parametrize('rows,N', [(1, 1), (1, 128), (3, 129), (64, 1001), (65, 512), (130, 4096), (1000, 72)])
+def test_bias_gelu8(dev, rows, N, dt, bias):
+    y = (2 * rand((rows, N), DT[dt], rows + N, 0.5)).requires_grad_(True)
+    b = (0.3 * rand((N,), torch.float32, 2)).requires_grad_(True) if bias else None
+    d = rand((rows, N), DT[dt], 4)
+    out = ops.bias_act(y, b, 'gelu', bits=8)
+    g = torch.autograd.grad(out, (y, b) if bias else (y,), d)
+    with torch.no_grad():
+        b64 = b.double() if bias else 0.0
+        u, v, d64 = y.double() + b64, int8(y) + b64, d.double()
+        # erfc to 1.5e-7 and a few fp32 steps of |u|; the slope the same plus the exponential's argument
+        # error (z^2 up to 16 before the bell underflows what matters: 16 steps of 2^-24)
+        tol = HALF[y.dtype] * gelu64(u).abs() + (2e-7 + 4 * 2.0 ** -24) * u.abs()
+        assert ((out.double() - gelu64(u)).abs() <= tol * (1 + 2.0 ** -7)).all()
+        ref = d64 * gelu_slope64(v)
+        tol = HALF[y.dtype] * ref.abs() + d64.abs() * (4e-7 + 20 * 2.0 ** -24 + 4 * 2.0 ** -24 * v.abs())
+        assert ((g[0].double() - ref).abs() <= tol * (1 + 2.0 ** -7)).all()
+        if bias:
+            t = (d64.abs() * (4e-7 + 24 * 2.0 ** -24 + 4 * 2.0 ** -24 * v.abs())).sum(0) + (rows + 8) * 2.0 ** -24 * ref.abs().sum(0)
+            assert ((g[1].double() - ref.sum(0)).abs() <= t).all()
+
+
+def test_bias_gelu8_keeps_one_byte(dev):
+    y = rand((300, 640), torch.bfloat16, 1).requires_grad_(True)
+    b = rand((640,), torch.float32, 2)
+    base = torch.cuda.memory_allocated()
+    out = ops.bias_act(y, b, 'gelu', bits=8)
+    kept = torch.cuda.memory_allocated() - base - out.numel() * 2
+    assert kept <= 300 * 640 + 300 * 5 + 2048     # codes, scale bytes, allocator rounding
+
+
+# ---------------------------------------------------------------- kept activations
+@pytest.mark.parametrize('dt', ['fp32', 'bf16'])
+@pytest.mark.parametrize('shape', [(1,), (128,), (3, 129), (2, 5, 768), (7, 1001), (1312, 768)])
+def test_pack8_exact(dev, shape, dt):
+    x = rand(shape, DT[dt], 3, 1.0)
+    p = ops.pack8(x)
+    got = ops.unpack8(p)
+    assert got.shape == x.shape and got.dtype == x.dtype
+    assert torch.equal(got.double(), int8(x.reshape(-1, shape[-1])).view(shape))
+    assert p.nbytes == (x.numel() // shape[-1]) * -(-shape[-1] // 128) * 129
+
+
+def test_pack8_border_and_nonfinite(dev):
+    x = torch.zeros(6, 130, device=dev)
+    x[0, :3] = torch.tensor([127.0, 0.5, 1.5])
+    x[1, :2] = torch.tensor([127.01, -127.01])
+    x[2, :3] = torch.tensor([float('inf'), float('nan'), 3.0])
+    x[3, 0] = torch.finfo(torch.float32).max
+    x[4, 0] = 1e-45
+    x[5, 129] = float('-inf')
+    # the value 64 2^122 of the largest fp32 number rounds to infinity in fp32, as 2^128 does
+    got, ref = ops.unpack8(ops.pack8(x)), int8(x).float()
+    assert torch.isinf(ref[3, 0]) and torch.isnan(ref).sum() == 3
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(got.nan_to_num(7.0), ref.nan_to_num(7.0))
+
+
+def test_pack8_no_rows_and_strides(dev):
+    e = ops.unpack8(ops.pack8(torch.zeros(0, 5, device=dev)))
+    assert e.shape == (0, 5)
+    x = rand((40, 300), torch.float32, 1)
+    assert torch.equal(ops.unpack8(ops.pack8(x[::2, 1:200])), ops.unpack8(ops.pack8(x[::2, 1:200].contiguous())))
+
+
+def test_checkpoint8(dev):
+    x = rand((50, 128), torch.float32, 1).requires_grad_(True)
+    W = (rand((128, 128), torch.float32, 2) * 0.05).requires_grad_(True)
+    f = lambda t, k: torch.tanh(t @ W) * k
+    out = ops.checkpoint8(f, x, 3.0)
+    assert torch.equal(out, f(x, 3.0))          # the forward runs on x itself
+    d = rand((50, 128), torch.float32, 4)
+    gx, gw = torch.autograd.grad(out, (x, W), d)
+    xh = ops.unpack8(ops.pack8(x)).requires_grad_(True)
+    rx, rw = torch.autograd.grad(f(xh, 3.0), (xh, W), d)
+    assert torch.equal(gx, rx) and torch.equal(gw, rw)
+
+
+# ---------------------------------------------------------------- streams, graphs, together
+def layer(x, w8, b1, w2, b2):
+    return ops.linear_fp8(ops.bias_act(ops.linear_fp8(x, w8), b1, 'gelu', bits=8), w2, b2)
+
+
+def test_another_stream(dev):
+    x = rand((700, 256), torch.bfloat16, 1)
+    W = rand((512, 256), torch.float32, 2) * 0.02
+    ref = ops.linear_fp8(x, W)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        got = ops.linear_fp8(x, W)
+    torch.cuda.current_stream().wait_stream(st)
+    assert torch.equal(got, ref)
+
+
+def test_training_pass_captured_and_replayed(dev):
+    """Forward and backward of FFN-shaped layers in a HIP graph: every replay on new inputs equals the
+    eager pass, with eager work between the replays."""
+    W1 = (rand((512, 256), torch.float32, 1) * 0.03).requires_grad_(True)
+    W2 = (rand((256, 512), torch.float32, 2) * 0.03).requires_grad_(True)
+    b1, b2 = (rand((n,), torch.float32, n).requires_grad_(True) for n in (512, 256))
+    x = rand((333, 256), torch.bfloat16, 3).requires_grad_(True)
+    d = rand((333, 256), torch.bfloat16, 4)
+    leaves = (x, W1, b1, W2, b2)
+
+    def step():
+        y = layer(x, W1, b1, W2, b2)
+        return (y,) + torch.autograd.grad(y, leaves, d)
+
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(rand((333, 256), torch.bfloat16, 30 + i))
+            d.copy_(rand((333, 256), torch.bfloat16, 40 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), i
+
+
+def test_results_repeat_bit_for_bit(dev):
+    x = rand((5000, 384), torch.bfloat16, 1).requires_grad_(True)
+    W = (rand((200, 384), torch.float32, 2) * 0.02).requires_grad_(True)
+    d = rand((5000, 200), torch.bfloat16, 3)
+    first = torch.autograd.grad(ops.linear_fp8(x, W), (x, W), d)
+    for _ in range(3):
+        for a, b in zip(first, torch.autograd.grad(ops.linear_fp8(x, W), (x, W), d)):
+            assert torch.equal(a, b)
