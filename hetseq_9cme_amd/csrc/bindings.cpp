@@ -832,8 +832,8 @@ Tensor gemm_fp8(Tensor a, Tensor as, Tensor b, Tensor bs, int64_t K, bool out_bf
   g.N = (int)N;
   g.nkb = (int)nkb;
   g.beta = beta ? 1 : 0;
-  const int cfg = hx_gemm_fp8_plan(g.M, g.N);
-  g.ks = hx_gemm_fp8_ks(g.M, g.N, g.nkb, cfg);
+  int cfg = 0;
+  hx_gemm_fp8_plan(g.M, g.N, g.nkb, out_bf16 ? 0 : 1, &cfg, &g.ks);
   g.vec = aligned16(g.C) && g.ldc * es % 16 == 0 && N * es % 16 == 0;
   Tensor part;
   if (g.ks > 1) {

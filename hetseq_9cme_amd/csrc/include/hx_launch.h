@@ -265,8 +265,7 @@ struct HxGemm8 {
   const float* bias;
   int M, N, nkb, beta, ks, vec;   // vec: C rows allow 16-B stores and N is a whole number of them
 };
-int hx_gemm_fp8_plan(int M, int N);
-int hx_gemm_fp8_ks(int M, int N, int nkb, int cfg);
+void hx_gemm_fp8_plan(int M, int N, int nkb, int exact, int* cfg, int* ks);   // tile configuration, split-K slabs
 int hx_gemm_fp8(const HxGemm8& g, int cfg, int exact, int out_bf16, hipStream_t s);
 void hx_gemm_fp8_slabs(const float* part, void* out, int out_bf16, int64_t ldc, int M, int N, int ks, const float* bias,
                        int beta, int vec, hipStream_t s);

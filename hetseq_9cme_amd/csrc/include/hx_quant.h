@@ -79,7 +79,12 @@ __device__ __forceinline__ void load8<uint16_t>(const uint16_t* p, float (&v)[8]
     v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
   }
 }
-__device__ __forceinline__ uint32_t bf16x2(float a, float b) { return f2bf(a) | ((uint32_t)f2bf(b) << 16); }
+// two fp32 values -> packed bf16 (one v_cvt_pk_bf16_f32: nearest even, NaN kept)
+__device__ __forceinline__ uint32_t bf16x2(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, b16x2));
+}
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]);
 template <>

@@ -56,8 +56,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) *
   constexpr int RPP = 1024 / KS;                       // rows per 1-KiB DMA piece
   constexpr int KA = BM / RPP, KB = BN / RPP, J = (KA + KB) / NW;
   static_assert((KA + KB) % NW == 0 && BM % RPP == 0 && BN % RPP == 0, "whole DMA pieces per wave");
-  static_assert(BM <= 256 && BN <= 256 && NW >= 2, "one DMA piece of scale words per operand");
-  constexpr int STAGE = (BM + BN) * KS, SCALES = NS * STAGE;   // + 2 slots x (A, B, spare) x 1 KiB
+  static_assert(BM <= 256 && BN <= 256 && NW >= 3, "one DMA piece of scale words per operand");
+  constexpr int STAGE = (BM + BN) * KS, SCALES = NS * STAGE;   // + 2 slots x (A, B) x 1 KiB
+  constexpr int BIAS = SCALES + 4096, SPARE = BIAS + 1024;      // the tile's bias; where idle pieces land
   extern __shared__ __attribute__((aligned(16))) char lds[];
 
   const int TM = (g.M + BM - 1) / BM, TN = (g.N + BN - 1) / BN, total = TM * TN;
@@ -79,8 +80,11 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) *
   const u32x4 ra = rsrc_of(g.A + (int64_t)m0 * g.lda, (uint32_t)(mrows * g.lda));
   const u32x4 rb = rsrc_of(g.B + (int64_t)n0 * g.ldb, (uint32_t)(nrows * g.ldb));
   const int64_t sam = (g.M + 3) & ~3, sbn = (g.N + 3) & ~3;
-  const u32x4 rsa = rsrc_of(g.sa + m0, (uint32_t)((groups * sam - m0) * 4));
-  const u32x4 rsb = rsrc_of(g.sb + n0, (uint32_t)((groups * sbn - n0) * 4));
+  // wave 0 fetches the scale words of A's rows, wave 1 B's, wave 2 the bias
+  const char* xp = (const char*)(wv == 0 ? (const void*)(g.sa + m0) : wv == 1 ? (const void*)(g.sb + n0) : (const void*)(g.bias + n0));
+  const uint32_t xbytes = wv == 0 ? (uint32_t)((groups * sam - m0) * 4) : wv == 1 ? (uint32_t)((groups * sbn - n0) * 4)
+                          : wv == 2 && g.bias ? (uint32_t)(g.N - n0) * 4 : 0u;
+  const u32x4 rx = rsrc_of(xp, xbytes);
   const uint32_t lds0 = (uint32_t)(size_t)(lds_void*)lds;
 
   // lane L of a DMA piece fetches (row L / (KS / 16), 16-B chunk c) so that the lane-linear LDS
@@ -94,26 +98,26 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) *
   }
   constexpr int SPB = 128 / KS;   // stages per k block
   const int st1 = (kb1 - kb0) * SPB;
-  auto dma = [&](int st) {
+  auto dma_one = [&](int st, int j) {   // piece j of this wave for stage st
     // past the slab's end: an offset past every buffer (zeros, no memory traffic, still counted)
     const uint32_t ko = st < st1 ? (uint32_t)(kb0 * 128 + st * KS) : 0x80000000u;
-    const uint32_t base = lds0 + (uint32_t)(st % NS) * STAGE;
+    const int q = wv + NW * j;
+    dma16(q < KA ? ra : rb, lds0 + (uint32_t)(st % NS) * STAGE + 1024u * q, voff[j] + ko);
+  };
+  auto dma = [&](int st) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int q = wv + NW * j;
-      dma16(q < KA ? ra : rb, base + 1024u * q, voff[j] + ko);
-    }
+    for (int j = 0; j < J; ++j) dma_one(st, j);
   };
-  auto dma_scales = [&](int grp) {   // scale words of k blocks 4 grp .. + 3: wave 0 A's rows, wave 1 B's
-    const uint32_t dst = lds0 + SCALES + (uint32_t)(grp & 1) * 3072 + (wv == 0 ? 0 : wv == 1 ? 1024 : 2048);
-    const uint32_t off = wv < 2 && grp < groups ? (uint32_t)(grp * (wv == 0 ? sam : sbn) * 4) + 16 * lane : 0x80000000u;
-    dma16(wv == 0 ? rsa : rsb, dst, off);
+  auto dma_scales = [&](int grp, bool first) {   // scale words of k blocks 4 grp .. + 3 (and, first, the bias)
+    const uint32_t dst = wv < 2 ? SCALES + (uint32_t)(grp & 1) * 2048 + wv * 1024 : first && wv == 2 ? BIAS : SPARE;
+    const uint32_t off = wv < 2 ? (uint32_t)(grp * (wv == 0 ? sam : sbn) * 4) : 0u;
+    const bool some = wv < 2 ? grp < groups : first;
+    dma16(rx, lds0 + dst, (some ? off : 0x80000000u) + 16 * lane);
   };
-  auto open = [&](int st) {   // stage st readable by every wave; the slot of stage st - 1 refilled
+  auto open = [&]() {   // the oldest stage in flight readable by every wave, the stage before it free
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     dma_wait<(NS - 2) * J>();
     raw_barrier();
-    dma(st - 1 + NS);
   };
 
   f32x16 acc[MB][NB];
@@ -122,9 +126,6 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) *
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[a][b] = f32x16{0};
 
-  struct Fr {
-    i32x8 a[MB], b[NB];
-  };
   auto frag = [&](const char* st, int row, int half) {
     const int r = row + l32;
     const char* p = st + r * KS;
@@ -133,127 +134,160 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) *
     const i32x4 hi = *reinterpret_cast<const i32x4*>(p + 16 * ((4 * half + 2 + h) ^ sw));
     return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
-  auto read = [&](int st, int half, Fr& F) {
-    const char* p = lds + (st % NS) * STAGE;
+  i32x8 fa[MB], fb[2][NB];   // A's fragments are read again as soon as their MFMAs are issued, B's by turns
+  auto read_a = [&](int st, int half, int a) { fa[a] = frag(lds + (st % NS) * STAGE, wm * WM + 32 * a, half); };
+  auto read_b = [&](int st, int half, i32x8 (&f)[NB]) {
 #pragma unroll
-    for (int a = 0; a < MB; ++a) F.a[a] = frag(p, wm * WM + 32 * a, half);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) F.b[b] = frag(p + BM * KS, wn * WN + 32 * b, half);
+    for (int b = 0; b < NB; ++b) f[b] = frag(lds + (st % NS) * STAGE + BM * KS, wn * WN + 32 * b, half);
   };
   uint32_t wa[MB], wb[NB];   // scale words, the current block's byte lowest
   auto read_scales = [&](int grp) {
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(lds + SCALES + (grp & 1) * 3072);
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(lds + SCALES + (grp & 1) * 2048);
 #pragma unroll
     for (int a = 0; a < MB; ++a) wa[a] = p[wm * WM + 32 * a + l32];
 #pragma unroll
     for (int b = 0; b < NB; ++b) wb[b] = p[256 + wn * WN + 32 * b + l32];
   };
-  // rows of the result run along n (the first MFMA operand), so a lane holds 4 consecutive columns
-  auto mma = [&](const Fr& F) {
-    if constexpr (!EXACT) {
+  // The MFMAs of one half, and between them the reads of the next half's fragments (stage st, half
+  // `half`; OPEN: a new stage) and the DMA pieces of stage dst -- one after the other as written: a
+  // wave that issued its reads first would hold its MFMAs back until the LDS had served all waves'
+  // reads.  The stage is opened under the first MFMAs.
+  // Rows of the result run along n (the first MFMA operand): a lane holds 4 consecutive columns.
+  auto half_step = [&](const i32x8 (&bc)[NB], i32x8 (&bn)[NB], int st, int half, auto open_it, int dst) {
+    constexpr bool OPEN = decltype(open_it)::value;
+    bf16x8v db[4][NB];
+    if constexpr (EXACT)
 #pragma unroll
-      for (int a = 0; a < MB; ++a)
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) db[q][b] = decode8(bc[b][2 * q], bc[b][2 * q + 1], hx::q8::scale_of(wb[b] & 0xffu));
+#pragma unroll
+    for (int a = 0; a < MB; ++a) {
+      if constexpr (!EXACT) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
-          acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(F.b[b], F.a[a], acc[a][b], 0, 0, 0, wb[b], 0, wa[a]);
-    } else {
+          acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bc[b], fa[a], acc[a][b], 0, 0, 0, wb[b], 0, wa[a]);
+      } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        bf16x8v fb[NB];
+        for (int q = 0; q < 4; ++q) {
+          const bf16x8v da = decode8(fa[a][2 * q], fa[a][2 * q + 1], hx::q8::scale_of(wa[a] & 0xffu));
 #pragma unroll
-        for (int b = 0; b < NB; ++b) fb[b] = decode8(F.b[b][2 * q], F.b[b][2 * q + 1], hx::q8::scale_of(wb[b] & 0xffu));
-#pragma unroll
-        for (int a = 0; a < MB; ++a) {
-          const bf16x8v fa = decode8(F.a[a][2 * q], F.a[a][2 * q + 1], hx::q8::scale_of(wa[a] & 0xffu));
-#pragma unroll
-          for (int b = 0; b < NB; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[b], fa, acc[a][b], 0, 0, 0);
+          for (int b = 0; b < NB; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(db[q][b], da, acc[a][b], 0, 0, 0);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      if (a == 0) {
+        if constexpr (OPEN) open();
+        read_b(st, half, bn);
+      }
+      read_a(st, half, a);
+      if constexpr (OPEN)
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (j * MB / J == a) dma_one(dst, j);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
   if (kb0 < kb1) {
-    dma_scales(kb0 / 4);
+    dma_scales(kb0 / 4, true);
 #pragma unroll
     for (int i = 0; i < NS; ++i) dma(i);
     dma_wait<(NS - 1) * J>();   // the scale words and stage 0 landed
     raw_barrier();
-    Fr F0, F1;
-    read(0, 0, F0);
+    read_b(0, 0, fb[0]);
+#pragma unroll
+    for (int a = 0; a < MB; ++a) read_a(0, 0, a);
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
     for (int kb = kb0; kb < kb1; ++kb) {
       if ((kb & 3) == 0) {
         read_scales(kb >> 2);
-        dma_scales((kb >> 2) + 1);
+        dma_scales((kb >> 2) + 1, false);
       } else {
 #pragma unroll
         for (int a = 0; a < MB; ++a) wa[a] >>= 8;
 #pragma unroll
         for (int b = 0; b < NB; ++b) wb[b] >>= 8;
       }
-      const int st = (kb - kb0) * SPB;
+      const int st = (kb - kb0) * SPB;   // (past the end a stale slot is read, and not used)
       if constexpr (SPB == 2) {
-        open(st + 1);
-        read(st + 1, 0, F1);
+        half_step(fb[0], fb[1], st + 1, 0, yes, st + NS);
+        half_step(fb[1], fb[0], st + 2, 0, yes, st + 1 + NS);
       } else {
-        read(st, 1, F1);
+        half_step(fb[0], fb[1], st, 1, no, 0);
+        half_step(fb[1], fb[0], st + 1, 0, yes, st + NS);
       }
-      mma(F0);
-      open(st + SPB);   // (past the end: a stale slot is read, and not used)
-      read(st + SPB, 0, F0);
-      mma(F1);
     }
   }
-  dma_wait<0>();
-  __syncthreads();
+  dma_wait<0>();   // no DMA piece may land after the workgroup's LDS has been given away
 
-  // ---- epilogue: 32 rows of the wave's tile at a time through its own piece of LDS, 16-B row stores
+  // ---- epilogue: a lane holds 4 consecutive columns of a row per quad of registers, the other half
+  // wave the next 4; bf16 quads change places in pairs so that every store is 16 B per lane
   using OutT = std::conditional_t<OB, uint16_t, float>;
-  constexpr int ES = OB ? 2 : 4, RS = WN * ES + 16;
-  static_assert(NW * 32 * RS <= NS * STAGE, "staging fits the stages");
-  char* my = lds + wv * 32 * RS;
   OutT* C = (OutT*)g.C + (int64_t)z * g.c_zs;
   const int cn = n0 + wn * WN;
 #pragma unroll
   for (int a = 0; a < MB; ++a) {
-    const int rbase = m0 + wm * WM + 32 * a;
+    const int r = m0 + wm * WM + 32 * a + l32;
+    OutT* row = C + (int64_t)r * g.ldc;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b) {
+      float v[4][4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int lc = 32 * b + 8 * q + 4 * h, c = cn + lc;
-        float v[4];
+        float4 bb = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (g.bias) bb = *reinterpret_cast<const float4*>(lds + BIAS + (wn * WN + lc) * 4);
+        v[q][0] = acc[a][b][4 * q] + bb.x;
+        v[q][1] = acc[a][b][4 * q + 1] + bb.y;
+        v[q][2] = acc[a][b][4 * q + 2] + bb.z;
+        v[q][3] = acc[a][b][4 * q + 3] + bb.w;
+        if (g.beta && r < g.M) {
+          if (g.vec) {
+            if (c < g.N) {
+              if constexpr (OB) {
+                const uint2 w = *reinterpret_cast<const uint2*>(row + c);
+                v[q][0] += __uint_as_float(w.x << 16); v[q][1] += __uint_as_float(w.x & 0xffff0000u);
+                v[q][2] += __uint_as_float(w.y << 16); v[q][3] += __uint_as_float(w.y & 0xffff0000u);
+              } else {
+                const float4 w = *reinterpret_cast<const float4*>(row + c);
+                v[q][0] += w.x; v[q][1] += w.y; v[q][2] += w.z; v[q][3] += w.w;
+              }
+            }
+          } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = acc[a][b][4 * q + i];
-          if (g.bias && c + i < g.N) v[i] += g.bias[c + i];
-          if (g.beta && rbase + l32 < g.M && c + i < g.N) {
-            const OutT o = C[(int64_t)(rbase + l32) * g.ldc + c + i];
-            if constexpr (OB) v[i] += bf2f(o);
-            else v[i] += o;
+            for (int i = 0; i < 4; ++i)
+              if (c + i < g.N) v[q][i] += hx::io<OutT>::ld(row + c + i);
           }
         }
-        if constexpr (OB) *reinterpret_cast<uint2*>(my + l32 * RS + lc * 2) = make_uint2(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]));
-        else *reinterpret_cast<float4*>(my + l32 * RS + lc * 4) = make_float4(v[0], v[1], v[2], v[3]);
       }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own writes; no other wave reads them
-    constexpr int CH = WN * ES / 16, RPI = 64 / CH, EPC = 16 / ES;
+      if (g.vec) {
+        if constexpr (OB) {
 #pragma unroll
-    for (int i = 0; i < 32 / RPI; ++i) {
-      const int lr = i * RPI + lane / CH, lc = (lane % CH) * EPC, r = rbase + lr, c = cn + lc;
-      const uint4 v = *reinterpret_cast<const uint4*>(my + lr * RS + lc * ES);
-      if (r < g.M && c < g.N) {
-        OutT* p = C + (int64_t)r * g.ldc + c;
-        if (g.vec) {
-          *reinterpret_cast<uint4*>(p) = v;
+          for (int q = 0; q < 4; q += 2) {   // columns 8 q + 8 h .. + 8 after the exchange
+            const auto x = __builtin_amdgcn_permlane32_swap(bf16x2(v[q][0], v[q][1]), bf16x2(v[q + 1][0], v[q + 1][1]), false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(bf16x2(v[q][2], v[q][3]), bf16x2(v[q + 1][2], v[q + 1][3]), false, false);
+            const int c = cn + 32 * b + 8 * q + 8 * h;
+            if (r < g.M && c < g.N) *reinterpret_cast<uint4*>(row + c) = make_uint4(x[0], y[0], x[1], y[1]);
+          }
         } else {
-          const OutT* e = reinterpret_cast<const OutT*>(&v);
 #pragma unroll
-          for (int k = 0; k < EPC; ++k)
-            if (c + k < g.N) p[k] = e[k];
+          for (int q = 0; q < 4; ++q) {
+            const int c = cn + 32 * b + 8 * q + 4 * h;
+            if (r < g.M && c < g.N) *reinterpret_cast<float4*>(row + c) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
+          }
         }
+      } else if (r < g.M) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int c = cn + 32 * b + 8 * q + 4 * h + i;
+            if (c < g.N) hx::io<OutT>::st(row + c, v[q][i]);
+          }
       }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the next 32 rows overwrite
   }
 }
 
@@ -300,7 +334,7 @@ __global__ __launch_bounds__(256) void fp8_slabs_k(const float* __restrict__ par
 template <int BM, int BN, int WM, int WN, int KS, int NS, int WGS, bool EXACT, bool OB>
 int launch(const HxGemm8& g, hipStream_t s) {
   constexpr int NT = (BM / WM) * (BN / WN) * 64;
-  constexpr int LDS = NS * (BM + BN) * KS + 6144;
+  constexpr int LDS = NS * (BM + BN) * KS + 6144;   // + scale words, bias, spare
   auto k = gemm_fp8_k<BM, BN, WM, WN, KS, NS, WGS, EXACT, OB>;
   static const hipError_t ok = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (ok != hipSuccess) return 1;
@@ -311,28 +345,51 @@ int launch(const HxGemm8& g, hipStream_t s) {
 template <bool EXACT, bool OB>
 int launch_cfg(const HxGemm8& g, int cfg, hipStream_t s) {
   switch (cfg) {
-    case 0: return launch<256, 128, 128, 64, 64, 3, 2, EXACT, OB>(g, s);
+    case 0: return launch<256, 256, 128, 64, 128, 2, 1, EXACT, OB>(g, s);
     case 1: return launch<128, 128, 64, 64, 128, 2, 2, EXACT, OB>(g, s);
     case 2: return launch<64, 64, 32, 32, 128, 2, 4, EXACT, OB>(g, s);
   }
   return 1;
 }
-constexpr int kBM[3] = {256, 128, 64}, kBN[3] = {128, 128, 64};
+constexpr int kTile[3] = {256, 128, 64};
+
+// Time in us of a product whose busiest CU gets n tiles of nkb k blocks: f + f1 nkb + n (t + t1 nkb),
+// fitted (non-negative least squares, 9 - 15 %) to 46 products of 128 .. 16384 tokens with the widths of
+// BERT-base and BERT-large.  The large tile is at the power limit of the matrix cores (a k block of a
+// 256 x 256 tile in 1.1 us on every CU: 3.9 PF; exact 2.15 us: 2.0 PF; instructions alone on such data
+// run at 3.8 and 1.8) but pays 7.7 us of first loads and stores per tile; the small one fills the
+// chip with few rows.  Choosing by it is on average 1 % from the best of the three, 15 % at most.
+struct Cost {
+  double f, f1, t, t1;
+};
+constexpr Cost kCost[2][3] = {{{0, 0, 7.7, 1.11}, {0, 0.04, 2.07, 0.554}, {0, 0.106, 0.74, 0.199}},
+                              {{0, 0, 12.8, 2.15}, {1.6, 0, 2.66, 0.913}, {0.97, 0.118, 0.835, 0.294}}};
 
 }  // namespace
 
-// the tile: the largest whose tiles give every CU one (a larger tile reads less LDS and L2 per product)
-int hx_gemm_fp8_plan(int M, int N) {
-  for (int c = 0; c < 2; ++c)
-    if ((int64_t)((M + kBM[c] - 1) / kBM[c]) * ((N + kBN[c] - 1) / kBN[c]) >= hx_cu_slots()) return c;
-  return 2;
-}
-// split-K slabs: as many as keep one workgroup per CU, of at least 4 scale groups (2048 deep)
-int hx_gemm_fp8_ks(int M, int N, int nkb, int cfg) {
-  const int64_t tiles = (int64_t)((M + kBM[cfg] - 1) / kBM[cfg]) * ((N + kBN[cfg] - 1) / kBN[cfg]);
-  const int groups = (nkb + 3) / 4;
-  const int ks = (int)std::min<int64_t>(hx_cu_slots() / std::max<int64_t>(tiles, 1), groups / 4);
-  return std::max(ks, 1);
+// The tile and the number of split-K slabs with the least predicted time.  Slabs are whole scale groups
+// (512 deep); their cost: a second launch (3 us) and fp32 slabs written and read at 8 bytes per ns.
+void hx_gemm_fp8_plan(int M, int N, int nkb, int exact, int* cfg, int* ks) {
+  const int slots = hx_cu_slots(), groups = (nkb + 3) / 4;
+  double best = 1e30;
+  *cfg = 2;
+  *ks = 1;
+  for (int c = 0; c < 3; ++c) {
+    const int64_t tiles = (int64_t)((M + kTile[c] - 1) / kTile[c]) * ((N + kTile[c] - 1) / kTile[c]);
+    for (int k = 1; k <= 16 && k <= groups; ++k) {
+      const int per = (groups + k - 1) / k;
+      if (k > 1 && (groups + per - 1) / per != k) continue;   // (an empty slab)
+      const Cost& q = kCost[exact ? 1 : 0][c];
+      const double n = (double)((tiles * k + slots - 1) / slots), kb = k == 1 ? nkb : 4.0 * per;
+      double t = q.f + q.f1 * kb + n * (q.t + q.t1 * kb);
+      if (k > 1) t += 3.0 + 8.0 * k * M * (double)N / 8e6;
+      if (t < best) {
+        best = t;
+        *cfg = c;
+        *ks = k;
+      }
+    }
+  }
 }
 
 int hx_gemm_fp8(const HxGemm8& g, int cfg, int exact, int out_bf16, hipStream_t s) {
