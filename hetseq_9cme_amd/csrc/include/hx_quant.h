@@ -41,10 +41,19 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a <= 3.402823466e38f ? a : 0.f;   // inf / NaN do not take part in the maximum
 }
 
-// 4 scaled values -> 4 e4m3 codes in one word (v_cvt_pk_fp8_f32: nearest even; |x| <= 448 or not finite)
-__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+// 4 values -> their 4 e4m3 codes at scale s = 2^e in one word: v_cvt_scalef32_pk_fp8_* rounds x / s to
+// nearest even, and what is not finite to NaN
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16v2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, float s) {
+  i16x2 r = {0, 0};
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, s, false);
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, s, true));
+}
+__device__ __forceinline__ uint32_t e4m3x4(uint32_t ab, uint32_t cd, float s) {   // of packed bf16 pairs
+  i16x2 r = {0, 0};
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16v2, ab), s, false);
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16v2, cd), s, true));
 }
 // one scaled value -> its int8 code in the low byte
 __device__ __forceinline__ uint32_t int8_of(float v) {
@@ -118,12 +127,14 @@ __device__ __forceinline__ void store_upto(T* p, int n, bool vec, const float (&
     if (k < n) io<T>::st(p + k, v[k]);
 }
 
-// max over the 16 lanes that hold one block's row
-__device__ __forceinline__ float max16(float m) {
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  return m;
+// max over the 16 lanes that hold one block's row (a DPP row): each step joins groups that already agree
+__device__ __forceinline__ uint32_t max16u(uint32_t m) {
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, false));    // lane ^ 1
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, false));    // lane ^ 2
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, false));   // mirrored in 8
+  return max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xF, 0xF, false));   // mirrored in 16
 }
+__device__ __forceinline__ float max16(float m) { return __uint_as_float(max16u(__float_as_uint(m))); }   // m >= 0
 
 }  // namespace q8
 }  // namespace hx

@@ -18,9 +18,11 @@ using namespace hx::q8;
 constexpr int NT = 256;
 
 // ---------------------------------------------------------------- split8
-// One 128 x 128 tile per workgroup; thread t holds rows 8 (t / 16) .. + 8, columns 8 (t % 16) .. + 8,
-// so a wave reads 4 rows of 256 (bf16) or 512 B at a time, a row block's maximum is 16 lanes, and
-// the thread's 8 consecutive rows are 8 consecutive bytes of a transposed row.
+// One 128 x 128 tile per workgroup of 512; thread t holds rows 4 (t / 16) .. + 4, columns 8 (t % 16) ..
+// + 8: a wave reads 4 rows of 256 (bf16) or 512 B at a time, a row block's maximum is one DPP row of 16
+// lanes, and the thread's 4 consecutive rows are 4 consecutive bytes of a transposed row.
+// Bound by memory where there are many tiles (dy of 16384 x 2304 bf16, 150 MB read and written),
+// by one tile's chain of loads, maxima and stores where there are few.
 struct Split8 {
   const void* x;
   int64_t ld;
@@ -33,76 +35,168 @@ struct Split8 {
   int vec;
 };
 
-template <typename T>
-__global__ __launch_bounds__(NT) void split8_k(Split8 a) {
-  __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 144];   // transposed codes, rows of 128 + 16
-  __shared__ float redm[4][128], reds[4][128];
+constexpr int SNT = 512, SR = 4;   // threads, rows per thread
+constexpr uint32_t kInf = 0x7f800000u;
+
+// A thread's SR x 8 values, their magnitudes as fp32 bits compared as integers (an infinity or NaN
+// then shows as a maximum >= kInf, and the block's finite maximum is taken again), and their codes.
+struct TileF32 {
+  float v[SR][8];
+  __device__ void load(const void* x, int64_t at, int i, int n, bool vec) { load_upto<float>((const float*)x + at, n, vec, v[i]); }
+  __device__ static uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+  __device__ uint32_t row_max(int i) const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = max(m, mag(v[i][k]));
+    return m;
+  }
+  __device__ void col_max(uint32_t (&m)[8]) const {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      m[k] = 0;
+#pragma unroll
+      for (int i = 0; i < SR; ++i) m[k] = max(m[k], mag(v[i][k]));
+    }
+  }
+  __device__ float at(int i, int k) const { return v[i][k]; }
+  __device__ uint2 row_codes(int i, float s) const {
+    return make_uint2(e4m3x4(v[i][0], v[i][1], v[i][2], v[i][3], s), e4m3x4(v[i][4], v[i][5], v[i][6], v[i][7], s));
+  }
+  __device__ uint32_t col_codes(int k, float s) const { return e4m3x4(v[0][k], v[1][k], v[2][k], v[3][k], s); }
+};
+
+// the same on packed bf16 pairs (word j: columns 2 j, 2 j + 1)
+struct TileBf16 {
+  uint32_t w[SR][4];
+  __device__ void load(const void* x, int64_t at, int i, int n, bool vec) {
+    const uint16_t* p = (const uint16_t*)x + at;
+    if (vec && n >= 8) {
+      const uint4 a = *reinterpret_cast<const uint4*>(p);
+      w[i][0] = a.x; w[i][1] = a.y; w[i][2] = a.z; w[i][3] = a.w;
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[i][j] = (2 * j < n ? (uint32_t)p[2 * j] : 0u) | (2 * j + 1 < n ? (uint32_t)p[2 * j + 1] << 16 : 0u);
+  }
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  __device__ static u16x2 mag2(uint32_t x) { return __builtin_bit_cast(u16x2, x & 0x7fff7fffu); }
+  __device__ uint32_t row_max(int i) const {
+    const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(mag2(w[i][0]), mag2(w[i][1])),
+                                              __builtin_elementwise_max(mag2(w[i][2]), mag2(w[i][3])));
+    return (uint32_t)max(m[0], m[1]) << 16;
+  }
+  __device__ void col_max(uint32_t (&m)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u16x2 a = mag2(w[0][j]);
+#pragma unroll
+      for (int i = 1; i < SR; ++i) a = __builtin_elementwise_max(a, mag2(w[i][j]));
+      m[2 * j] = (uint32_t)a[0] << 16;
+      m[2 * j + 1] = (uint32_t)a[1] << 16;
+    }
+  }
+  __device__ float at(int i, int k) const { return __uint_as_float(k & 1 ? w[i][k >> 1] & 0xffff0000u : w[i][k >> 1] << 16); }
+  __device__ uint2 row_codes(int i, float s) const { return make_uint2(e4m3x4(w[i][0], w[i][1], s), e4m3x4(w[i][2], w[i][3], s)); }
+  __device__ uint32_t col_codes(int k, float s) const {
+    const uint32_t sel = k & 1 ? 0x07060302u : 0x05040100u;   // (row i, row i + 1) of column k as a pair
+    return e4m3x4(__builtin_amdgcn_perm(w[1][k >> 1], w[0][k >> 1], sel), __builtin_amdgcn_perm(w[3][k >> 1], w[2][k >> 1], sel), s);
+  }
+};
+
+template <typename Tile>
+__global__ __launch_bounds__(SNT) void split8_k(Split8 a) {
+  // transposed codes, 128 rows of 128 B; 16-B chunk ch of row c at ch ^ (c / 8 % 8): the writes of a
+  // wave (16 columns, 8 apart, of one chunk) and the reads (8 chunks of a row) spread over the banks
+  __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
+  __shared__ uint32_t redm[SNT / 64][128];
+  __shared__ float reds[SNT / 64][128];
   const int t = threadIdx.x, cg = t & 15, rg = t >> 4, w = t >> 6;
   const int nc = (a.C + 127) / 128;
   const int cb = blockIdx.x % nc, rb = blockIdx.x / nc;
-  const int c0 = cb * 128 + 8 * cg, r0 = rb * 128 + 8 * rg;
+  const int c0 = cb * 128 + 8 * cg, r0 = rb * 128 + SR * rg;
   const int64_t Rs = (a.R + 3) & ~3, Cs = (a.C + 3) & ~3;
   const int Cp = (a.C + 127) / 128 * 128, Rp = (a.R + 127) / 128 * 128;
-  float v[8][8];
+  Tile x;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    load_upto<T>((const T*)a.x + (int64_t)(r0 + i) * a.ld + c0, r0 + i < a.R ? a.C - c0 : 0, a.vec, v[i]);
+  for (int i = 0; i < SR; ++i) x.load(a.x, (int64_t)(r0 + i) * a.ld + c0, i, r0 + i < a.R ? a.C - c0 : 0, a.vec);
   if (a.q) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float m = 0.f;
+    for (int i = 0; i < SR; ++i) {
+      uint32_t m = max16u(x.row_max(i));
+      if (__builtin_expect(m >= kInf, 0)) {   // (a row's 16 lanes agree)
+        m = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[i][k]));
-      const int e = block_exp<E4M3>(max16(m));
-      const float is = exp2i(-e);
+        for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(finite_abs(x.at(i, k))));
+        m = max16u(m);
+      }
+      const int e = block_exp<E4M3>(__uint_as_float(m));
       if (r0 + i < a.R) {
-        const uint2 o = make_uint2(e4m3x4(v[i][0] * is, v[i][1] * is, v[i][2] * is, v[i][3] * is),
-                                   e4m3x4(v[i][4] * is, v[i][5] * is, v[i][6] * is, v[i][7] * is));
-        *reinterpret_cast<uint2*>(a.q + (int64_t)(r0 + i) * Cp + c0) = o;
+        *reinterpret_cast<uint2*>(a.q + (int64_t)(r0 + i) * Cp + c0) = x.row_codes(i, exp2i(e));
         if (cg == 0) a.s[((cb >> 2) * Rs + r0 + i) * 4 + (cb & 3)] = (uint8_t)(e + 127);
       }
     }
   }
   if (!a.qt && !a.colpart) return;
-  // column maxima and sums: the wave's four row groups by shuffles, the four waves through LDS
+  // column maxima and sums: the wave's four row groups by shuffles, the waves through LDS
+  if (a.qt) {
+    uint32_t m[8];
+    x.col_max(m);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    float m = 0.f, s = 0.f;
+    for (int k = 0; k < 8; ++k) {
+      if (__builtin_expect(m[k] >= kInf, 0)) {
+        m[k] = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      m = fmaxf(m, finite_abs(v[i][k]));
-      s += v[i][k];
+        for (int i = 0; i < SR; ++i) m[k] = max(m[k], __float_as_uint(finite_abs(x.at(i, k))));
+      }
+      m[k] = max(m[k], (uint32_t)__shfl_xor((int)m[k], 16, 64));
+      m[k] = max(m[k], (uint32_t)__shfl_xor((int)m[k], 32, 64));
     }
-    m = fmaxf(m, __shfl_xor(m, 16, 64));
-    m = fmaxf(m, __shfl_xor(m, 32, 64));
-    s += __shfl_xor(s, 16, 64);
-    s += __shfl_xor(s, 32, 64);
     if ((t & 63) < 16) {
-      redm[w][8 * cg + k] = m;
-      reds[w][8 * cg + k] = s;
+      *reinterpret_cast<uint4*>(&redm[w][8 * cg]) = make_uint4(m[0], m[1], m[2], m[3]);
+      *reinterpret_cast<uint4*>(&redm[w][8 * cg + 4]) = make_uint4(m[4], m[5], m[6], m[7]);
+    }
+  }
+  if (a.colpart) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float s = (x.at(0, k) + x.at(1, k)) + (x.at(2, k) + x.at(3, k));
+      s += __shfl_xor(s, 16, 64);
+      s += __shfl_xor(s, 32, 64);
+      if ((t & 63) < 16) reds[w][8 * cg + k] = s;
     }
   }
   __syncthreads();
-  if (a.colpart && t < 128 && cb * 128 + t < a.C)
-    a.colpart[(int64_t)rb * a.C + cb * 128 + t] = (reds[0][t] + reds[1][t]) + (reds[2][t] + reds[3][t]);
+  if (a.colpart && t < 128 && cb * 128 + t < a.C) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < SNT / 64; ++k) s += reds[k][t];
+    a.colpart[(int64_t)rb * a.C + cb * 128 + t] = s;
+  }
   if (!a.qt) return;
+  // one thread per column folds the waves' maxima into the column's exponent
+  if (t < 128) {
+    uint32_t m = redm[0][t];
+#pragma unroll
+    for (int k = 1; k < SNT / 64; ++k) m = max(m, redm[k][t]);
+    const int e = block_exp<E4M3>(__uint_as_float(m));
+    redm[0][t] = __float_as_uint(exp2i(e));
+    if (cb * 128 + t < a.C) a.st[((rb >> 2) * Cs + cb * 128 + t) * 4 + (rb & 3)] = (uint8_t)(e + 127);
+  }
+  __syncthreads();
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const int c = 8 * cg + k;
-    const int e = block_exp<E4M3>(fmaxf(fmaxf(redm[0][c], redm[1][c]), fmaxf(redm[2][c], redm[3][c])));
-    const float is = exp2i(-e);
-    *reinterpret_cast<uint2*>(tile + c * 144 + 8 * rg) =
-        make_uint2(e4m3x4(v[0][k] * is, v[1][k] * is, v[2][k] * is, v[3][k] * is),
-                   e4m3x4(v[4][k] * is, v[5][k] * is, v[6][k] * is, v[7][k] * is));
-    if (rg == 0 && cb * 128 + c < a.C) a.st[((rb >> 2) * Cs + cb * 128 + c) * 4 + (rb & 3)] = (uint8_t)(e + 127);
+    *reinterpret_cast<uint32_t*>(tile + c * 128 + 16 * ((rg >> 2) ^ (cg & 7)) + 4 * (rg & 3)) =
+        x.col_codes(k, __uint_as_float(redm[0][c]));
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {   // 128 transposed rows of 8 x 16 B
-    const int c = 32 * i + (t >> 3), ch = t & 7;
+  for (int i = 0; i < 128 * 8 / SNT; ++i) {   // 128 transposed rows of 8 x 16 B
+    const int c = SNT / 8 * i + (t >> 3), ch = t & 7;
     if (cb * 128 + c < a.C)
       *reinterpret_cast<uint4*>(a.qt + (int64_t)(cb * 128 + c) * Rp + rb * 128 + 16 * ch) =
-          *reinterpret_cast<const uint4*>(tile + c * 144 + 16 * ch);
+          *reinterpret_cast<const uint4*>(tile + c * 128 + 16 * (ch ^ ((c >> 3) & 7)));
   }
 }
 
@@ -249,8 +343,8 @@ void hx_split8(int bf16, const void* x, int64_t ld, int R, int C, uint8_t* q, ui
                float* colpart, float* colsum, int vec, hipStream_t stream) {
   Split8 a{x, ld, R, C, q, s, qt, st, colpart, vec};
   const unsigned grid = (unsigned)(((C + 127) / 128) * (int64_t)((R + 127) / 128));
-  if (bf16) split8_k<uint16_t><<<grid, NT, 0, stream>>>(a);
-  else split8_k<float><<<grid, NT, 0, stream>>>(a);
+  if (bf16) split8_k<TileBf16><<<grid, SNT, 0, stream>>>(a);
+  else split8_k<TileF32><<<grid, SNT, 0, stream>>>(a);
   if (colpart) fold_rows(colpart, hx_split8_row_tiles(R), C, C, C, colsum, nullptr, nullptr, 0, stream);
 }
 
