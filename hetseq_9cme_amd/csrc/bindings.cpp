@@ -855,6 +855,112 @@ Tensor gemm_fp8(Tensor a, Tensor as, Tensor b, Tensor bs, int64_t K, bool out_bf
   return out;
 }
 
+// x [M, K] W^T (+ bias) from W's codes; with `keep`, also x's codes blocked along the rows (the weight
+// gradient's operand).  Few rows that need no such copy go through one launch (fp8_rows_k).
+static Tensor linear_fp8_y(const Tensor& x2, const Tensor& wq, const Tensor& ws, const OptT& bias, bool keep, OptT* qt, OptT* st) {
+  const int64_t M = x2.size(0), K = x2.size(1), N = wq.size(0);
+  if (!keep && M > 0 && M <= hx_fp8_rows_max()) {
+    check_rows8(x2, "linear_fp8");
+    TORCH_CHECK(wq.is_cuda() && wq.device() == x2.device() && wq.size(1) == blocks128(K) * 128 && wq.is_contiguous() && aligned16(wq.data_ptr()) &&
+                    ws.numel() == (blocks128(K) + 3) / 4 * ((N + 3) / 4 * 4) * 4, "linear_fp8: the weight's codes do not fit x");
+    check_bias8(bias, N, x2, "linear_fp8 bias");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x2.device());
+    Tensor y = torch::empty({M, N}, x2.options());
+    HxRows8 g{};
+    g.x = x2.data_ptr();
+    g.ldx = M > 1 ? x2.stride(0) : K;
+    g.B = wq.data_ptr<uint8_t>();
+    g.ldb = wq.size(1);
+    g.sb = reinterpret_cast<const uint32_t*>(ws.data_ptr());
+    g.y = y.data_ptr();
+    g.bias = ptr_or_null<float>(bias);
+    g.M = (int)M;
+    g.N = (int)N;
+    g.K = (int)K;
+    g.nkb = (int)blocks128(K);
+    g.xvec = rows_vec(x2, g.ldx);
+    TORCH_CHECK(hx_fp8_rows(g, act_bf16(x2), cur_stream(x2)) == 0, "linear_fp8: launch failed");
+    dbg_finite(y, "linear_fp8");
+    return y;
+  }
+  std::vector<OptT> c = split8(x2, true, keep, false, c10::nullopt);
+  if (keep) {
+    *qt = c[2];
+    *st = c[3];
+  }
+  return gemm_fp8(*c[0], *c[1], wq, ws, K, x2.scalar_type() == torch::kBFloat16, c10::nullopt, false, bias);
+}
+// [.., K] -> [rows, K] with unit column stride (a contiguous copy if it has none)
+static Tensor as_rows8(const Tensor& x) {
+  Tensor x2 = x.reshape({-1, x.size(-1)});
+  const bool ok = (x2.stride(1) == 1 || x2.size(1) == 1) && (x2.stride(0) >= x2.size(1) || x2.size(0) <= 1);
+  return ok ? x2 : x2.contiguous();
+}
+
+// forward alone, for the autograd functions of the Python layer: (y, x's kept codes, their scales)
+std::vector<OptT> linear_fp8_fwd(Tensor x2, Tensor wq, Tensor ws, OptT bias, bool keep) {
+  OptT qt, st;
+  Tensor y = linear_fp8_y(x2, wq, ws, bias, keep, &qt, &st);
+  return {y, qt, st};
+}
+
+// The whole layer as one autograd node for parameters that autograd accumulates itself (no flat gradient
+// slots, no residual mailbox): a small layer's step is bound by the host, and a node in C++ runs its
+// backward without the interpreter lock (ops/fp8.py: training step of 41 x 1024 x 1024)
+struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor x, OptT W, OptT b, Tensor wq, Tensor ws, OptT wqt,
+                        OptT wst, bool keep) {
+    const int64_t N = wq.size(0);
+    Tensor x2 = as_rows8(x);
+    OptT qt, st;
+    Tensor y = linear_fp8_y(x2.detach(), wq, ws, has(b) ? OptT(b->detach()) : OptT(), keep, &qt, &st);
+    ctx->save_for_backward({qt.value_or(Tensor()), st.value_or(Tensor()), wqt.value_or(Tensor()), wst.value_or(Tensor())});
+    ctx->saved_data["xshape"] = x.sizes().vec();
+    ctx->saved_data["N"] = N;
+    ctx->saved_data["wbf16"] = has(W) && W->scalar_type() == torch::kBFloat16;
+    // the inputs that are there have the first edges, in order
+    ctx->saved_data["ew"] = has(W) ? 1 : 0;
+    ctx->saved_data["eb"] = has(b) ? (has(W) ? 2 : 1) : 0;
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = N;
+    return y.view(shape);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const auto xshape = ctx->saved_data["xshape"].toIntVector();
+    const int64_t N = ctx->saved_data["N"].toInt(), K = xshape.back();
+    const int64_t ew = ctx->saved_data["ew"].toInt(), eb = ctx->saved_data["eb"].toInt();
+    const bool need_x = ctx->needs_input_grad(0), need_w = ew && ctx->needs_input_grad(ew), need_b = eb && ctx->needs_input_grad(eb);
+    Tensor dy2 = as_rows8(g[0]);
+    const int64_t M = dy2.size(0);
+    const bool bf16 = dy2.scalar_type() == torch::kBFloat16;
+    std::vector<OptT> c = split8(dy2, need_x, need_w && M > 0, need_b, c10::nullopt);
+    Tensor dx, dW;
+    if (need_w) {
+      if (M == 0) dW = torch::zeros({N, K}, dy2.options().dtype(torch::kFloat32));
+      else dW = gemm_fp8(*c[2], *c[3], saved[0], saved[1], M, false, c10::nullopt, false, c10::nullopt);
+      if (ctx->saved_data["wbf16"].toBool()) dW = dW.to(torch::kBFloat16);
+    }
+    if (need_x) dx = gemm_fp8(*c[0], *c[1], saved[2], saved[3], N, bf16, c10::nullopt, false, c10::nullopt).view(xshape);
+    return {dx, dW, need_b ? *c[4] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+// W: the parameter whose gradient is wanted (or none); w8: its codes and scales (wq, ws, wqt, wst -- the
+// last two may be absent), or none: they are made here from W
+Tensor linear_fp8(Tensor x, OptT W, OptT b, std::vector<OptT> w8, bool grad) {
+  OptT wq, ws, wqt, wst;
+  if (w8.empty()) {
+    TORCH_CHECK(has(W), "linear_fp8: a weight or its codes");
+    std::vector<OptT> c = split8(as_rows8(W->detach()), true, grad && x.requires_grad(), false, c10::nullopt);
+    wq = c[0]; ws = c[1]; wqt = c[2]; wst = c[3];
+  } else {
+    TORCH_CHECK(w8.size() == 4 && has(w8[0]) && has(w8[1]), "linear_fp8: the weight's codes and scales");
+    wq = w8[0]; ws = w8[1]; wqt = w8[2]; wst = w8[3];
+  }
+  const bool keep = grad && has(W) && W->requires_grad();
+  return LinearFp8::apply(x, W, b, *wq, *ws, wqt, wst, keep);
+}
+
 // ---- int8 blocks along the last dimension (contiguous rows): codes [rows, nb, 128], scale bytes [rows, nb]
 inline void check_kept(const Tensor& q, const Tensor& s, const Tensor& like, int64_t rows, int64_t N, const char* what) {
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == torch::kUInt8 && q.is_contiguous() && aligned16(q.data_ptr()) &&
@@ -908,6 +1014,22 @@ std::vector<OptT> gelu8_bwd(Tensor dout, Tensor q, Tensor s, OptT b, bool want_d
   dbg_finite(dy, "gelu8_bwd");
   return {dy, db};
 }
+
+// bias + GELU as one autograd node (see LinearFp8)
+struct BiasGelu8 : public torch::autograd::Function<BiasGelu8> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor y, OptT b) {
+    std::vector<Tensor> r = gelu8_fwd(y.detach(), has(b) ? OptT(b->detach()) : OptT());
+    ctx->save_for_backward({r[1], r[2], has(b) ? b->detach() : Tensor()});
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const bool need_b = saved[2].defined() && ctx->needs_input_grad(1);
+    std::vector<OptT> r = gelu8_bwd(g[0].contiguous(), saved[0], saved[1], saved[2].defined() ? OptT(saved[2]) : OptT(), need_b, c10::nullopt);
+    return {*r[0], need_b ? *r[1] : Tensor()};
+  }
+};
+Tensor bias_gelu8(Tensor y, OptT b) { return BiasGelu8::apply(y.contiguous(), b); }
 
 std::vector<Tensor> pack8(Tensor x) {
   const auto [rows, N] = rows_cols8(x, "pack8 x");
@@ -1303,6 +1425,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("sum_out") = py::none());
   m.def("gemm_fp8", &gemm_fp8, py::arg("a"), py::arg("as"), py::arg("b"), py::arg("bs"), py::arg("K"), py::arg("out_bf16"),
         py::arg("out") = py::none(), py::arg("beta") = false, py::arg("bias") = py::none());
+  m.def("linear_fp8_fwd", &linear_fp8_fwd, py::arg("x"), py::arg("wq"), py::arg("ws"), py::arg("bias"), py::arg("keep"));
+  m.def("linear_fp8", &linear_fp8, py::arg("x"), py::arg("W"), py::arg("bias"), py::arg("w8"), py::arg("grad"));
+  m.def("bias_gelu8", &bias_gelu8, py::arg("y"), py::arg("bias"));
   m.def("gelu8_fwd", &gelu8_fwd);
   m.def("gelu8_bwd", &gelu8_bwd, py::arg("dout"), py::arg("q"), py::arg("s"), py::arg("bias"), py::arg("want_db"),
         py::arg("db_out") = py::none());

@@ -269,3 +269,17 @@ void hx_gemm_fp8_plan(int M, int N, int nkb, int exact, int* cfg, int* ks);   //
 int hx_gemm_fp8(const HxGemm8& g, int cfg, int exact, int out_bf16, hipStream_t s);
 void hx_gemm_fp8_slabs(const float* part, void* out, int out_bf16, int64_t ldc, int M, int N, int ks, const float* bias,
                        int beta, int vec, hipStream_t s);
+// y [M, N] (x's type, contiguous) = Q(x) B^T (+ bias) for M <= hx_fp8_rows_max() rows of fp32 or bf16 x
+// (row stride ldx; xvec: rows allow 16-B accesses), B as in HxGemm8
+struct HxRows8 {
+  const void* x;
+  int64_t ldx;
+  const uint8_t* B;
+  int64_t ldb;
+  const uint32_t* sb;
+  void* y;
+  const float* bias;
+  int M, N, K, nkb, xvec;
+};
+int hx_fp8_rows_max();
+int hx_fp8_rows(const HxRows8& g, int bf16, hipStream_t s);

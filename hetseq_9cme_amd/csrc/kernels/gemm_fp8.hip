@@ -331,6 +331,90 @@ __global__ __launch_bounds__(256) void fp8_slabs_k(const float* __restrict__ par
   }
 }
 
+// ---------------------------------------------------------------- few rows
+// y = Q(x) W^T (+ bias) for up to 16 MBK rows of unquantised x, in one launch: 16 output features per
+// workgroup, the k blocks dealt over its 8 waves.  A wave reads its W codes straight into registers
+// (32 B of a row per lane: a whole 128-B line per row), rounds its 32 x values per lane to e4m3 (the
+// block's maximum is 4 lanes), runs both through exact bf16 MFMAs, and the waves' sums are added in
+// LDS in wave order.  Bound by latency (one token through 768 x 2304: 1.8 MB of codes): splitting the
+// reduction inside the workgroup keeps 8 waves of loads in flight where a tile per wave would leave one.
+template <typename T, int MBK>
+__global__ __launch_bounds__(512) void fp8_rows_k(HxRows8 g) {
+  constexpr int NW = 8;
+  __shared__ float red[NW][MBK][256];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l16 = lane & 15, h = lane >> 4;
+  const int n0 = blockIdx.x * 16, n = n0 + l16;
+  const int64_t sbn = (g.N + 3) & ~3;
+  f32x4 acc[MBK];
+#pragma unroll
+  for (int m = 0; m < MBK; ++m) acc[m] = f32x4{0, 0, 0, 0};
+  for (int kb = wv; kb < g.nkb; kb += NW) {
+    const int k0 = kb * 128 + 32 * h;
+    uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
+    uint32_t sw = 0x7f7f7f7fu;
+    if (n < g.N) {
+      const uint4* p = reinterpret_cast<const uint4*>(g.B + (int64_t)n * g.ldb + k0);
+      w0 = p[0];
+      w1 = p[1];
+      sw = g.sb[(kb >> 2) * sbn + n];
+    }
+    float x[MBK][32];
+#pragma unroll
+    for (int m = 0; m < MBK; ++m) {
+      const int r = 16 * m + l16;
+      const T* p = (const T*)g.x + (int64_t)r * g.ldx + k0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float v[8];
+        hx::q8::load_upto<T>(p + 8 * q, r < g.M ? g.K - k0 - 8 * q : 0, g.xvec, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[m][8 * q + i] = v[i];
+      }
+    }
+    const float ws = hx::q8::scale_of((sw >> (8 * (kb & 3))) & 0xffu);
+    const uint32_t wc[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+    bf16x8v wd[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) wd[q] = decode8(wc[2 * q], wc[2 * q + 1], ws);
+#pragma unroll
+    for (int m = 0; m < MBK; ++m) {
+      uint32_t a = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) a = max(a, __float_as_uint(x[m][i]) & 0x7fffffffu);
+      a = max(a, (uint32_t)__shfl_xor((int)a, 16, 64));
+      a = max(a, (uint32_t)__shfl_xor((int)a, 32, 64));
+      if (__builtin_expect(a >= 0x7f800000u, 0)) {   // something not finite: the maximum of the rest
+        a = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) a = max(a, __float_as_uint(hx::q8::finite_abs(x[m][i])));
+        a = max(a, (uint32_t)__shfl_xor((int)a, 16, 64));
+        a = max(a, (uint32_t)__shfl_xor((int)a, 32, 64));
+      }
+      const float xs = hx::q8::exp2i(hx::q8::block_exp<hx::q8::E4M3>(__uint_as_float(a)));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float* v = &x[m][8 * q];
+        const bf16x8v xd = decode8((int)hx::q8::e4m3x4(v[0], v[1], v[2], v[3], xs), (int)hx::q8::e4m3x4(v[4], v[5], v[6], v[7], xs), xs);
+        acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wd[q], xd, acc[m], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MBK; ++m) *reinterpret_cast<f32x4*>(&red[wv][m][4 * lane]) = acc[m];
+  __syncthreads();
+  for (int t = threadIdx.x; t < 256 * MBK; t += 512) {
+    const int m = t >> 8, e = t & 255;   // element e of a 16 x 16 block: lane e / 4, register e % 4
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) v += red[k][m][e];
+    const int r = 16 * m + ((e >> 2) & 15), c = n0 + 4 * (e >> 6) + (e & 3);
+    if (r < g.M && c < g.N) {
+      if (g.bias) v += g.bias[c];
+      hx::io<T>::st((T*)g.y + (int64_t)r * g.N + c, v);
+    }
+  }
+}
+
 template <int BM, int BN, int WM, int WN, int KS, int NS, int WGS, bool EXACT, bool OB>
 int launch(const HxGemm8& g, hipStream_t s) {
   constexpr int NT = (BM / WM) * (BN / WN) * 64;
@@ -390,6 +474,24 @@ void hx_gemm_fp8_plan(int M, int N, int nkb, int exact, int* cfg, int* ks) {
       }
     }
   }
+}
+
+int hx_fp8_rows_max() { return 64; }
+
+int hx_fp8_rows(const HxRows8& g, int bf16, hipStream_t s) {
+  const unsigned grid = (unsigned)((g.N + 15) / 16);
+  const int mbk = (g.M + 15) / 16;
+  if (mbk < 1 || mbk > 4) return 1;
+  if (bf16) {
+    if (mbk == 1) fp8_rows_k<uint16_t, 1><<<grid, 512, 0, s>>>(g);
+    else if (mbk == 2) fp8_rows_k<uint16_t, 2><<<grid, 512, 0, s>>>(g);
+    else fp8_rows_k<uint16_t, 4><<<grid, 512, 0, s>>>(g);
+  } else {
+    if (mbk == 1) fp8_rows_k<float, 1><<<grid, 512, 0, s>>>(g);
+    else if (mbk == 2) fp8_rows_k<float, 2><<<grid, 512, 0, s>>>(g);
+    else fp8_rows_k<float, 4><<<grid, 512, 0, s>>>(g);
+  }
+  return 0;
 }
 
 int hx_gemm_fp8(const HxGemm8& g, int cfg, int exact, int out_bf16, hipStream_t s) {

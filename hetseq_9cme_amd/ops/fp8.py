@@ -43,6 +43,12 @@ def _check_act(x, what):
         raise ValueError('{}: needs a last dimension of at least 1, got shape {}'.format(what, tuple(x.shape)))
 
 
+def _check_weight(W, what):
+    _check_act(W, what)
+    if W.dim() != 2 or W.shape[0] < 1:
+        raise ValueError('{}: a non-empty [out, in] weight, got shape {}'.format(what, tuple(W.shape)))
+
+
 def _check_bias(b, n, like, what):
     if b is None:
         return
@@ -89,9 +95,7 @@ class Fp8Weight(object):
     __slots__ = ('shape', 'dtype', 'device', 'q', 's', 'qt', 'st', 'ref')
 
     def __init__(self, W, grad=True):
-        _check_act(W, 'Fp8Weight')
-        if W.dim() != 2 or W.shape[0] < 1:
-            raise ValueError('Fp8Weight: a non-empty [out, in] weight, got shape {}'.format(tuple(W.shape)))
+        _check_weight(W, 'Fp8Weight')
         W = W.detach()
         self.shape, self.dtype, self.device = tuple(W.shape), W.dtype, W.device
         self.q = self.s = self.qt = self.st = self.ref = None
@@ -126,14 +130,11 @@ class fp8_scope(object):
         return False
 
 
-def _weight(W, grad):
-    if isinstance(W, Fp8Weight):
-        return W
-    if _Scope.weights is not None:
-        w = _Scope.weights.get((W.data_ptr(), tuple(W.shape)))
-        if w is not None:
-            return w
-    return Fp8Weight(W, grad)
+def _scoped(W):
+    """The running ``fp8_scope``'s copy of W, if it has one."""
+    if _Scope.weights is None:
+        return None
+    return _Scope.weights.get((W.data_ptr(), tuple(W.shape)))
 
 
 def _rows2(x):
@@ -158,8 +159,7 @@ class _LinearFp8Fn(torch.autograd.Function):
         # the weight gradient reads the 8-bit copy of x blocked along the tokens
         keep = any(ctx.needs_input_grad[6:6 + n])
         if use_kernels(x):
-            q, s, qt, st, _ = C().split8(x2, True, keep)
-            y = C().gemm_fp8(q, s, w8.q, w8.s, K, x.dtype == torch.bfloat16, bias=bias)
+            y, qt, st = C().linear_fp8_fwd(x2, w8.q, w8.s, bias, keep)
         else:
             y = e4m3_ref(x2) @ w8.ref[0].t()
             y = (y if bias is None else y + bias).to(x.dtype)
@@ -247,23 +247,31 @@ def linear_fp8(x, W, b=None, res_grad=None):
     ``Fp8Weight`` (then it gets no gradient: inference, frozen layers); ``b`` fp32 [N].
     ``res_grad``: see ``ResidualGrad``."""
     _check_act(x, 'linear_fp8')
-    if not isinstance(W, Fp8Weight):
-        _check_act(W, 'linear_fp8 weight')
-        if W.dim() != 2 or W.shape[0] < 1:
-            raise ValueError('linear_fp8: a non-empty [out, in] weight, got shape {}'.format(tuple(W.shape)))
+    kept = isinstance(W, Fp8Weight)
+    if not kept:
+        _check_weight(W, 'linear_fp8')
     N, K = W.shape
     if x.shape[-1] != K:
         raise ValueError('linear_fp8: x has {} features, the weight takes {}'.format(x.shape[-1], K))
     if x.device != W.device:
         raise ValueError('linear_fp8: x on {}, the weight on {}'.format(x.device, W.device))
     _check_bias(b, N, x, 'linear_fp8')
-    grad = torch.is_grad_enabled() and x.requires_grad
-    w8 = _weight(W, grad)
-    if grad and not w8.has_grad:
+    grad = torch.is_grad_enabled()
+    w8 = W if kept else _scoped(W)
+    if grad and x.requires_grad and w8 is not None and not w8.has_grad:
         raise ValueError('linear_fp8: x needs a gradient, the Fp8Weight was built with grad=False')
-    if isinstance(W, Fp8Weight):
+    if use_kernels(x) and res_grad is None and (kept or not _flat(W)) and not _flat(b):
+        # autograd keeps the gradients: the whole layer is one node (bindings.cpp LinearFp8)
+        return C().linear_fp8(x, None if kept else W, b, [] if w8 is None else [w8.q, w8.s, w8.qt, w8.st], grad)
+    if w8 is None:
+        w8 = Fp8Weight(W, grad and x.requires_grad)
+    if kept:
         return _LinearFp8Fn.apply(x, w8, b, res_grad, True, 0, *(() if b is None else (b,)))
     return _LinearFp8Fn.apply(x, w8, b, res_grad, True, 1, W, *(() if b is None else (b,)))
+
+
+def _flat(p):
+    return getattr(p, '_hx_flat', None) is not None
 
 
 def linear3_fp8(x, wq, wk, wv, bq, bk, bv, res_grad=None, bias_grad=True):
@@ -276,7 +284,7 @@ def linear3_fp8(x, wq, wk, wv, bq, bk, bv, res_grad=None, bias_grad=True):
         bs, bias = (bq, bk, bv), fused._adjacent_view([bq, bk, bv])
         bias = bias if bias is not None else torch.cat([t.detach() for t in bs], 0)
     _check_bias(bias, W.shape[0], x, 'linear3_fp8')
-    w8 = _weight(W, torch.is_grad_enabled() and x.requires_grad)
+    w8 = _scoped(W) or Fp8Weight(W, torch.is_grad_enabled() and x.requires_grad)
     return _LinearFp8Fn.apply(x, w8, bias, res_grad, bool(bias_grad), 3, wq, wk, wv, *bs)
 
 
@@ -309,6 +317,8 @@ def bias_gelu8(y, b):
     """gelu(y + b); the backward reads y from int8 blocks (``bias_act(y, b, 'gelu', bits=8)``)."""
     _check_act(y, 'bias_act(bits=8)')
     _check_bias(b, y.shape[-1], y, 'bias_act(bits=8)')
+    if use_kernels(y) and not _flat(b):
+        return C().bias_gelu8(y, b)
     return _BiasGelu8Fn.apply(y.contiguous(), b)
 
 
