@@ -759,6 +759,22 @@ inline Tensor scale_words(int64_t rows, int64_t cols, const Tensor& like) {
   return torch::empty({(blocks128(cols) + 3) / 4, (rows + 3) / 4 * 4, 4}, like.options().dtype(torch::kUInt8));
 }
 
+static HxSplit8 split8_job(const Tensor& x, uint8_t* q, uint8_t* s, uint8_t* qt, uint8_t* st, float* colpart) {
+  HxSplit8 j{};
+  j.bf16 = act_bf16(x);
+  j.x = x.data_ptr();
+  j.R = (int)x.size(0);
+  j.C = (int)x.size(1);
+  j.ld = x.size(0) > 1 ? x.stride(0) : x.size(1);
+  j.q = q;
+  j.s = s;
+  j.qt = qt;
+  j.st = st;
+  j.colpart = colpart;
+  j.vec = rows_vec(x, j.ld);
+  return j;
+}
+
 // x [R, C] -> (q, s, qt, st, sum): its e4m3 codes blocked along the columns (by_rows) and transposed,
 // blocked along the rows (by_cols), and its fp32 column sums (sum_out / want_sum); undefined where
 // not wanted
@@ -786,12 +802,52 @@ std::vector<OptT> split8(Tensor x, bool by_rows, bool by_cols, bool want_sum, Op
     if (R == 0) sum->zero_();
     else part = torch::empty({hx_split8_row_tiles(R), C}, f32);
   }
-  if (R > 0 && (by_rows || by_cols || want_sum))
-    hx_split8(act_bf16(x), x.data_ptr(), R > 1 ? x.stride(0) : C, (int)R, (int)C, ptr_or_null<uint8_t>(q),
-              ptr_or_null<uint8_t>(s), ptr_or_null<uint8_t>(qt), ptr_or_null<uint8_t>(st),
-              want_sum ? part.data_ptr<float>() : nullptr, ptr_or_null<float>(sum), rows_vec(x, R > 1 ? x.stride(0) : C),
-              cur_stream(x));
+  if (R > 0 && (by_rows || by_cols || want_sum)) {
+    const HxSplit8 job = split8_job(x, ptr_or_null<uint8_t>(q), ptr_or_null<uint8_t>(s), ptr_or_null<uint8_t>(qt),
+                                    ptr_or_null<uint8_t>(st), want_sum ? part.data_ptr<float>() : nullptr);
+    hx_split8(&job, 1, cur_stream(x));
+    if (want_sum) hx_fold_cols(part.data_ptr<float>(), hx_split8_row_tiles(R), (int)C, sum->data_ptr<float>(), 0, cur_stream(x));
+  }
   return {q, s, qt, st, sum};
+}
+
+// out [M, N] (fp32 or bf16, unit column stride) (+)= A . B^T (+ bias) from split8's codes and scale words
+static void gemm8_run(const uint8_t* a, const uint8_t* as, int64_t M, const uint8_t* b, const uint8_t* bs, int64_t N, int64_t K,
+                      const Tensor& out, bool beta, const float* bias) {
+  const bool out_bf16 = out.scalar_type() == torch::kBFloat16;
+  const int es = out_bf16 ? 2 : 4;
+  HxGemm8 g{};
+  g.A = a;
+  g.sa = reinterpret_cast<const uint32_t*>(as);
+  g.B = b;
+  g.sb = reinterpret_cast<const uint32_t*>(bs);
+  g.lda = g.ldb = blocks128(K) * 128;
+  g.C = out.data_ptr();
+  g.ldc = M > 1 ? out.stride(0) : N;
+  g.bias = bias;
+  g.M = (int)M;
+  g.N = (int)N;
+  g.nkb = (int)blocks128(K);
+  g.beta = beta ? 1 : 0;
+  int cfg = 0;
+  hx_gemm_fp8_plan(g.M, g.N, g.nkb, out_bf16 ? 0 : 1, &cfg, &g.ks);
+  g.vec = aligned16(g.C) && g.ldc * es % 16 == 0 && N * es % 16 == 0;
+  const hipStream_t stream = cur_stream(out);
+  if (g.ks > 1) {
+    Tensor part = torch::empty({g.ks, M, N}, out.options().dtype(torch::kFloat32));
+    HxGemm8 p = g;
+    p.C = part.data_ptr();
+    p.ldc = N;
+    p.c_zs = M * N;
+    p.bias = nullptr;
+    p.beta = 0;
+    p.vec = N % 4 == 0;
+    TORCH_CHECK(hx_gemm_fp8(p, cfg, out_bf16 ? 0 : 1, 0, stream) == 0, "gemm_fp8: split-K launch failed");
+    hx_gemm_fp8_slabs(part.data_ptr<float>(), g.C, out_bf16, g.ldc, g.M, g.N, g.ks, g.bias, g.beta,
+                      N % 4 == 0 && aligned16(g.C) && g.ldc % 4 == 0 && (!out_bf16 || g.ldc % 8 == 0), stream);
+  } else {
+    TORCH_CHECK(hx_gemm_fp8(g, cfg, out_bf16 ? 0 : 1, out_bf16 ? 1 : 0, stream) == 0, "gemm_fp8: launch failed");
+  }
 }
 
 // C [M, N] (+)= A . B^T (+ bias) on split8's codes: A (q, s) of an [M, K] operand, B of an [N, K] one.
@@ -817,40 +873,8 @@ Tensor gemm_fp8(Tensor a, Tensor as, Tensor b, Tensor bs, int64_t K, bool out_bf
                   (out.stride(1) == 1 || N == 1) && (M <= 1 || out.stride(0) >= N),
               "gemm_fp8: out must be [M, N] of the result type with unit column stride");
   if (M == 0 || N == 0) return out;
-  const int es = out_bf16 ? 2 : 4;
-  HxGemm8 g{};
-  g.A = a.data_ptr<uint8_t>();
-  g.lda = a.size(1);
-  g.sa = reinterpret_cast<const uint32_t*>(as.data_ptr());
-  g.B = b.data_ptr<uint8_t>();
-  g.ldb = b.size(1);
-  g.sb = reinterpret_cast<const uint32_t*>(bs.data_ptr());
-  g.C = out.data_ptr();
-  g.ldc = M > 1 ? out.stride(0) : N;
-  g.bias = ptr_or_null<float>(bias);
-  g.M = (int)M;
-  g.N = (int)N;
-  g.nkb = (int)nkb;
-  g.beta = beta ? 1 : 0;
-  int cfg = 0;
-  hx_gemm_fp8_plan(g.M, g.N, g.nkb, out_bf16 ? 0 : 1, &cfg, &g.ks);
-  g.vec = aligned16(g.C) && g.ldc * es % 16 == 0 && N * es % 16 == 0;
-  Tensor part;
-  if (g.ks > 1) {
-    part = torch::empty({g.ks, M, N}, a.options().dtype(torch::kFloat32));
-    HxGemm8 p = g;
-    p.C = part.data_ptr();
-    p.ldc = N;
-    p.c_zs = M * N;
-    p.bias = nullptr;
-    p.beta = 0;
-    p.vec = N % 4 == 0;
-    TORCH_CHECK(hx_gemm_fp8(p, cfg, out_bf16 ? 0 : 1, 0, cur_stream(a)) == 0, "gemm_fp8: split-K launch failed");
-    hx_gemm_fp8_slabs(part.data_ptr<float>(), g.C, out_bf16, g.ldc, g.M, g.N, g.ks, g.bias, g.beta,
-                      N % 4 == 0 && aligned16(g.C) && g.ldc % 4 == 0 && (!out_bf16 || g.ldc % 8 == 0), cur_stream(a));
-  } else {
-    TORCH_CHECK(hx_gemm_fp8(g, cfg, out_bf16 ? 0 : 1, out_bf16 ? 1 : 0, cur_stream(a)) == 0, "gemm_fp8: launch failed");
-  }
+  gemm8_run(a.data_ptr<uint8_t>(), as.data_ptr<uint8_t>(), M, b.data_ptr<uint8_t>(), bs.data_ptr<uint8_t>(), N, K, out, beta,
+            ptr_or_null<float>(bias));
   dbg_finite(out, "gemm_fp8");
   return out;
 }
@@ -904,25 +928,75 @@ std::vector<OptT> linear_fp8_fwd(Tensor x2, Tensor wq, Tensor ws, OptT bias, boo
   return {y, qt, st};
 }
 
+// codes and scale words of an operand [rows, n] inside a workspace
+inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+struct Codes8 {
+  int64_t rows, n, qb, sb;   // bytes of the codes and of the scale words, 256-B steps
+  Codes8(int64_t rows_, int64_t n_, bool on = true)
+      : rows(rows_), n(n_), qb(on ? up256(rows_ * blocks128(n_) * 128) : 0), sb(on ? up256((blocks128(n_) + 3) / 4 * ((rows_ + 3) / 4) * 16) : 0) {}
+  int64_t bytes() const { return qb + sb; }
+  uint8_t* q(uint8_t* base) const { return bytes() ? base : nullptr; }
+  uint8_t* s(uint8_t* base) const { return bytes() ? base + qb : nullptr; }
+};
+
 // The whole layer as one autograd node for parameters that autograd accumulates itself (no flat gradient
-// slots, no residual mailbox): a small layer's step is bound by the host, and a node in C++ runs its
-// backward without the interpreter lock (ops/fp8.py: training step of 41 x 1024 x 1024)
+// slots, no residual mailbox).  A small layer's step is bound by the host: a node in C++ runs its
+// backward without the interpreter lock, all of a direction's codes share one workspace, and x and W
+// are split in one launch (training step of 41 x 1024 x 1024: 164 us of host through Python and single
+// calls).
 struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
-  static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor x, OptT W, OptT b, Tensor wq, Tensor ws, OptT wqt,
-                        OptT wst, bool keep) {
-    const int64_t N = wq.size(0);
-    Tensor x2 = as_rows8(x);
-    OptT qt, st;
-    Tensor y = linear_fp8_y(x2.detach(), wq, ws, has(b) ? OptT(b->detach()) : OptT(), keep, &qt, &st);
-    ctx->save_for_backward({qt.value_or(Tensor()), st.value_or(Tensor()), wqt.value_or(Tensor()), wst.value_or(Tensor())});
+  static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor x, OptT W, OptT b, OptT wq, OptT ws, OptT wqt, OptT wst,
+                        bool grad) {
+    const bool own = !has(wq);   // W's codes are made here
+    const int64_t K = x.size(-1), N = own ? W->size(0) : wq->size(0);
+    Tensor x2 = as_rows8(x.detach());
+    const int64_t M = x2.size(0);
+    const bool keep = grad && has(W) && W->requires_grad(), wt = grad && x.requires_grad();
+    OptT bias = has(b) ? OptT(b->detach()) : OptT();
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = N;
+    Tensor y, kept, wkept;
+    if (!own && !keep) {
+      y = linear_fp8_y(x2, *wq, *ws, bias, false, nullptr, nullptr);
+    } else {
+      check_rows8(x2, "linear_fp8");
+      check_bias8(bias, N, x2, "linear_fp8 bias");
+      Tensor W2 = own ? as_rows8(W->detach()) : Tensor();
+      if (own) check_rows8(W2, "linear_fp8 weight");
+      TORCH_CHECK(!keep || M <= (1LL << 22), "linear_fp8: at most 2^22 rows in a training step");
+      TORCH_CHECK(!own || N <= (1LL << 22), "linear_fp8: at most 2^22 output features");
+      c10::hip::HIPGuardMasqueradingAsCUDA guard(x2.device());
+      const auto u8 = x2.options().dtype(torch::kUInt8);
+      const Codes8 cx(M, K), cxt(K, M, keep), cw(N, K, own), cwt(K, N, own && wt);
+      Tensor tmp = torch::empty({cx.bytes() + cw.bytes()}, u8);
+      if (keep && M > 0) kept = torch::empty({cxt.bytes()}, u8);
+      if (cwt.bytes()) wkept = torch::empty({cwt.bytes()}, u8);
+      uint8_t *px = tmp.data_ptr<uint8_t>(), *pw = px + cx.bytes();
+      uint8_t* pk = kept.defined() ? kept.data_ptr<uint8_t>() : nullptr;
+      uint8_t* pt = wkept.defined() ? wkept.data_ptr<uint8_t>() : nullptr;
+      HxSplit8 jobs[2];
+      int n = 0;
+      if (M > 0) jobs[n++] = split8_job(x2, cx.q(px), cx.s(px), cxt.q(pk), pk ? cxt.s(pk) : nullptr, nullptr);
+      if (own) jobs[n++] = split8_job(W2, cw.q(pw), cw.s(pw), cwt.q(pt), pt ? cwt.s(pt) : nullptr, nullptr);
+      if (n) hx_split8(jobs, n, cur_stream(x2));
+      y = torch::empty({M, N}, x2.options());
+      if (M > 0) {
+        if (!own)
+          TORCH_CHECK(wq->is_cuda() && wq->device() == x2.device() && wq->size(1) == blocks128(K) * 128 && wq->is_contiguous(),
+                      "linear_fp8: the weight's codes do not fit x");
+        gemm8_run(cx.q(px), cx.s(px), M, own ? cw.q(pw) : wq->data_ptr<uint8_t>(), own ? cw.s(pw) : ws->data_ptr<uint8_t>(), N, K, y,
+                  false, ptr_or_null<float>(bias));
+        dbg_finite(y, "linear_fp8");
+      }
+    }
+    ctx->save_for_backward({kept, own ? wkept : wqt.value_or(Tensor()), own ? Tensor() : wst.value_or(Tensor())});
     ctx->saved_data["xshape"] = x.sizes().vec();
     ctx->saved_data["N"] = N;
+    ctx->saved_data["own"] = own;
     ctx->saved_data["wbf16"] = has(W) && W->scalar_type() == torch::kBFloat16;
     // the inputs that are there have the first edges, in order
     ctx->saved_data["ew"] = has(W) ? 1 : 0;
     ctx->saved_data["eb"] = has(b) ? (has(W) ? 2 : 1) : 0;
-    std::vector<int64_t> shape = x.sizes().vec();
-    shape.back() = N;
     return y.view(shape);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
@@ -931,34 +1005,46 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
     const int64_t N = ctx->saved_data["N"].toInt(), K = xshape.back();
     const int64_t ew = ctx->saved_data["ew"].toInt(), eb = ctx->saved_data["eb"].toInt();
     const bool need_x = ctx->needs_input_grad(0), need_w = ew && ctx->needs_input_grad(ew), need_b = eb && ctx->needs_input_grad(eb);
-    Tensor dy2 = as_rows8(g[0]);
-    const int64_t M = dy2.size(0);
-    const bool bf16 = dy2.scalar_type() == torch::kBFloat16;
-    std::vector<OptT> c = split8(dy2, need_x, need_w && M > 0, need_b, c10::nullopt);
-    Tensor dx, dW;
-    if (need_w) {
-      if (M == 0) dW = torch::zeros({N, K}, dy2.options().dtype(torch::kFloat32));
-      else dW = gemm_fp8(*c[2], *c[3], saved[0], saved[1], M, false, c10::nullopt, false, c10::nullopt);
-      if (ctx->saved_data["wbf16"].toBool()) dW = dW.to(torch::kBFloat16);
+    const bool own = ctx->saved_data["own"].toBool();
+    Tensor dy = as_rows8(g[0]);
+    check_rows8(dy, "linear_fp8 output gradient");
+    const int64_t M = dy.size(0);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(dy.device());
+    const auto f32 = dy.options().dtype(torch::kFloat32);
+    Tensor dx, dW, db;
+    if (need_x) dx = torch::empty({M, K}, dy.options());
+    if (need_w) dW = M > 0 ? torch::empty({N, K}, f32) : torch::zeros({N, K}, f32);
+    if (need_b) db = M > 0 ? torch::empty({N}, f32) : torch::zeros({N}, f32);
+    if (M > 0) {
+      const Codes8 cd(M, N, need_x), cdt(N, M, need_w), cxt(K, M, need_w), cwt(K, N, own);
+      const int64_t part = need_b ? up256(hx_split8_row_tiles(M) * N * 4) : 0;
+      Tensor tmp = torch::empty({cd.bytes() + cdt.bytes() + part}, dy.options().dtype(torch::kUInt8));
+      uint8_t *pd = tmp.data_ptr<uint8_t>(), *pt = pd + cd.bytes(), *pp = pt + cdt.bytes();
+      const HxSplit8 job = split8_job(dy, cd.q(pd), cd.s(pd), cdt.q(pt), cdt.s(pt), need_b ? reinterpret_cast<float*>(pp) : nullptr);
+      hx_split8(&job, 1, cur_stream(dy));
+      if (need_b) hx_fold_cols(reinterpret_cast<float*>(pp), hx_split8_row_tiles(M), (int)N, db.data_ptr<float>(), 0, cur_stream(dy));
+      if (need_w) {
+        uint8_t* pk = saved[0].data_ptr<uint8_t>();
+        gemm8_run(cdt.q(pt), cdt.s(pt), N, cxt.q(pk), cxt.s(pk), K, M, dW, false, nullptr);
+        dbg_finite(dW, "linear_fp8 weight gradient");
+      }
+      if (need_x) {
+        uint8_t* pw = saved[1].data_ptr<uint8_t>();
+        gemm8_run(cd.q(pd), cd.s(pd), M, pw, own ? cwt.s(pw) : saved[2].data_ptr<uint8_t>(), K, N, dx, false, nullptr);
+        dbg_finite(dx, "linear_fp8 input gradient");
+      }
     }
-    if (need_x) dx = gemm_fp8(*c[0], *c[1], saved[2], saved[3], N, bf16, c10::nullopt, false, c10::nullopt).view(xshape);
-    return {dx, dW, need_b ? *c[4] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    if (need_x) dx = dx.view(xshape);
+    if (need_w && ctx->saved_data["wbf16"].toBool()) dW = dW.to(torch::kBFloat16);
+    return {dx, dW, db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 // W: the parameter whose gradient is wanted (or none); w8: its codes and scales (wq, ws, wqt, wst -- the
-// last two may be absent), or none: they are made here from W
+// last two may be absent), or empty: they are made from W
 Tensor linear_fp8(Tensor x, OptT W, OptT b, std::vector<OptT> w8, bool grad) {
-  OptT wq, ws, wqt, wst;
-  if (w8.empty()) {
-    TORCH_CHECK(has(W), "linear_fp8: a weight or its codes");
-    std::vector<OptT> c = split8(as_rows8(W->detach()), true, grad && x.requires_grad(), false, c10::nullopt);
-    wq = c[0]; ws = c[1]; wqt = c[2]; wst = c[3];
-  } else {
-    TORCH_CHECK(w8.size() == 4 && has(w8[0]) && has(w8[1]), "linear_fp8: the weight's codes and scales");
-    wq = w8[0]; ws = w8[1]; wqt = w8[2]; wst = w8[3];
-  }
-  const bool keep = grad && has(W) && W->requires_grad();
-  return LinearFp8::apply(x, W, b, *wq, *ws, wqt, wst, keep);
+  TORCH_CHECK(w8.empty() ? has(W) : w8.size() == 4 && has(w8[0]) && has(w8[1]), "linear_fp8: a weight or its codes and scales");
+  if (w8.empty()) return LinearFp8::apply(x, W, b, OptT(), OptT(), OptT(), OptT(), grad);
+  return LinearFp8::apply(x, W, b, w8[0], w8[1], w8[2], w8[3], grad);
 }
 
 // ---- int8 blocks along the last dimension (contiguous rows): codes [rows, nb, 128], scale bytes [rows, nb]

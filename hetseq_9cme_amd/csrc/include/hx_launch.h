@@ -237,11 +237,22 @@ void hx_spin(int blocks, double us, int lds_bytes, uint32_t* sink, hipStream_t s
 // quant8.hip -- 8-bit blocks of 128 (hx_quant.h).  vec: rows allow 16-B accesses.
 // split8: x [R, C] (row stride ld) -> e4m3 codes q [R, 128 ceil(C / 128)] blocked along the columns and
 // / or qt [C, 128 ceil(R / 128)] blocked along the rows (either may be null), with their scale bytes s /
-// st (block b of row r at ((b / 4) Rs + r) 4 + b % 4, Rs = rows rounded up to 4), and / or the column
-// sums (colpart: [row tiles][C] fp32 workspace, with colsum [C])
+// st (block b of row r at ((b / 4) Rs + r) 4 + b % 4, Rs = rows rounded up to 4), and / or column sums
+// per row tile (colpart: [row tiles][C] fp32, to be folded); one or two tensors in one launch
+struct HxSplit8 {
+  int bf16;
+  const void* x;
+  int64_t ld;
+  int R, C;
+  uint8_t* q;
+  uint8_t* s;
+  uint8_t* qt;
+  uint8_t* st;
+  float* colpart;
+  int vec;
+};
 int hx_split8_row_tiles(int64_t R);
-void hx_split8(int bf16, const void* x, int64_t ld, int R, int C, uint8_t* q, uint8_t* s, uint8_t* qt, uint8_t* st,
-               float* colpart, float* colsum, int vec, hipStream_t stream);
+void hx_split8(const HxSplit8* jobs, int n, hipStream_t stream);
 // int8 blocks along contiguous rows of N: codes [rows][nb][128], scale bytes [rows][nb], nb = ceil(N / 128)
 void hx_gelu8_fwd(int bf16, const void* y, const float* b, void* out, uint8_t* q, uint8_t* s, int64_t rows, int N,
                   int vec, hipStream_t stream);

@@ -7,6 +7,8 @@
 //  * gelu8_fwd   out = gelu(y + b), and y kept as int8 blocks
 //  * gelu8_bwd   dy = dout gelu'(y^ + b) with y^ decoded from the blocks, and the column sums of dy
 //  * pack8 / unpack8   x <-> its int8 blocks
+#include <type_traits>
+
 #include "hx_launch.h"
 #include "hx_quant.h"
 #include "hx_reduce.h"
@@ -23,18 +25,6 @@ constexpr int NT = 256;
 // lanes, and the thread's 4 consecutive rows are 4 consecutive bytes of a transposed row.
 // Bound by memory where there are many tiles (dy of 16384 x 2304 bf16, 150 MB read and written),
 // by one tile's chain of loads, maxima and stores where there are few.
-struct Split8 {
-  const void* x;
-  int64_t ld;
-  int R, C;
-  uint8_t* q;        // [R, Cp] codes blocked along the columns (null: not wanted), Cp = 128 ceil(C / 128)
-  uint8_t* s;        // their scale bytes: block b of row r at ((b / 4) Rs + r) 4 + b % 4, Rs = R rounded up to 4
-  uint8_t* qt;       // [C, Rp] codes blocked along the rows (null: not wanted)
-  uint8_t* st;
-  float* colpart;    // [row tiles][C] column sums (null: not wanted)
-  int vec;
-};
-
 constexpr int SNT = 512, SR = 4;   // threads, rows per thread
 constexpr uint32_t kInf = 0x7f800000u;
 
@@ -104,16 +94,22 @@ struct TileBf16 {
   }
 };
 
-template <typename Tile>
-__global__ __launch_bounds__(SNT) void split8_k(Split8 a) {
+struct Split8Lds {
   // transposed codes, 128 rows of 128 B; 16-B chunk ch of row c at ch ^ (c / 8 % 8): the writes of a
   // wave (16 columns, 8 apart, of one chunk) and the reads (8 chunks of a row) spread over the banks
-  __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
-  __shared__ uint32_t redm[SNT / 64][128];
-  __shared__ float reds[SNT / 64][128];
+  uint8_t tile[128 * 128];
+  uint32_t redm[SNT / 64][128];
+  float reds[SNT / 64][128];
+};
+
+template <typename Tile>
+__device__ __forceinline__ void split8_tile(const HxSplit8& a, int bid, Split8Lds& lds) {
+  auto& tile = lds.tile;
+  auto& redm = lds.redm;
+  auto& reds = lds.reds;
   const int t = threadIdx.x, cg = t & 15, rg = t >> 4, w = t >> 6;
   const int nc = (a.C + 127) / 128;
-  const int cb = blockIdx.x % nc, rb = blockIdx.x / nc;
+  const int cb = bid % nc, rb = bid / nc;
   const int c0 = cb * 128 + 8 * cg, r0 = rb * 128 + SR * rg;
   const int64_t Rs = (a.R + 3) & ~3, Cs = (a.C + 3) & ~3;
   const int Cp = (a.C + 127) / 128 * 128, Rp = (a.R + 127) / 128 * 128;
@@ -197,6 +193,21 @@ __global__ __launch_bounds__(SNT) void split8_k(Split8 a) {
     if (cb * 128 + c < a.C)
       *reinterpret_cast<uint4*>(a.qt + (int64_t)(cb * 128 + c) * Rp + rb * 128 + 16 * ch) =
           *reinterpret_cast<const uint4*>(tile + c * 128 + 16 * (ch ^ ((c >> 3) & 7)));
+  }
+}
+
+__device__ __forceinline__ int split8_tiles(const HxSplit8& a) { return ((a.C + 127) / 128) * ((a.R + 127) / 128); }
+
+// the tiles of a, then those of b (TB = void: a alone)
+template <typename TA, typename TB>
+__global__ __launch_bounds__(SNT) void split8_k(HxSplit8 a, HxSplit8 b) {
+  __shared__ __attribute__((aligned(16))) Split8Lds lds;
+  if constexpr (std::is_same_v<TB, void>) {
+    split8_tile<TA>(a, blockIdx.x, lds);
+  } else {
+    const int na = split8_tiles(a);   // uniform over the workgroup
+    if ((int)blockIdx.x < na) split8_tile<TA>(a, blockIdx.x, lds);
+    else split8_tile<TB>(b, blockIdx.x - na, lds);
   }
 }
 
@@ -339,13 +350,19 @@ inline unsigned stream_grid(int64_t nblk) {   // one pass up to 16 workgroups pe
 
 int hx_split8_row_tiles(int64_t R) { return (int)((R + 127) / 128); }
 
-void hx_split8(int bf16, const void* x, int64_t ld, int R, int C, uint8_t* q, uint8_t* s, uint8_t* qt, uint8_t* st,
-               float* colpart, float* colsum, int vec, hipStream_t stream) {
-  Split8 a{x, ld, R, C, q, s, qt, st, colpart, vec};
-  const unsigned grid = (unsigned)(((C + 127) / 128) * (int64_t)((R + 127) / 128));
-  if (bf16) split8_k<TileBf16><<<grid, SNT, 0, stream>>>(a);
-  else split8_k<TileF32><<<grid, SNT, 0, stream>>>(a);
-  if (colpart) fold_rows(colpart, hx_split8_row_tiles(R), C, C, C, colsum, nullptr, nullptr, 0, stream);
+void hx_split8(const HxSplit8* jobs, int n, hipStream_t stream) {
+  auto tiles = [](const HxSplit8& j) { return (unsigned)(((j.C + 127) / 128) * (int64_t)((j.R + 127) / 128)); };
+  const HxSplit8 &a = jobs[0], &b = jobs[n > 1 ? 1 : 0];
+  if (n == 1) {
+    if (a.bf16) split8_k<TileBf16, void><<<tiles(a), SNT, 0, stream>>>(a, b);
+    else split8_k<TileF32, void><<<tiles(a), SNT, 0, stream>>>(a, b);
+    return;
+  }
+  const unsigned grid = tiles(a) + tiles(b);
+  if (a.bf16 && b.bf16) split8_k<TileBf16, TileBf16><<<grid, SNT, 0, stream>>>(a, b);
+  else if (a.bf16) split8_k<TileBf16, TileF32><<<grid, SNT, 0, stream>>>(a, b);
+  else if (b.bf16) split8_k<TileF32, TileBf16><<<grid, SNT, 0, stream>>>(a, b);
+  else split8_k<TileF32, TileF32><<<grid, SNT, 0, stream>>>(a, b);
 }
 
 void hx_gelu8_fwd(int bf16, const void* y, const float* b, void* out, uint8_t* q, uint8_t* s, int64_t rows, int N,
