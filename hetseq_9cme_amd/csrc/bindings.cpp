@@ -831,7 +831,8 @@ static void gemm8_run(const uint8_t* a, const uint8_t* as, int64_t M, const uint
   g.beta = beta ? 1 : 0;
   int cfg = 0;
   hx_gemm_fp8_plan(g.M, g.N, g.nkb, out_bf16 ? 0 : 1, &cfg, &g.ks);
-  g.vec = aligned16(g.C) && g.ldc * es % 16 == 0 && N * es % 16 == 0;
+  // 16-B stores, and a tile's 256 rows within one buffer descriptor
+  g.vec = aligned16(g.C) && g.ldc * es % 16 == 0 && N * es % 16 == 0 && 256 * g.ldc * es < (1LL << 31);
   const hipStream_t stream = cur_stream(out);
   if (g.ks > 1) {
     Tensor part = torch::empty({g.ks, M, N}, out.options().dtype(torch::kFloat32));
@@ -841,7 +842,7 @@ static void gemm8_run(const uint8_t* a, const uint8_t* as, int64_t M, const uint
     p.c_zs = M * N;
     p.bias = nullptr;
     p.beta = 0;
-    p.vec = N % 4 == 0;
+    p.vec = N % 4 == 0 && 1024 * N < (1LL << 31);
     TORCH_CHECK(hx_gemm_fp8(p, cfg, out_bf16 ? 0 : 1, 0, stream) == 0, "gemm_fp8: split-K launch failed");
     hx_gemm_fp8_slabs(part.data_ptr<float>(), g.C, out_bf16, g.ldc, g.M, g.N, g.ks, g.bias, g.beta,
                       N % 4 == 0 && aligned16(g.C) && g.ldc % 4 == 0 && (!out_bf16 || g.ldc % 8 == 0), stream);

@@ -32,6 +32,14 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 
+// a wave-uniform descriptor chosen from two, kept in scalar registers
+__device__ __forceinline__ u32x4 pick(bool first, const u32x4& a, const u32x4& b) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(first ? a[i] : b[i]);
+  return r;
+}
+
 __device__ __forceinline__ void raw_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // 8 codes (two words of a fragment) -> bf16 values times s
@@ -43,118 +51,134 @@ __device__ __forceinline__ bf16x8v decode8(int w0, int w1, float s) {
   return bf16x8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// C[M][N] on a BM x BN tile per workgroup, (BM / WM)(BN / WN) waves of WM x WN.
-// LDS: NS stages of KS codes of every row of the tile, filled by LDS-DMA, and two slots of scale
-// words (one word = 4 blocks of a row).  A k block is two 64-deep halves: while the MFMAs of one run
-// on fragments in registers, the fragments of the next are read.  A stage is opened (`open`) by a
-// counted vmcnt and one raw barrier, which also frees the stage before it for the next DMA.
-template <int BM, int BN, int WM, int WN, int KS, int NS, int WGS, bool EXACT, bool OB>
+// C[M][N] in tiles of BM x BN, (BM / WM)(BN / WN) waves of WM x WN, one k block (128 codes of every row)
+// per stage, two stages of LDS.  Persistent: a workgroup takes the tiles (and slabs) of its XCD's share
+// in turn, and its streams of stages, scale words and biases run on from one tile into the next, so the
+// first loads of a tile are under way while the one before it is stored.
+//
+// A k block is two 64-deep halves: while the MFMAs of one run on fragments in registers, the fragments
+// of the next are read.  A stage is opened (`open`) by a counted vmcnt and one raw barrier, which also
+// frees the stage before it for the next DMA.
+template <int BM, int BN, int WM, int WN, int WGS, bool EXACT, bool OB>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) * WGS / 4) void gemm_fp8_k(HxGemm8 g) {
   constexpr int NWM = BM / WM, NWN = BN / WN, NW = NWM * NWN;
   constexpr int MB = WM / 32, NB = WN / 32;
-  static_assert(KS == 64 || KS == 128, "stage depth");
-  constexpr int RPP = 1024 / KS;                       // rows per 1-KiB DMA piece
-  constexpr int KA = BM / RPP, KB = BN / RPP, J = (KA + KB) / NW;
-  static_assert((KA + KB) % NW == 0 && BM % RPP == 0 && BN % RPP == 0, "whole DMA pieces per wave");
+  constexpr int KA = BM / 8, KB = BN / 8, J = (KA + KB) / NW;   // 1-KiB DMA pieces (8 rows) per stage; per wave
+  static_assert((KA + KB) % NW == 0, "whole DMA pieces per wave");
   static_assert(BM <= 256 && BN <= 256 && NW >= 3, "one DMA piece of scale words per operand");
-  constexpr int STAGE = (BM + BN) * KS, SCALES = NS * STAGE;   // + 2 slots x (A, B) x 1 KiB
-  constexpr int BIAS = SCALES + 4096, SPARE = BIAS + 1024;      // the tile's bias; where idle pieces land
+  // LDS: two stages, two slots of scale words (A 1 KiB, B 1 KiB; one word = 4 k blocks of a row), the
+  // biases of two tiles, and where idle DMA pieces land
+  constexpr int STAGE = (BM + BN) * 128, SCALES = 2 * STAGE, BIAS = SCALES + 4096, SPARE = BIAS + 2048;
+  constexpr int STORES = MB * NB * (OB ? 2 : 4);   // of a lane in the epilogue
+  static_assert(STORES < 63, "counted by vmcnt");
   extern __shared__ __attribute__((aligned(16))) char lds[];
 
-  const int TM = (g.M + BM - 1) / BM, TN = (g.N + BN - 1) / BN, total = TM * TN;
-  const int per = (total * g.ks + 7) / 8;
-  const int work0 = (blockIdx.x % 8) * per + blockIdx.x / 8;   // tiles dealt XCD by XCD
-  if (work0 >= total * g.ks || (int)(blockIdx.x / 8) >= per) return;   // uniform per workgroup
-  const int z = work0 / total, work = work0 - z * total;
-  const int nt = work % TN, mt = work / TN;
-  const int m0 = mt * BM, n0 = nt * BN;
-  // k blocks of this slab: whole groups of four (one scale word)
+  const int TM = (g.M + BM - 1) / BM, TN = (g.N + BN - 1) / BN, tiles = TM * TN;
+  // work items (slab, tile) dealt XCD by XCD: items [x per, x per + per) to the workgroups of XCD x
+  const int per = (tiles * g.ks + 7) / 8, step = gridDim.x / 8;
+  const int first = (blockIdx.x % 8) * per + blockIdx.x / 8;
+  const int end = min((int)(blockIdx.x % 8) * per + per, tiles * g.ks);
+  if (first >= end) return;   // uniform per workgroup
+  // k blocks of a slab: whole groups of four
   const int groups = (g.nkb + 3) / 4, gper = (groups + g.ks - 1) / g.ks;
-  const int kb0 = min(z * gper * 4, g.nkb), kb1 = min(kb0 + gper * 4, g.nkb);
+  struct Item {
+    int m0, n0, z, kb0, n;
+  };
+  auto item = [&](int w) {
+    Item t;
+    t.z = w / tiles;
+    const int r = w - t.z * tiles;
+    t.m0 = r / TN * BM;
+    t.n0 = (r - r / TN * TN) * BN;
+    t.kb0 = t.z * gper * 4;
+    t.n = min(gper * 4, g.nkb - t.kb0);   // >= 1: the plan makes no empty slab
+    return t;
+  };
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wv % NWM, wn = wv / NWM, h = lane >> 5, l32 = lane & 31;
-
-  const int mrows = min(BM, g.M - m0), nrows = min(BN, g.N - n0);
-  const u32x4 ra = rsrc_of(g.A + (int64_t)m0 * g.lda, (uint32_t)(mrows * g.lda));
-  const u32x4 rb = rsrc_of(g.B + (int64_t)n0 * g.ldb, (uint32_t)(nrows * g.ldb));
   const int64_t sam = (g.M + 3) & ~3, sbn = (g.N + 3) & ~3;
-  // wave 0 fetches the scale words of A's rows, wave 1 B's, wave 2 the bias
-  const char* xp = (const char*)(wv == 0 ? (const void*)(g.sa + m0) : wv == 1 ? (const void*)(g.sb + n0) : (const void*)(g.bias + n0));
-  const uint32_t xbytes = wv == 0 ? (uint32_t)((groups * sam - m0) * 4) : wv == 1 ? (uint32_t)((groups * sbn - n0) * 4)
-                          : wv == 2 && g.bias ? (uint32_t)(g.N - n0) * 4 : 0u;
-  const u32x4 rx = rsrc_of(xp, xbytes);
   const uint32_t lds0 = (uint32_t)(size_t)(lds_void*)lds;
+  constexpr uint32_t NONE = 0x80000000u;   // an offset past every buffer: zeros, no memory traffic, still counted
 
-  // lane L of a DMA piece fetches (row L / (KS / 16), 16-B chunk c) so that the lane-linear LDS
-  // write lands chunk c of row r at position c ^ swz(r): fragment reads are free of bank conflicts
+  // Lane L of a DMA piece fetches 16-B chunk L % 8 ^ swz of row L / 8 so that the
+  // lane-linear LDS write lands chunk c of row r at position c ^ (r / 2 % 8): fragment reads are free of
+  // bank conflicts
   uint32_t voff[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    const int q = wv + NW * j, r = (q < KA ? q : q - KA) * RPP + lane / (KS / 16);
-    const int c = (lane % (KS / 16)) ^ (KS == 128 ? (r >> 1) & 7 : (r >> 2) & 3);
-    voff[j] = (uint32_t)(r * (q < KA ? g.lda : g.ldb) + 16 * c);
+    const int q = wv + NW * j, r = (q < KA ? q : q - KA) * 8 + lane / 8;
+    voff[j] = (uint32_t)(r * (q < KA ? g.lda : g.ldb) + 16 * ((lane % 8) ^ ((r >> 1) & 7)));
   }
-  constexpr int SPB = 128 / KS;   // stages per k block
-  const int st1 = (kb1 - kb0) * SPB;
-  auto dma_one = [&](int st, int j) {   // piece j of this wave for stage st
-    // past the slab's end: an offset past every buffer (zeros, no memory traffic, still counted)
-    const uint32_t ko = st < st1 ? (uint32_t)(kb0 * 128 + st * KS) : 0x80000000u;
+  // what a tile's DMA needs; `next` is the tile after the one in work (its loads start two stages early)
+  struct Src {
+    u32x4 a, b, x;   // A's and B's rows; wave 0: scale words of A's rows, wave 1: of B's, wave 2: the bias
+    uint32_t ko, so;   // byte offsets of the first k block in a row, of the first scale words (NONE: no such tile)
+  };
+  auto source = [&](const Item& t, bool some) {
+    Src s;
+    s.a = rsrc_of(g.A + (int64_t)t.m0 * g.lda, (uint32_t)(min(BM, g.M - t.m0) * g.lda));
+    s.b = rsrc_of(g.B + (int64_t)t.n0 * g.ldb, (uint32_t)(min(BN, g.N - t.n0) * g.ldb));
+    const char* p = (const char*)(wv == 0 ? (const void*)(g.sa + t.m0) : wv == 1 ? (const void*)(g.sb + t.n0) : (const void*)(g.bias + t.n0));
+    const uint32_t bytes = wv == 0 ? (uint32_t)((groups * sam - t.m0) * 4) : wv == 1 ? (uint32_t)((groups * sbn - t.n0) * 4)
+                           : wv == 2 && g.bias ? (uint32_t)(g.N - t.n0) * 4 : 0u;
+    s.x = rsrc_of(p, bytes);
+    s.ko = some ? (uint32_t)t.kb0 * 128u : NONE;
+    s.so = !some ? NONE : wv < 2 ? (uint32_t)((t.kb0 >> 2) * (wv == 0 ? sam : sbn) * 4) : 0u;
+    return s;
+  };
+  auto dma_one = [&](const u32x4& a, const u32x4& b, uint32_t ko, int slot, int j) {
     const int q = wv + NW * j;
-    dma16(q < KA ? ra : rb, lds0 + (uint32_t)(st % NS) * STAGE + 1024u * q, voff[j] + ko);
+    dma16(pick(q < KA, a, b), lds0 + (uint32_t)slot * STAGE + 1024u * q, voff[j] + ko);
   };
-  auto dma = [&](int st) {
-#pragma unroll
-    for (int j = 0; j < J; ++j) dma_one(st, j);
-  };
-  auto dma_scales = [&](int grp, bool first) {   // scale words of k blocks 4 grp .. + 3 (and, first, the bias)
-    const uint32_t dst = wv < 2 ? SCALES + (uint32_t)(grp & 1) * 2048 + wv * 1024 : first && wv == 2 ? BIAS : SPARE;
-    const uint32_t off = wv < 2 ? (uint32_t)(grp * (wv == 0 ? sam : sbn) * 4) : 0u;
-    const bool some = wv < 2 ? grp < groups : first;
-    dma16(rx, lds0 + dst, (some ? off : 0x80000000u) + 16 * lane);
-  };
-  auto open = [&]() {   // the oldest stage in flight readable by every wave, the stage before it free
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    dma_wait<(NS - 2) * J>();
-    raw_barrier();
+  // the scale words of k blocks 4 grp .. + 3 of a tile, and with its first ones the bias
+  auto dma_scales = [&](const u32x4& x, uint32_t so, int grp, int slot, int bslot) {
+    const uint32_t dst = wv < 2 ? SCALES + slot * 2048 + wv * 1024 : wv == 2 && grp == 0 ? BIAS + bslot * 1024 : (uint32_t)SPARE;
+    const uint32_t off = wv < 2 ? so + (uint32_t)(grp * (wv == 0 ? sam : sbn) * 4) : wv == 2 && grp == 0 ? so : NONE;
+    dma16(pick(true, x, x), lds0 + dst, off + 16 * lane);
   };
 
   f32x16 acc[MB][NB];
-#pragma unroll
-  for (int a = 0; a < MB; ++a)
-#pragma unroll
-    for (int b = 0; b < NB; ++b) acc[a][b] = f32x16{0};
-
   auto frag = [&](const char* st, int row, int half) {
     const int r = row + l32;
-    const char* p = st + r * KS;
-    const int sw = KS == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
+    const char* p = st + r * 128;
+    const int sw = (r >> 1) & 7;
     const i32x4 lo = *reinterpret_cast<const i32x4*>(p + 16 * ((4 * half + h) ^ sw));
     const i32x4 hi = *reinterpret_cast<const i32x4*>(p + 16 * ((4 * half + 2 + h) ^ sw));
     return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
   i32x8 fa[MB], fb[2][NB];   // A's fragments are read again as soon as their MFMAs are issued, B's by turns
-  auto read_a = [&](int st, int half, int a) { fa[a] = frag(lds + (st % NS) * STAGE, wm * WM + 32 * a, half); };
-  auto read_b = [&](int st, int half, i32x8 (&f)[NB]) {
+  auto read_a = [&](int slot, int half, int a) { fa[a] = frag(lds + slot * STAGE, wm * WM + 32 * a, half); };
+  auto read_b = [&](int slot, int half, i32x8 (&f)[NB]) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) f[b] = frag(lds + (st % NS) * STAGE + BM * KS, wn * WN + 32 * b, half);
+    for (int b = 0; b < NB; ++b) f[b] = frag(lds + slot * STAGE + BM * 128, wn * WN + 32 * b, half);
   };
   uint32_t wa[MB], wb[NB];   // scale words, the current block's byte lowest
-  auto read_scales = [&](int grp) {
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(lds + SCALES + (grp & 1) * 2048);
+  auto read_scales = [&](int slot) {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(lds + SCALES + slot * 2048);
 #pragma unroll
     for (int a = 0; a < MB; ++a) wa[a] = p[wm * WM + 32 * a + l32];
 #pragma unroll
     for (int b = 0; b < NB; ++b) wb[b] = p[256 + wn * WN + 32 * b + l32];
   };
-  // The MFMAs of one half, and between them the reads of the next half's fragments (stage st, half
-  // `half`; OPEN: a new stage) and the DMA pieces of stage dst -- one after the other as written: a
-  // wave that issued its reads first would hold its MFMAs back until the LDS had served all waves'
-  // reads.  The stage is opened under the first MFMAs.
+  auto open = [&](uint32_t stores) {   // the next stage readable by every wave, the one before it free
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // its DMA is the oldest in flight; in a tile's first block the tile before it may still be storing
+    // (in one asm block: a branch that the compiler sees splits the MFMA sequence, which costs registers)
+    asm volatile("s_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 .Lopen%=\n\ts_waitcnt vmcnt(0)\n.Lopen%=:\n\ts_waitcnt vmcnt(%1)"
+                 ::"s"(__builtin_amdgcn_readfirstlane(stores)), "n"(STORES) : "memory", "scc");
+    raw_barrier();
+  };
+  // The MFMAs of one half, and between them the reads of the next half's fragments (OPEN: of the next
+  // stage, and the DMA pieces of the stage after it) -- one after the other as written: a wave that
+  // issued its reads first would hold its MFMAs back until the LDS had served all waves' reads.  The
+  // stage is opened under the first MFMAs.
   // Rows of the result run along n (the first MFMA operand): a lane holds 4 consecutive columns.
-  auto half_step = [&](const i32x8 (&bc)[NB], i32x8 (&bn)[NB], int st, int half, auto open_it, int dst) {
+  auto half_step = [&](const i32x8 (&bc)[NB], i32x8 (&bn)[NB], int slot, auto open_it, uint32_t stores, const u32x4& sa_, const u32x4& sb_,
+                       uint32_t ko) {
     constexpr bool OPEN = decltype(open_it)::value;
+    const int ns = OPEN ? slot ^ 1 : slot, half = OPEN ? 0 : 1;
     bf16x8v db[4][NB];
     if constexpr (EXACT)
 #pragma unroll
@@ -177,118 +201,148 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) *
       }
       __builtin_amdgcn_sched_barrier(0);
       if (a == 0) {
-        if constexpr (OPEN) open();
-        read_b(st, half, bn);
+        if constexpr (OPEN) open(stores);
+        read_b(ns, half, bn);
       }
-      read_a(st, half, a);
+      read_a(ns, half, a);
       if constexpr (OPEN)
 #pragma unroll
         for (int j = 0; j < J; ++j)
-          if (j * MB / J == a) dma_one(dst, j);
+          if (j * MB / J == a) dma_one(sa_, sb_, ko, slot, j);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  if (kb0 < kb1) {
-    dma_scales(kb0 / 4, true);
+  // ---- epilogue: a lane holds 4 consecutive columns of a row per quad of registers, the other half wave
+  // the next 4; bf16 quads change places in pairs so that every store is 16 B per lane
+  using OutT = std::conditional_t<OB, uint16_t, float>;
+  auto store = [&](const Item& t, int bslot_) {
+    OutT* C = (OutT*)g.C + (int64_t)t.z * g.c_zs + (int64_t)t.m0 * g.ldc;
+    const hx::Buf rc(C, g.vec ? (uint32_t)((int64_t)min(BM, g.M - t.m0) * g.ldc * sizeof(OutT)) : 0u);
+    const float* bias = reinterpret_cast<const float*>(lds + BIAS + bslot_ * 1024);
 #pragma unroll
-    for (int i = 0; i < NS; ++i) dma(i);
-    dma_wait<(NS - 1) * J>();   // the scale words and stage 0 landed
-    raw_barrier();
-    read_b(0, 0, fb[0]);
+    for (int a = 0; a < MB; ++a) {
+      const int lr = wm * WM + 32 * a + l32;
+      const bool in = t.m0 + lr < g.M;
+      OutT* row = C + (int64_t)lr * g.ldc;
 #pragma unroll
-    for (int a = 0; a < MB; ++a) read_a(0, 0, a);
-    constexpr std::true_type yes{};
-    constexpr std::false_type no{};
-    for (int kb = kb0; kb < kb1; ++kb) {
+      for (int b = 0; b < NB; ++b) {
+        float v[4][4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int lc = wn * WN + 32 * b + 8 * q + 4 * h, c = t.n0 + lc;
+          float4 bb = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (g.bias) bb = *reinterpret_cast<const float4*>(bias + lc);
+          v[q][0] = acc[a][b][4 * q] + bb.x;
+          v[q][1] = acc[a][b][4 * q + 1] + bb.y;
+          v[q][2] = acc[a][b][4 * q + 2] + bb.z;
+          v[q][3] = acc[a][b][4 * q + 3] + bb.w;
+          if (g.beta && in) {
+            if (g.vec) {
+              if (c < g.N) {
+                if constexpr (OB) {
+                  const uint2 w = *reinterpret_cast<const uint2*>(row + c);
+                  v[q][0] += __uint_as_float(w.x << 16); v[q][1] += __uint_as_float(w.x & 0xffff0000u);
+                  v[q][2] += __uint_as_float(w.y << 16); v[q][3] += __uint_as_float(w.y & 0xffff0000u);
+                } else {
+                  const float4 w = *reinterpret_cast<const float4*>(row + c);
+                  v[q][0] += w.x; v[q][1] += w.y; v[q][2] += w.z; v[q][3] += w.w;
+                }
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (c + i < g.N) v[q][i] += hx::io<OutT>::ld(row + c + i);
+            }
+          }
+        }
+        if (g.vec) {   // every lane of every store is issued (outside the tile: dropped), so they can be counted
+          const uint32_t ro = (uint32_t)(lr * g.ldc * sizeof(OutT));
+          if constexpr (OB) {
+#pragma unroll
+            for (int q = 0; q < 4; q += 2) {   // columns 8 q + 8 h .. + 8 after the exchange
+              const auto x = __builtin_amdgcn_permlane32_swap(bf16x2(v[q][0], v[q][1]), bf16x2(v[q + 1][0], v[q + 1][1]), false, false);
+              const auto y = __builtin_amdgcn_permlane32_swap(bf16x2(v[q][2], v[q][3]), bf16x2(v[q + 1][2], v[q + 1][3]), false, false);
+              const int c = t.n0 + wn * WN + 32 * b + 8 * q + 8 * h;
+              __builtin_amdgcn_raw_buffer_store_b128(u32x4{(uint32_t)x[0], (uint32_t)y[0], (uint32_t)x[1], (uint32_t)y[1]}, rc.r,
+                                                     in && c < g.N ? ro + c * 2 : NONE, 0, 0);
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int c = t.n0 + wn * WN + 32 * b + 8 * q + 4 * h;
+              const f32x4 x = {v[q][0], v[q][1], v[q][2], v[q][3]};
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), rc.r, in && c < g.N ? ro + c * 4 : NONE, 0, 0);
+            }
+          }
+        } else if (in) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int c = t.n0 + wn * WN + 32 * b + 8 * q + 4 * h + i;
+              if (c < g.N) hx::io<OutT>::st(row + c, v[q][i]);
+            }
+        }
+      }
+    }
+    if (!g.vec) dma_wait<0>();   // stores that `open` does not count
+  };
+
+  Item t = item(first);
+  Src src = source(t, true);
+  bool more = first + step < end;
+  Item u = item(more ? first + step : first);
+  Src nxt = source(u, more);
+  dma_scales(src.x, src.so, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {   // (a tile of one block is its workgroup's only one: `launch`)
+    const uint32_t ko = i < t.n ? src.ko + 128u * i : NONE;
+#pragma unroll
+    for (int j = 0; j < J; ++j) dma_one(src.a, src.b, ko, i, j);
+  }
+  dma_wait<J>();   // the first scale words and stage 0 landed
+  raw_barrier();
+  read_b(0, 0, fb[0]);
+#pragma unroll
+  for (int a = 0; a < MB; ++a) read_a(0, 0, a);
+  int slot = 0, gslot = 0, tslot = 0;
+  for (int w = first;;) {
+#pragma unroll
+    for (int a = 0; a < MB; ++a)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[a][b] = f32x16{0};
+    for (int kb = 0; kb < t.n; ++kb) {
       if ((kb & 3) == 0) {
-        read_scales(kb >> 2);
-        dma_scales((kb >> 2) + 1, false);
+        read_scales(gslot);
+        gslot ^= 1;
+        const bool here = kb + 4 < t.n;
+        dma_scales(pick(here, src.x, nxt.x), here ? src.so : nxt.so, here ? (kb >> 2) + 1 : 0, gslot, tslot ^ 1);
       } else {
 #pragma unroll
         for (int a = 0; a < MB; ++a) wa[a] >>= 8;
 #pragma unroll
         for (int b = 0; b < NB; ++b) wb[b] >>= 8;
       }
-      const int st = (kb - kb0) * SPB;   // (past the end a stale slot is read, and not used)
-      if constexpr (SPB == 2) {
-        half_step(fb[0], fb[1], st + 1, 0, yes, st + NS);
-        half_step(fb[1], fb[0], st + 2, 0, yes, st + 1 + NS);
-      } else {
-        half_step(fb[0], fb[1], st, 1, no, 0);
-        half_step(fb[1], fb[0], st + 1, 0, yes, st + NS);
-      }
+      const int k2 = kb + 2 - t.n;   // the stage to fetch: of this tile, or block k2 (0, 1) of the next
+      const bool here = k2 < 0;
+      const uint32_t ko = here ? src.ko + 128u * (kb + 2) : more ? nxt.ko + 128u * k2 : NONE;
+      half_step(fb[0], fb[1], slot, std::false_type{}, 0u, src.a, src.b, 0u);
+      half_step(fb[1], fb[0], slot, std::true_type{}, (uint32_t)(kb == 0 && w != first), pick(here, src.a, nxt.a),
+                pick(here, src.b, nxt.b), ko);
+      slot ^= 1;
     }
+    store(t, tslot);
+    if (!more) break;
+    w += step;
+    tslot ^= 1;
+    t = u;
+    src = nxt;
+    more = w + step < end;
+    u = item(more ? w + step : w);
+    nxt = source(u, more);
   }
   dma_wait<0>();   // no DMA piece may land after the workgroup's LDS has been given away
-
-  // ---- epilogue: a lane holds 4 consecutive columns of a row per quad of registers, the other half
-  // wave the next 4; bf16 quads change places in pairs so that every store is 16 B per lane
-  using OutT = std::conditional_t<OB, uint16_t, float>;
-  OutT* C = (OutT*)g.C + (int64_t)z * g.c_zs;
-  const int cn = n0 + wn * WN;
-#pragma unroll
-  for (int a = 0; a < MB; ++a) {
-    const int r = m0 + wm * WM + 32 * a + l32;
-    OutT* row = C + (int64_t)r * g.ldc;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      float v[4][4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int lc = 32 * b + 8 * q + 4 * h, c = cn + lc;
-        float4 bb = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (g.bias) bb = *reinterpret_cast<const float4*>(lds + BIAS + (wn * WN + lc) * 4);
-        v[q][0] = acc[a][b][4 * q] + bb.x;
-        v[q][1] = acc[a][b][4 * q + 1] + bb.y;
-        v[q][2] = acc[a][b][4 * q + 2] + bb.z;
-        v[q][3] = acc[a][b][4 * q + 3] + bb.w;
-        if (g.beta && r < g.M) {
-          if (g.vec) {
-            if (c < g.N) {
-              if constexpr (OB) {
-                const uint2 w = *reinterpret_cast<const uint2*>(row + c);
-                v[q][0] += __uint_as_float(w.x << 16); v[q][1] += __uint_as_float(w.x & 0xffff0000u);
-                v[q][2] += __uint_as_float(w.y << 16); v[q][3] += __uint_as_float(w.y & 0xffff0000u);
-              } else {
-                const float4 w = *reinterpret_cast<const float4*>(row + c);
-                v[q][0] += w.x; v[q][1] += w.y; v[q][2] += w.z; v[q][3] += w.w;
-              }
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (c + i < g.N) v[q][i] += hx::io<OutT>::ld(row + c + i);
-          }
-        }
-      }
-      if (g.vec) {
-        if constexpr (OB) {
-#pragma unroll
-          for (int q = 0; q < 4; q += 2) {   // columns 8 q + 8 h .. + 8 after the exchange
-            const auto x = __builtin_amdgcn_permlane32_swap(bf16x2(v[q][0], v[q][1]), bf16x2(v[q + 1][0], v[q + 1][1]), false, false);
-            const auto y = __builtin_amdgcn_permlane32_swap(bf16x2(v[q][2], v[q][3]), bf16x2(v[q + 1][2], v[q + 1][3]), false, false);
-            const int c = cn + 32 * b + 8 * q + 8 * h;
-            if (r < g.M && c < g.N) *reinterpret_cast<uint4*>(row + c) = make_uint4(x[0], y[0], x[1], y[1]);
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int c = cn + 32 * b + 8 * q + 4 * h;
-            if (r < g.M && c < g.N) *reinterpret_cast<float4*>(row + c) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
-          }
-        }
-      } else if (r < g.M) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int c = cn + 32 * b + 8 * q + 4 * h + i;
-            if (c < g.N) hx::io<OutT>::st(row + c, v[q][i]);
-          }
-      }
-    }
-  }
 }
 
 // out[M][N] = sum of ks slabs (+ bias) (+ out), 4 elements per thread
@@ -415,39 +469,47 @@ __global__ __launch_bounds__(512) void fp8_rows_k(HxRows8 g) {
   }
 }
 
-template <int BM, int BN, int WM, int WN, int KS, int NS, int WGS, bool EXACT, bool OB>
+template <int BM, int BN, int WM, int WN, int WGS, bool EXACT, bool OB>
 int launch(const HxGemm8& g, hipStream_t s) {
   constexpr int NT = (BM / WM) * (BN / WN) * 64;
-  constexpr int LDS = NS * (BM + BN) * KS + 6144;   // + scale words, bias, spare
-  auto k = gemm_fp8_k<BM, BN, WM, WN, KS, NS, WGS, EXACT, OB>;
+  constexpr int LDS = 2 * (BM + BN) * 128 + 4096 + 2048 + 1024;   // stages, scale words, biases, spare
+  auto k = gemm_fp8_k<BM, BN, WM, WN, WGS, EXACT, OB>;
   static const hipError_t ok = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (ok != hipSuccess) return 1;
-  const int64_t total = (int64_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN) * g.ks;
-  k<<<(unsigned)((total + 7) / 8 * 8), NT, LDS, s>>>(g);
+  const int64_t items = (int64_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN) * g.ks;
+  if (items > 0x7fffffff) return 1;
+  // one workgroup per item, at most what the CUs hold at a time -- but where an item is one k block, which
+  // leaves no room for the next one's first two stages
+  const int gper = ((g.nkb + 3) / 4 + g.ks - 1) / g.ks * 4, last = g.nkb - (g.ks - 1) * gper;
+  if (last < 1) return 1;
+  const int64_t all = (items + 7) / 8;
+  const int64_t n = last < 2 ? all : std::min<int64_t>(all, std::max(hx_cu_slots() * WGS / 8, 1));
+  k<<<(unsigned)(8 * n), NT, LDS, s>>>(g);
   return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 template <bool EXACT, bool OB>
 int launch_cfg(const HxGemm8& g, int cfg, hipStream_t s) {
   switch (cfg) {
-    case 0: return launch<256, 256, 128, 64, 128, 2, 1, EXACT, OB>(g, s);
-    case 1: return launch<128, 128, 64, 64, 128, 2, 2, EXACT, OB>(g, s);
-    case 2: return launch<64, 64, 32, 32, 128, 2, 4, EXACT, OB>(g, s);
+    case 0: return launch<256, 256, 128, 64, 1, EXACT, OB>(g, s);
+    case 1: return launch<256, 192, 64, 96, 1, EXACT, OB>(g, s);
+    case 2: return launch<128, 128, 64, 64, 2, EXACT, OB>(g, s);
+    case 3: return launch<64, 64, 32, 32, 4, EXACT, OB>(g, s);
   }
   return 1;
 }
-constexpr int kTile[3] = {256, 128, 64};
+constexpr int kBM[4] = {256, 256, 128, 64}, kBN[4] = {256, 192, 128, 64};
 
 // Time in us of a product whose busiest CU gets n tiles of nkb k blocks: f + f1 nkb + n (t + t1 nkb),
-// fitted (non-negative least squares, 9 - 15 %) to 46 products of 128 .. 16384 tokens with the widths of
-// BERT-base and BERT-large.  The large tile is at the power limit of the matrix cores (a k block of a
-// 256 x 256 tile in 1.1 us on every CU: 3.9 PF; exact 2.15 us: 2.0 PF; instructions alone on such data
-// run at 3.8 and 1.8) but pays 7.7 us of first loads and stores per tile; the small one fills the
-// chip with few rows.  Choosing by it is on average 1 % from the best of the three, 15 % at most.
+// fitted (non-negative least squares, 6 - 15 %) to 46 products of 128 .. 16384 tokens with the widths of
+// BERT-base and BERT-large.  A k block of a 256 x 256 tile takes 1.1 us with every CU at work (3.9 PF;
+// exact 2.2 us: 1.9 PF), which is the power limit: the instructions alone, on such data, run at 3.8 and
+// 1.8 PF.  Each large tile pays 5 - 12 us of first loads and stores; 256 x 192 fits widths of 768 and
+// 2304; the small tiles fill the chip with few rows.  The choice is on average 1 - 2 % from the best.
 struct Cost {
   double f, f1, t, t1;
 };
-constexpr Cost kCost[2][3] = {{{0, 0, 7.7, 1.11}, {0, 0.04, 2.07, 0.554}, {0, 0.106, 0.74, 0.199}},
-                              {{0, 0, 12.8, 2.15}, {1.6, 0, 2.66, 0.913}, {0.97, 0.118, 0.835, 0.294}}};
+constexpr Cost kCost[2][4] = {{{0, 0, 6.3, 1.116}, {0, 0, 5.2, 1.0}, {0.67, 0, 1.78, 0.587}, {0.33, 0.153, 0.76, 0.197}},
+                              {{0, 0, 12.6, 2.234}, {0, 0, 8.6, 1.826}, {1.05, 0, 2.55, 0.961}, {1.02, 0.152, 0.95, 0.31}}};
 
 }  // namespace
 
@@ -456,10 +518,10 @@ constexpr Cost kCost[2][3] = {{{0, 0, 7.7, 1.11}, {0, 0.04, 2.07, 0.554}, {0, 0.
 void hx_gemm_fp8_plan(int M, int N, int nkb, int exact, int* cfg, int* ks) {
   const int slots = hx_cu_slots(), groups = (nkb + 3) / 4;
   double best = 1e30;
-  *cfg = 2;
+  *cfg = 3;
   *ks = 1;
-  for (int c = 0; c < 3; ++c) {
-    const int64_t tiles = (int64_t)((M + kTile[c] - 1) / kTile[c]) * ((N + kTile[c] - 1) / kTile[c]);
+  for (int c = 0; c < 4; ++c) {
+    const int64_t tiles = (int64_t)((M + kBM[c] - 1) / kBM[c]) * ((N + kBN[c] - 1) / kBN[c]);
     for (int k = 1; k <= 16 && k <= groups; ++k) {
       const int per = (groups + k - 1) / k;
       if (k > 1 && (groups + per - 1) / per != k) continue;   // (an empty slab)
