@@ -46,7 +46,7 @@ def parse():
     ap.add_argument('--batch', type=int, default=128, help='per-GPU sequences per step')
     ap.add_argument('--seq', type=int, default=128)
     ap.add_argument('--max-pred', type=int, default=20)
-    ap.add_argument('--precision', default='fp32', choices=['fp32', 'bf16'])
+    ap.add_argument('--precision', default='fp32', choices=['fp32', 'bf16', 'fp8'])
     ap.add_argument('--fp32-gemm', default='fp16x3', choices=['fp16x3', 'native'],
                     help='fp32 GEMMs: fp16x3 (default, fp32 class: ops/gemm16.py) or native f32 MFMA '
                          '(ops/fp32_mode.py)')
@@ -397,7 +397,7 @@ def run(a, rank, world, dev_index, init_method):
             'higher_is_better': True,
             'scaling': 'weak',
             'vs_baseline': round(value / ref, 2) if ref else None,
-            'dtype': 'fp32' if a.precision == 'fp32' else 'bf16',
+            'dtype': a.precision,
             'data': 'synthetic (NVIDIA-schema HDF5 shards, random-init weights)',
             'config': {'model': 'bert-base (L12 H768 A12 V30522, 110.1M params)' if a.model == 'base' else a.model,
                        'global_batch': global_batch, 'per_gpu_batch': a.batch * a.update_freq,

@@ -25,6 +25,7 @@ MI355X-native engine underneath:
   * batches arrive already staged on the HIP copy stream (``DeviceBatch``).
 """
 import contextlib
+import inspect
 import math
 import os
 import threading
@@ -63,6 +64,10 @@ def state_order_ambiguous(optim_state, ck_args):
     return own and not hasattr(ck_args, 'fp32_gemm')
 
 
+def _takes(fn, name):
+    return name in inspect.signature(fn).parameters
+
+
 class Controller(object):
     def __init__(self, args, task, model, criterion=None, dummy_batch=None, oom_batch=None):
         self.args = args
@@ -85,13 +90,19 @@ class Controller(object):
         if self.cuda:
             gemm_tuning.configure(getattr(args, 'gemm_tuning', 'table'), getattr(args, 'gemm_tuning_file', None))
         model = model.to(self.device)
-        if getattr(args, 'precision', 'fp32') == 'bf16' and hasattr(model, 'set_compute_dtype'):
+        precision = getattr(args, 'precision', 'fp32')
+        if precision == 'fp8':
+            # bf16 activations, the encoder's linears on e4m3 operands (ops/fp8.py)
+            if not hasattr(model, 'set_compute_dtype') or not _takes(model.set_compute_dtype, 'fp8'):
+                raise ValueError('--precision fp8: {} has no 8-bit encoder layers'.format(type(model).__name__))
+            model.set_compute_dtype(torch.bfloat16, fp8=True)
+        elif precision == 'bf16' and hasattr(model, 'set_compute_dtype'):
             model.set_compute_dtype(torch.bfloat16)
         self._model = model
         self.world_size = args.distributed_world_size
         groups = model.flat_contiguous_groups() if hasattr(model, 'flat_contiguous_groups') else None
         self.flat = FlatParamSpace(model, self.device, contiguous_groups=groups)
-        if getattr(args, 'precision', 'fp32') == 'bf16' and self.cuda:
+        if precision in ('bf16', 'fp8') and self.cuda:
             self.flat.enable_bf16_shadow()
         force = bool(getattr(args, 'force_reducer', False))
         use_reducer = (self.world_size > 1 or force) and not getattr(args, 'use_bmuf', False)

@@ -811,6 +811,40 @@ std::vector<OptT> split8(Tensor x, bool by_rows, bool by_cols, bool want_sum, Op
   return {q, s, qt, st, sum};
 }
 
+// both blockings of every weight, one launch: [(q, s, qt, st)] as split8 makes them
+std::vector<std::vector<Tensor>> split8_weights(std::vector<Tensor> Ws) {
+  TORCH_CHECK(!Ws.empty() && Ws.size() <= HX_WBATCH, "split8_weights: 1..64 weights");
+  HxSplit8Batch d{};
+  d.n = (int)Ws.size();
+  std::vector<std::vector<Tensor>> out;
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(Ws[0].device());
+  auto u8 = Ws[0].options().dtype(torch::kUInt8);
+  int64_t tiles = 0;
+  for (int i = 0; i < d.n; ++i) {
+    const Tensor& W = Ws[i];
+    check_rows8(W, "split8_weights");
+    check_f32(W, "split8_weights");
+    TORCH_CHECK(W.size(0) >= 1 && W.size(0) <= (1LL << 22) && aligned16(W.data_ptr()) && W.device() == Ws[0].device(),
+                "split8_weights: contiguous fp32 [1 .. 2^22, K] weights with 16-B aligned storage on one device");
+    const int64_t N = W.size(0), K = W.size(1);
+    out.push_back({torch::empty({N, blocks128(K) * 128}, u8), scale_words(N, K, W), torch::empty({K, blocks128(N) * 128}, u8),
+                   scale_words(K, N, W)});
+    d.W[i] = W.data_ptr<float>();
+    d.q[i] = out[i][0].data_ptr<uint8_t>();
+    d.s[i] = out[i][1].data_ptr<uint8_t>();
+    d.qt[i] = out[i][2].data_ptr<uint8_t>();
+    d.st[i] = out[i][3].data_ptr<uint8_t>();
+    d.R[i] = (int)N;
+    d.C[i] = (int)K;
+    d.start[i] = (int)tiles;
+    tiles += blocks128(N) * blocks128(K);
+    TORCH_CHECK(tiles < (1LL << 31), "split8_weights: too many tiles");
+  }
+  d.start[d.n] = (int)tiles;
+  hx_split8_many(d, cur_stream(Ws[0]));
+  return out;
+}
+
 // out [M, N] (fp32 or bf16, unit column stride) (+)= A . B^T (+ bias) from split8's codes and scale words
 static void gemm8_run(const uint8_t* a, const uint8_t* as, int64_t M, const uint8_t* b, const uint8_t* bs, int64_t N, int64_t K,
                       const Tensor& out, bool beta, const float* bias) {
@@ -956,7 +990,11 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
     OptT bias = has(b) ? OptT(b->detach()) : OptT();
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = N;
-    Tensor y, kept, wkept;
+    Tensor y, kept, wtq, wts;   // what the backward needs: x's codes; the codes of W^T and their scales
+    if (wt && !own) {
+      wtq = wqt.value_or(Tensor());
+      wts = wst.value_or(Tensor());
+    }
     if (!own && !keep) {
       y = linear_fp8_y(x2, *wq, *ws, bias, false, nullptr, nullptr);
     } else {
@@ -968,17 +1006,22 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
       TORCH_CHECK(!own || N <= (1LL << 22), "linear_fp8: at most 2^22 output features");
       c10::hip::HIPGuardMasqueradingAsCUDA guard(x2.device());
       const auto u8 = x2.options().dtype(torch::kUInt8);
-      const Codes8 cx(M, K), cxt(K, M, keep), cw(N, K, own), cwt(K, N, own && wt);
+      const Codes8 cx(M, K), cxt(K, M, keep), cw(N, K, own);
       Tensor tmp = torch::empty({cx.bytes() + cw.bytes()}, u8);
       if (keep && M > 0) kept = torch::empty({cxt.bytes()}, u8);
-      if (cwt.bytes()) wkept = torch::empty({cwt.bytes()}, u8);
+      if (own && wt) {
+        // of the shapes that an Fp8Weight has: a checkpointed segment may run with one and be recomputed
+        // without it, and what is saved has to match
+        wtq = torch::empty({K, blocks128(N) * 128}, u8);
+        wts = scale_words(K, N, x2);
+      }
       uint8_t *px = tmp.data_ptr<uint8_t>(), *pw = px + cx.bytes();
       uint8_t* pk = kept.defined() ? kept.data_ptr<uint8_t>() : nullptr;
-      uint8_t* pt = wkept.defined() ? wkept.data_ptr<uint8_t>() : nullptr;
+      uint8_t* pt = own && wt ? wtq.data_ptr<uint8_t>() : nullptr;
       HxSplit8 jobs[2];
       int n = 0;
       if (M > 0) jobs[n++] = split8_job(x2, cx.q(px), cx.s(px), cxt.q(pk), pk ? cxt.s(pk) : nullptr, nullptr);
-      if (own) jobs[n++] = split8_job(W2, cw.q(pw), cw.s(pw), cwt.q(pt), pt ? cwt.s(pt) : nullptr, nullptr);
+      if (own) jobs[n++] = split8_job(W2, cw.q(pw), cw.s(pw), pt, pt ? wts.data_ptr<uint8_t>() : nullptr, nullptr);
       if (n) hx_split8(jobs, n, cur_stream(x2));
       y = torch::empty({M, N}, x2.options());
       if (M > 0) {
@@ -990,10 +1033,9 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
         dbg_finite(y, "linear_fp8");
       }
     }
-    ctx->save_for_backward({kept, own ? wkept : wqt.value_or(Tensor()), own ? Tensor() : wst.value_or(Tensor())});
+    ctx->save_for_backward({kept, wtq, wts});
     ctx->saved_data["xshape"] = x.sizes().vec();
     ctx->saved_data["N"] = N;
-    ctx->saved_data["own"] = own;
     ctx->saved_data["wbf16"] = has(W) && W->scalar_type() == torch::kBFloat16;
     // the inputs that are there have the first edges, in order
     ctx->saved_data["ew"] = has(W) ? 1 : 0;
@@ -1006,7 +1048,6 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
     const int64_t N = ctx->saved_data["N"].toInt(), K = xshape.back();
     const int64_t ew = ctx->saved_data["ew"].toInt(), eb = ctx->saved_data["eb"].toInt();
     const bool need_x = ctx->needs_input_grad(0), need_w = ew && ctx->needs_input_grad(ew), need_b = eb && ctx->needs_input_grad(eb);
-    const bool own = ctx->saved_data["own"].toBool();
     Tensor dy = as_rows8(g[0]);
     check_rows8(dy, "linear_fp8 output gradient");
     const int64_t M = dy.size(0);
@@ -1017,7 +1058,7 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
     if (need_w) dW = M > 0 ? torch::empty({N, K}, f32) : torch::zeros({N, K}, f32);
     if (need_b) db = M > 0 ? torch::empty({N}, f32) : torch::zeros({N}, f32);
     if (M > 0) {
-      const Codes8 cd(M, N, need_x), cdt(N, M, need_w), cxt(K, M, need_w), cwt(K, N, own);
+      const Codes8 cd(M, N, need_x), cdt(N, M, need_w), cxt(K, M, need_w);
       const int64_t part = need_b ? up256(hx_split8_row_tiles(M) * N * 4) : 0;
       Tensor tmp = torch::empty({cd.bytes() + cdt.bytes() + part}, dy.options().dtype(torch::kUInt8));
       uint8_t *pd = tmp.data_ptr<uint8_t>(), *pt = pd + cd.bytes(), *pp = pt + cdt.bytes();
@@ -1030,8 +1071,8 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
         dbg_finite(dW, "linear_fp8 weight gradient");
       }
       if (need_x) {
-        uint8_t* pw = saved[1].data_ptr<uint8_t>();
-        gemm8_run(cd.q(pd), cd.s(pd), M, pw, own ? cwt.s(pw) : saved[2].data_ptr<uint8_t>(), K, N, dx, false, nullptr);
+        TORCH_CHECK(saved[1].defined(), "linear_fp8: the weight's codes were made without those of its transpose");
+        gemm8_run(cd.q(pd), cd.s(pd), M, saved[1].data_ptr<uint8_t>(), saved[2].data_ptr<uint8_t>(), K, N, dx, false, nullptr);
         dbg_finite(dx, "linear_fp8 input gradient");
       }
     }
@@ -1510,6 +1551,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("bias") = py::none(), py::arg("out_bf16") = true);
   m.def("split8", &split8, py::arg("x"), py::arg("by_rows"), py::arg("by_cols"), py::arg("want_sum") = false,
         py::arg("sum_out") = py::none());
+  m.def("split8_weights", &split8_weights);
   m.def("gemm_fp8", &gemm_fp8, py::arg("a"), py::arg("as"), py::arg("b"), py::arg("bs"), py::arg("K"), py::arg("out_bf16"),
         py::arg("out") = py::none(), py::arg("beta") = false, py::arg("bias") = py::none());
   m.def("linear_fp8_fwd", &linear_fp8_fwd, py::arg("x"), py::arg("wq"), py::arg("ws"), py::arg("bias"), py::arg("keep"));

@@ -253,6 +253,15 @@ struct HxSplit8 {
 };
 int hx_split8_row_tiles(int64_t R);
 void hx_split8(const HxSplit8* jobs, int n, hipStream_t stream);
+// up to HX_WBATCH contiguous fp32 weights [R, C], both blockings of each, in one launch; tile t of weight
+// i is workgroup start[i] + t
+struct HxSplit8Batch {
+  int n;
+  const float* W[HX_WBATCH];
+  uint8_t *q[HX_WBATCH], *s[HX_WBATCH], *qt[HX_WBATCH], *st[HX_WBATCH];
+  int R[HX_WBATCH], C[HX_WBATCH], start[HX_WBATCH + 1];
+};
+void hx_split8_many(const HxSplit8Batch& d, hipStream_t stream);
 // int8 blocks along contiguous rows of N: codes [rows][nb][128], scale bytes [rows][nb], nb = ceil(N / 128)
 void hx_gelu8_fwd(int bf16, const void* y, const float* b, void* out, uint8_t* q, uint8_t* s, int64_t rows, int N,
                   int vec, hipStream_t stream);

@@ -211,6 +211,15 @@ __global__ __launch_bounds__(SNT) void split8_k(HxSplit8 a, HxSplit8 b) {
   }
 }
 
+// every weight of an encoder at once (ops.fp8_scope): one launch per forward instead of one per layer
+__global__ __launch_bounds__(SNT) void split8_many_k(HxSplit8Batch d) {
+  __shared__ __attribute__((aligned(16))) Split8Lds lds;
+  int i = 0;
+  while (i + 1 < d.n && (int)blockIdx.x >= d.start[i + 1]) ++i;   // uniform over the workgroup
+  const HxSplit8 a{0, d.W[i], d.C[i], d.R[i], d.C[i], d.q[i], d.s[i], d.qt[i], d.st[i], nullptr, d.C[i] % 4 == 0};
+  split8_tile<TileF32>(a, blockIdx.x - d.start[i], lds);
+}
+
 // ---------------------------------------------------------------- bias + GELU with an int8 checkpoint
 // gelu(u) = u Phi(u), Phi(u) = (1 + erf(z)) / 2 with z = u / 1.41421 (the model's truncated constant).
 // erfc by Abramowitz & Stegun 7.1.26 (a degree-5 polynomial in 1 / (1 + p z) times exp(-z^2), error
@@ -363,6 +372,10 @@ void hx_split8(const HxSplit8* jobs, int n, hipStream_t stream) {
   else if (a.bf16) split8_k<TileBf16, TileF32><<<grid, SNT, 0, stream>>>(a, b);
   else if (b.bf16) split8_k<TileF32, TileBf16><<<grid, SNT, 0, stream>>>(a, b);
   else split8_k<TileF32, TileF32><<<grid, SNT, 0, stream>>>(a, b);
+}
+
+void hx_split8_many(const HxSplit8Batch& d, hipStream_t stream) {
+  split8_many_k<<<d.start[d.n], SNT, 0, stream>>>(d);
 }
 
 void hx_gelu8_fwd(int bf16, const void* y, const float* b, void* out, uint8_t* q, uint8_t* s, int64_t rows, int N,

@@ -111,6 +111,7 @@ class BertConfig(object):
 class LinearActivation(nn.Module):
     """Linear + activation; GELU/tanh with bias run as one fused epilogue kernel."""
     __constants__ = ['bias']
+    fp8 = False     # set_compute_dtype(fp8=True): e4m3 products, 8-bit kept activations (encoder layers)
 
     def __init__(self, in_features, out_features, act='gelu', bias=True):
         super().__init__()
@@ -133,7 +134,12 @@ class LinearActivation(nn.Module):
             init.uniform_(self.bias, -bound, bound)
 
     def forward(self, x, res_grad=None):
-        y = ops.linear(x, self.weight, res_grad=res_grad)
+        if self.fp8:
+            y = ops.linear_fp8(x, self.weight, res_grad=res_grad)
+            if self.act == 'gelu':   # the backward reads y from int8 blocks
+                return ops.bias_act(y, self.bias, 'gelu', bits=8)
+        else:
+            y = ops.linear(x, self.weight, res_grad=res_grad)
         if self.act in ('gelu', 'tanh', 'relu'):
             return ops.bias_act(y, self.bias, self.act)
         if self.bias is not None:
@@ -183,6 +189,8 @@ _QKV_BIAS_EPILOGUE = os.environ.get('HX_QKV_BIAS_EPILOGUE', '1') != '0'
 
 
 class BertSelfAttention(nn.Module):
+    fp8 = False
+
     def __init__(self, config):
         super().__init__()
         if config.hidden_size % config.num_attention_heads != 0:
@@ -198,6 +206,11 @@ class BertSelfAttention(nn.Module):
 
     def forward(self, hidden_states, attention_mask_bias, res_grad=None):
         bias = (self.query.bias, self.key.bias, self.value.bias)
+        if self.fp8:
+            qkv = ops.linear3_fp8(hidden_states, self.query.weight, self.key.weight, self.value.weight, *bias,
+                                  res_grad=res_grad, bias_grad=False)
+            return ops.attention(qkv, attention_mask_bias, self.num_attention_heads, self.dropout.p, self.training,
+                                 bias_grad=bias)
         if _QKV_BIAS_EPILOGUE:
             # one N=3H projection GEMM with the Q/K/V biases in its epilogue; their gradients (the
             # column sums of dQKV) come out of the fused attention backward's registers
@@ -213,6 +226,8 @@ class BertSelfAttention(nn.Module):
 
 
 class BertSelfOutput(nn.Module):
+    fp8 = False
+
     def __init__(self, config):
         super().__init__()
         self.dense = nn.Linear(config.hidden_size, config.hidden_size)
@@ -220,7 +235,7 @@ class BertSelfOutput(nn.Module):
         self.dropout = nn.Dropout(config.hidden_dropout_prob)
 
     def forward(self, hidden_states, input_tensor, res_grad=None):
-        y = ops.linear(hidden_states, self.dense.weight)
+        y = (ops.linear_fp8 if self.fp8 else ops.linear)(hidden_states, self.dense.weight)
         return ops.bias_dropout_residual_ln(y, self.dense.bias, input_tensor, self.LayerNorm.weight,
                                             self.LayerNorm.bias, self.LayerNorm.variance_epsilon,
                                             self.dropout.p, self.training, res_grad=res_grad)
@@ -249,6 +264,8 @@ class BertIntermediate(nn.Module):
 
 
 class BertOutput(nn.Module):
+    fp8 = False
+
     def __init__(self, config):
         super().__init__()
         self.dense = nn.Linear(config.intermediate_size, config.hidden_size)
@@ -256,7 +273,8 @@ class BertOutput(nn.Module):
         self.dropout = nn.Dropout(config.hidden_dropout_prob)
 
     def forward(self, hidden_states, input_tensor, res_grad=None):
-        return self.finish(ops.linear(hidden_states, self.dense.weight), input_tensor, res_grad)
+        linear = ops.linear_fp8 if self.fp8 else ops.linear
+        return self.finish(linear(hidden_states, self.dense.weight), input_tensor, res_grad)
 
     def finish(self, y, input_tensor, res_grad=None):
         """dense bias -> dropout -> + residual -> LayerNorm on the bias-less projection ``y``."""
@@ -276,7 +294,7 @@ class BertLayer(nn.Module):
         attention_output = self.attention(hidden_states, attention_mask_bias)
         rg = ops.ResidualGrad()     # residual grad of attention_output -> FFN-up dgrad GEMM
         up = self.intermediate.dense_act
-        if up.act == 'gelu' and ops.ffn_fusable(attention_output, up.weight, up.bias, self.output.dense.weight):
+        if not up.fp8 and up.act == 'gelu' and ops.ffn_fusable(attention_output, up.weight, up.bias, self.output.dense.weight):
             # fp32 runs: bias + GELU in the FFN-up GEMM's epilogue, the GELU backward in the
             # FFN-down data gradient's (ops.ffn)
             y = ops.ffn(attention_output, up.weight, up.bias, self.output.dense.weight, rg)
@@ -308,7 +326,8 @@ class BertEncoder(nn.Module):
 
     def forward(self, hidden_states, attention_mask_bias, output_all_encoded_layers=True,
                 checkpoint_activations=False):
-        with ops.weight_pieces_scope(self._piece_weights(), hidden_states):
+        fp8 = len(self.layer) > 0 and self.layer[0].output.fp8
+        with (ops.fp8_scope(self._piece_weights()) if fp8 else ops.weight_pieces_scope(self._piece_weights(), hidden_states)):
             return self._forward(hidden_states, attention_mask_bias, output_all_encoded_layers,
                                  checkpoint_activations)
 
@@ -343,8 +362,12 @@ class BertEncoder(nn.Module):
             chunk = math.ceil(math.sqrt(num_layers))
             l = 0
             while l < num_layers:
-                hidden_states = checkpoint(_rng_replaying(custom(l, l + chunk)), hidden_states,
-                                           attention_mask_bias, use_reentrant=False)
+                segment = _rng_replaying(custom(l, l + chunk))
+                if checkpoint_activations == 8:
+                    # 8: a segment's input is kept as int8 blocks, a byte per element
+                    hidden_states = ops.checkpoint8(segment, hidden_states, attention_mask_bias)
+                else:
+                    hidden_states = checkpoint(segment, hidden_states, attention_mask_bias, use_reentrant=False)
                 l += chunk
         else:
             for layer_module in self.layer:
@@ -574,10 +597,15 @@ class BertPreTrainedModel(nn.Module):
         if isinstance(module, nn.Linear) and module.bias is not None:
             module.bias.data.zero_()
 
-    def set_compute_dtype(self, dtype):
+    def set_compute_dtype(self, dtype, fp8=False):
+        """Activations in ``dtype``; ``fp8``: the encoder layers' linears on e4m3 operands, with the
+        activations that only the backward reads kept in 8 bits (ops/fp8.py)."""
         for m in self.modules():
             if isinstance(m, BertEmbeddings):
                 m.compute_dtype = dtype
+            elif isinstance(m, BertLayer):
+                for part in (m.attention.self, m.attention.output, m.intermediate.dense_act, m.output):
+                    part.fp8 = bool(fp8)
 
     def flat_contiguous_groups(self):
         """Parameter-name groups that must be adjacent in the flat buffer so the

@@ -104,6 +104,13 @@ class Fp8Weight(object):
         else:
             self.ref = (e4m3_ref(W), e4m3_ref(W.t()) if grad else None)
 
+    @classmethod
+    def _of(cls, W, q, s, qt, st):
+        w = cls.__new__(cls)
+        w.shape, w.dtype, w.device, w.ref = tuple(W.shape), W.dtype, W.device, None
+        w.q, w.s, w.qt, w.st = q, s, qt, st
+        return w
+
     @property
     def has_grad(self):
         return self.qt is not None or (self.ref is not None and self.ref[1] is not None)
@@ -114,15 +121,23 @@ class _Scope(object):
 
 
 class fp8_scope(object):
-    """``Fp8Weight`` copies of every weight in ``Ws`` for the running forward: ``linear_fp8`` finds
-    them by the weight; a recompute outside the scope builds its own."""
+    """``Fp8Weight`` copies of every weight in ``Ws`` for the running forward, made in one launch:
+    ``linear_fp8`` / ``linear3_fp8`` find them by the weight.  A recompute outside the scope makes its
+    own."""
 
     def __init__(self, Ws):
         self.Ws = [W for W in Ws if W is not None]
 
     def __enter__(self):
         self.prev = _Scope.weights
-        _Scope.weights = {(W.data_ptr(), tuple(W.shape)): Fp8Weight(W) for W in self.Ws if use_kernels(W)}
+        d = {}
+        Ws = [W.detach() for W in self.Ws if use_kernels(W) and W.dtype == torch.float32 and W.is_contiguous() and
+              W.data_ptr() % 16 == 0]
+        for i in range(0, len(Ws), 64):
+            chunk = Ws[i:i + 64]
+            for W, t in zip(chunk, C().split8_weights(chunk)):
+                d[(W.data_ptr(), tuple(W.shape))] = Fp8Weight._of(W, *t)
+        _Scope.weights = d
         return self
 
     def __exit__(self, *exc):
@@ -154,7 +169,7 @@ class _LinearFp8Fn(torch.autograd.Function):
     def forward(ctx, x, w8, bias, mbox, bgrad, n, *params):
         N, K = w8.shape
         x2 = _rows2(x)
-        ctx.w8, ctx.mbox, ctx.xshape, ctx.n, ctx.bgrad = w8, mbox, x.shape, n, bgrad
+        ctx.wshape, ctx.mbox, ctx.xshape, ctx.n, ctx.bgrad = w8.shape, mbox, x.shape, n, bgrad
         ctx.Ws, ctx.bs = params[:n], params[n:]
         # the weight gradient reads the 8-bit copy of x blocked along the tokens
         keep = any(ctx.needs_input_grad[6:6 + n])
@@ -164,21 +179,24 @@ class _LinearFp8Fn(torch.autograd.Function):
             y = e4m3_ref(x2) @ w8.ref[0].t()
             y = (y if bias is None else y + bias).to(x.dtype)
             qt, st = (e4m3_ref(x2.t()), None) if keep else (None, None)
-        ctx.save_for_backward(qt, st)
+        wt = (None, None)
+        if ctx.needs_input_grad[0]:
+            wt = (w8.qt, w8.st) if w8.ref is None else (w8.ref[1], None)
+        ctx.save_for_backward(qt, st, *wt)
         return y.view(*x.shape[:-1], N)
 
     @staticmethod
     def backward(ctx, dy):
-        xt, xs = ctx.saved_tensors
-        w8, n, Ws, bs = ctx.w8, ctx.n, ctx.Ws, ctx.bs
-        N, K = w8.shape
+        xt, xs, wt, ws = ctx.saved_tensors
+        n, Ws, bs = ctx.n, ctx.Ws, ctx.bs
+        N, K = ctx.wshape
         need_x = ctx.needs_input_grad[0]
         need_w = any(ctx.needs_input_grad[6:6 + n])
         need_b = ctx.bgrad and any(ctx.needs_input_grad[6 + n:])
         dy2 = _rows2(dy)
         M = dy2.shape[0]
         if not use_kernels(dy):
-            dx = (e4m3_ref(dy2) @ w8.ref[1].t()).to(dy.dtype).view(ctx.xshape) if need_x else None
+            dx = (e4m3_ref(dy2) @ wt.t()).to(dy.dtype).view(ctx.xshape) if need_x else None
             dW = e4m3_ref(dy2.t()) @ xt.t() if need_w else None
             db = dy2.float().sum(0) if need_b else None
             return (_residual(dx, ctx.mbox), None, None, None, None, None,
@@ -202,7 +220,7 @@ class _LinearFp8Fn(torch.autograd.Function):
             if ctx.mbox is not None:
                 acc, other = ctx.mbox.take(dy.dtype)
             acc = acc.view(M, K) if acc is not None else None
-            dx = C().gemm_fp8(q, s, w8.qt, w8.st, N, dy.dtype == torch.bfloat16, out=acc, beta=acc is not None).view(ctx.xshape)
+            dx = C().gemm_fp8(q, s, wt, ws, N, dy.dtype == torch.bfloat16, out=acc, beta=acc is not None).view(ctx.xshape)
             if other is not None:
                 dx = dx + other.view(ctx.xshape).to(dx.dtype)
         return (dx, None, None, None, None, None, *gW, *_parts(db, bs, bslots, bview is not None))

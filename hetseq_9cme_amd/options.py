@@ -49,12 +49,14 @@ def get_training_parser(task='bert', optimizer='adam', lr_scheduler='PolynomialD
     parser.add_argument('--log-format', default='simple', choices=['none', 'simple', 'json', 'tqdm'],
                         help='log format to use')
     # --- MI355X-native execution knobs (not in the reference) ---
-    parser.add_argument('--precision', default='fp32', choices=['fp32', 'bf16'],
+    parser.add_argument('--precision', default='fp32', choices=['fp32', 'bf16', 'fp8'],
                         help='compute precision: fp32 (the reference\'s precision: fp32 tensors end to end; '
                              'the GEMMs and attention products run as --fp32-gemm says -- by default fp16x3, '
                              'fp32 class on the fp16 matrix cores; --fp32-gemm native gives plain f32 MFMA, '
                              'bitwise the reference\'s fp32 FMA chain) or bf16 (bf16 MFMA, fp32 master weights '
-                             'and optimizer state)')
+                             'and optimizer state) or fp8 (bf16 activations; the encoder layers\' linear products '
+                             'on e4m3 operands with one power-of-two scale per block of 128, and the activations '
+                             'that only the backward reads kept in 8 bits, ops/fp8.py)')
     parser.add_argument('--fp32-gemm', default='fp16x3', choices=['fp16x3', 'native'],
                         help='how fp32 (--precision fp32) runs use the matrix cores: fp16x3 (default: every '
                              'linear-layer GEMM on the hand-written kernels with operands scaled by a power of two '
