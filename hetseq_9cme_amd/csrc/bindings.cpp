@@ -737,9 +737,6 @@ std::vector<Tensor> gemm_f16_dgelu(Tensor a, Tensor a_amax, Tensor b, Tensor b_a
 }
 
 // ------------------------------------------------------------------ 8-bit blocks (quant8.hip, gemm_fp8.hip)
-inline bool rows_vec(const Tensor& t, int64_t ld) {   // 16-B accesses of 8 consecutive elements of a row
-  return aligned16(t.data_ptr()) && ld % (t.scalar_type() == torch::kFloat32 ? 4 : 8) == 0;
-}
 inline int64_t blocks128(int64_t n) { return (n + 127) / 128; }
 inline void check_bias8(const OptT& b, int64_t N, const Tensor& like, const char* what) {
   if (!has(b)) return;
@@ -771,7 +768,6 @@ static HxSplit8 split8_job(const Tensor& x, uint8_t* q, uint8_t* s, uint8_t* qt,
   j.qt = qt;
   j.st = st;
   j.colpart = colpart;
-  j.vec = rows_vec(x, j.ld);
   return j;
 }
 
@@ -937,7 +933,6 @@ static Tensor linear_fp8_y(const Tensor& x2, const Tensor& wq, const Tensor& ws,
     g.N = (int)N;
     g.K = (int)K;
     g.nkb = (int)blocks128(K);
-    g.xvec = rows_vec(x2, g.ldx);
     TORCH_CHECK(hx_fp8_rows(g, act_bf16(x2), cur_stream(x2)) == 0, "linear_fp8: launch failed");
     dbg_finite(y, "linear_fp8");
     return y;
@@ -1112,10 +1107,9 @@ std::vector<Tensor> gelu8_fwd(Tensor y, OptT b) {
   Tensor out = torch::empty_like(y);
   Tensor q = torch::empty({rows, blocks128(N), 128}, y.options().dtype(torch::kUInt8));
   Tensor s = torch::empty({rows, blocks128(N)}, y.options().dtype(torch::kUInt8));
-  const bool vec = rows_vec(y, N) && aligned16(out.data_ptr()) && (!has(b) || aligned16(b->data_ptr()));
   if (rows > 0)
     hx_gelu8_fwd(act_bf16(y), y.data_ptr(), ptr_or_null<float>(b), out.data_ptr(), q.data_ptr<uint8_t>(),
-                 s.data_ptr<uint8_t>(), rows, (int)N, vec, cur_stream(y));
+                 s.data_ptr<uint8_t>(), rows, (int)N, cur_stream(y));
   dbg_finite(out, "gelu8_fwd");
   return {out, q, s};
 }
@@ -1134,10 +1128,9 @@ std::vector<OptT> gelu8_bwd(Tensor dout, Tensor q, Tensor s, OptT b, bool want_d
     if (rows == 0) db->zero_();
     else part = torch::empty({hx_gelu8_chunks(rows), N}, f32);
   }
-  const bool vec = rows_vec(dout, N) && aligned16(dy.data_ptr()) && (!has(b) || aligned16(b->data_ptr()));
   if (rows > 0)
     hx_gelu8_bwd(act_bf16(dout), dout.data_ptr(), q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), ptr_or_null<float>(b),
-                 dy.data_ptr(), want_db ? part.data_ptr<float>() : nullptr, ptr_or_null<float>(db), rows, (int)N, vec,
+                 dy.data_ptr(), want_db ? part.data_ptr<float>() : nullptr, ptr_or_null<float>(db), rows, (int)N,
                  cur_stream(dout));
   dbg_finite(dy, "gelu8_bwd");
   return {dy, db};
@@ -1165,7 +1158,7 @@ std::vector<Tensor> pack8(Tensor x) {
   Tensor q = torch::empty({rows, blocks128(N), 128}, x.options().dtype(torch::kUInt8));
   Tensor s = torch::empty({rows, blocks128(N)}, x.options().dtype(torch::kUInt8));
   if (rows > 0)
-    hx_pack8(act_bf16(x), x.data_ptr(), q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), rows, (int)N, rows_vec(x, N), cur_stream(x));
+    hx_pack8(act_bf16(x), x.data_ptr(), q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), rows, (int)N, cur_stream(x));
   return {q, s};
 }
 
@@ -1176,7 +1169,7 @@ Tensor unpack8(Tensor q, Tensor s, int64_t N, bool bf16) {
   c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   Tensor x = torch::empty({rows, N}, q.options().dtype(bf16 ? torch::kBFloat16 : torch::kFloat32));
   if (rows > 0)
-    hx_unpack8(bf16, q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), x.data_ptr(), rows, (int)N, rows_vec(x, N), cur_stream(q));
+    hx_unpack8(bf16, q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), x.data_ptr(), rows, (int)N, cur_stream(q));
   return x;
 }
 

@@ -234,7 +234,7 @@ void hx_stream_priority_range(int* least, int* greatest);
 void hx_destroy_stream(hipStream_t s);
 void hx_spin(int blocks, double us, int lds_bytes, uint32_t* sink, hipStream_t s);
 
-// quant8.hip -- 8-bit blocks of 128 (hx_quant.h).  vec: rows allow 16-B accesses.
+// quant8.hip -- 8-bit blocks of 128 (hx_quant.h)
 // split8: x [R, C] (row stride ld) -> e4m3 codes q [R, 128 ceil(C / 128)] blocked along the columns and
 // / or qt [C, 128 ceil(R / 128)] blocked along the rows (either may be null), with their scale bytes s /
 // st (block b of row r at ((b / 4) Rs + r) 4 + b % 4, Rs = rows rounded up to 4), and / or column sums
@@ -249,7 +249,6 @@ struct HxSplit8 {
   uint8_t* qt;
   uint8_t* st;
   float* colpart;
-  int vec;
 };
 int hx_split8_row_tiles(int64_t R);
 void hx_split8(const HxSplit8* jobs, int n, hipStream_t stream);
@@ -264,12 +263,12 @@ struct HxSplit8Batch {
 void hx_split8_many(const HxSplit8Batch& d, hipStream_t stream);
 // int8 blocks along contiguous rows of N: codes [rows][nb][128], scale bytes [rows][nb], nb = ceil(N / 128)
 void hx_gelu8_fwd(int bf16, const void* y, const float* b, void* out, uint8_t* q, uint8_t* s, int64_t rows, int N,
-                  int vec, hipStream_t stream);
+                  hipStream_t stream);
 int hx_gelu8_chunks(int64_t rows);
 void hx_gelu8_bwd(int bf16, const void* dout, const uint8_t* q, const uint8_t* s, const float* b, void* dy,
-                  float* partial, float* db, int64_t rows, int N, int vec, hipStream_t stream);
-void hx_pack8(int bf16, const void* x, uint8_t* q, uint8_t* s, int64_t rows, int N, int vec, hipStream_t stream);
-void hx_unpack8(int bf16, const uint8_t* q, const uint8_t* s, void* x, int64_t rows, int N, int vec, hipStream_t stream);
+                  float* partial, float* db, int64_t rows, int N, hipStream_t stream);
+void hx_pack8(int bf16, const void* x, uint8_t* q, uint8_t* s, int64_t rows, int N, hipStream_t stream);
+void hx_unpack8(int bf16, const uint8_t* q, const uint8_t* s, void* x, int64_t rows, int N, hipStream_t stream);
 
 // gemm_fp8.hip -- C[M][N] (+)= A . B^T (+ bias) on split8's codes (lda / ldb = padded row lengths,
 // multiples of 128; nkb = k blocks); sa / sb: their scale words
@@ -290,7 +289,7 @@ int hx_gemm_fp8(const HxGemm8& g, int cfg, int exact, int out_bf16, hipStream_t 
 void hx_gemm_fp8_slabs(const float* part, void* out, int out_bf16, int64_t ldc, int M, int N, int ks, const float* bias,
                        int beta, int vec, hipStream_t s);
 // y [M, N] (x's type, contiguous) = Q(x) B^T (+ bias) for M <= hx_fp8_rows_max() rows of fp32 or bf16 x
-// (row stride ldx; xvec: rows allow 16-B accesses), B as in HxGemm8
+// (row stride ldx), B as in HxGemm8
 struct HxRows8 {
   const void* x;
   int64_t ldx;
@@ -299,7 +298,7 @@ struct HxRows8 {
   const uint32_t* sb;
   void* y;
   const float* bias;
-  int M, N, K, nkb, xvec;
+  int M, N, K, nkb;
 };
 int hx_fp8_rows_max();
 int hx_fp8_rows(const HxRows8& g, int bf16, hipStream_t s);

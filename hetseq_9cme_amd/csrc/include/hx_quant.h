@@ -69,57 +69,52 @@ __device__ __forceinline__ float int8_val(uint32_t w, int j, float s) {
   return c == -128 ? __uint_as_float(0x7fc00000u) : (float)c * s;
 }
 
-// ---- typed access of 8 consecutive elements as fp32
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <>
-__device__ __forceinline__ void load8<uint16_t>(const uint16_t* p, float (&v)[8]) {
-  const uint4 x = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    v[2 * k] = __uint_as_float(w[k] << 16);
-    v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-  }
-}
 // two fp32 values -> packed bf16 (one v_cvt_pk_bf16_f32: nearest even, NaN kept)
 __device__ __forceinline__ uint32_t bf16x2(float a, float b) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
-  typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, b16x2));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16v2));
 }
+
+// ---- 16-B accesses at any element: global_load / store_dwordx4 take addresses of any alignment, so rows
+// of odd length or stride need no path of their own, only their last elements do
+typedef uint32_t u32v4 __attribute__((ext_vector_type(4)));
+typedef u32v4 u32v4_any __attribute__((aligned(2)));
+__device__ __forceinline__ u32v4 load16(const void* p) { return *reinterpret_cast<const u32v4_any*>(p); }
+__device__ __forceinline__ void store16(void* p, u32v4 v) { *reinterpret_cast<u32v4_any*>(p) = v; }
+
+// 8 consecutive elements of a row, of which n (<= 0: none) are inside, as fp32
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8]);
-template <>
-__device__ __forceinline__ void store8<float>(float* p, const float (&v)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
-template <>
-__device__ __forceinline__ void store8<uint16_t>(uint16_t* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) =
-      make_uint4(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]), bf16x2(v[4], v[5]), bf16x2(v[6], v[7]));
-}
-// 8 elements of a row of which n (<= 0: none) are inside; vec: the row allows one wide access
-template <typename T>
-__device__ __forceinline__ void load_upto(const T* p, int n, bool vec, float (&v)[8]) {
-  if (vec && n >= 8) {
-    load8<T>(p, v);
+__device__ __forceinline__ void load_upto(const T* p, int n, float (&v)[8]) {
+  if (n >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const u32v4 a = load16(p), b = load16(p + 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[k] = __uint_as_float(a[k]);
+        v[4 + k] = __uint_as_float(b[k]);
+      }
+    } else {
+      const u32v4 w = load16(p);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[2 * k] = __uint_as_float(w[k] << 16);
+        v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+      }
+    }
     return;
   }
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = k < n ? io<T>::ld(p + k) : 0.f;
 }
 template <typename T>
-__device__ __forceinline__ void store_upto(T* p, int n, bool vec, const float (&v)[8]) {
-  if (vec && n >= 8) {
-    store8<T>(p, v);
+__device__ __forceinline__ void store_upto(T* p, int n, const float (&v)[8]) {
+  if (n >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      store16(p, u32v4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
+      store16(p + 4, u32v4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])});
+    } else {
+      store16(p, u32v4{bf16x2(v[0], v[1]), bf16x2(v[2], v[3]), bf16x2(v[4], v[5]), bf16x2(v[6], v[7])});
+    }
     return;
   }
 #pragma unroll

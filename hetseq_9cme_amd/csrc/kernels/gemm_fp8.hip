@@ -275,14 +275,34 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) *
               __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), rc.r, in && c < g.N ? ro + c * 4 : NONE, 0, 0);
             }
           }
+        } else if constexpr (OB) {   // rows of any stride: 16 B at any element, and the last ones singly
+#pragma unroll
+          for (int q = 0; q < 4; q += 2) {
+            const auto x = __builtin_amdgcn_permlane32_swap(bf16x2(v[q][0], v[q][1]), bf16x2(v[q + 1][0], v[q + 1][1]), false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(bf16x2(v[q][2], v[q][3]), bf16x2(v[q + 1][2], v[q + 1][3]), false, false);
+            const int c = t.n0 + wn * WN + 32 * b + 8 * q + 8 * h;
+            const uint32_t e[4] = {(uint32_t)x[0], (uint32_t)y[0], (uint32_t)x[1], (uint32_t)y[1]};
+            if (in && c + 8 <= g.N) {
+              hx::q8::store16(row + c, u32x4{e[0], e[1], e[2], e[3]});
+            } else if (in) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (c + i < g.N) row[c + i] = (uint16_t)(e[i >> 1] >> (16 * (i & 1)));
+            }
+          }
         } else if (in) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 4; ++q) {
+            const int c = t.n0 + wn * WN + 32 * b + 8 * q + 4 * h;
+            if (c + 4 <= g.N) {
+              const f32x4 x = {v[q][0], v[q][1], v[q][2], v[q][3]};
+              hx::q8::store16(row + c, __builtin_bit_cast(u32x4, x));
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int c = t.n0 + wn * WN + 32 * b + 8 * q + 4 * h + i;
-              if (c < g.N) hx::io<OutT>::st(row + c, v[q][i]);
+              for (int i = 0; i < 4; ++i)
+                if (c + i < g.N) row[c + i] = v[q][i];
             }
+          }
         }
       }
     }
@@ -420,7 +440,7 @@ __global__ __launch_bounds__(512) void fp8_rows_k(HxRows8 g) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float v[8];
-        hx::q8::load_upto<T>(p + 8 * q, r < g.M ? g.K - k0 - 8 * q : 0, g.xvec, v);
+        hx::q8::load_upto<T>(p + 8 * q, r < g.M ? g.K - k0 - 8 * q : 0, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[m][8 * q + i] = v[i];
       }
@@ -557,7 +577,7 @@ int hx_fp8_rows(const HxRows8& g, int bf16, hipStream_t s) {
 }
 
 int hx_gemm_fp8(const HxGemm8& g, int cfg, int exact, int out_bf16, hipStream_t s) {
-  if (out_bf16) return exact ? launch_cfg<true, true>(g, cfg, s) : launch_cfg<false, true>(g, cfg, s);
+  if (out_bf16) return exact ? 1 : launch_cfg<false, true>(g, cfg, s);   // (a bf16 result needs no exact sums)
   return exact ? launch_cfg<true, false>(g, cfg, s) : launch_cfg<false, false>(g, cfg, s);
 }
 

@@ -32,7 +32,7 @@ constexpr uint32_t kInf = 0x7f800000u;
 // then shows as a maximum >= kInf, and the block's finite maximum is taken again), and their codes.
 struct TileF32 {
   float v[SR][8];
-  __device__ void load(const void* x, int64_t at, int i, int n, bool vec) { load_upto<float>((const float*)x + at, n, vec, v[i]); }
+  __device__ void load(const void* x, int64_t at, int i, int n) { load_upto<float>((const float*)x + at, n, v[i]); }
   __device__ static uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
   __device__ uint32_t row_max(int i) const {
     uint32_t m = 0;
@@ -58,11 +58,11 @@ struct TileF32 {
 // the same on packed bf16 pairs (word j: columns 2 j, 2 j + 1)
 struct TileBf16 {
   uint32_t w[SR][4];
-  __device__ void load(const void* x, int64_t at, int i, int n, bool vec) {
+  __device__ void load(const void* x, int64_t at, int i, int n) {
     const uint16_t* p = (const uint16_t*)x + at;
-    if (vec && n >= 8) {
-      const uint4 a = *reinterpret_cast<const uint4*>(p);
-      w[i][0] = a.x; w[i][1] = a.y; w[i][2] = a.z; w[i][3] = a.w;
+    if (n >= 8) {
+      const u32v4 a = load16(p);
+      w[i][0] = a[0]; w[i][1] = a[1]; w[i][2] = a[2]; w[i][3] = a[3];
       return;
     }
 #pragma unroll
@@ -115,7 +115,7 @@ __device__ __forceinline__ void split8_tile(const HxSplit8& a, int bid, Split8Ld
   const int Cp = (a.C + 127) / 128 * 128, Rp = (a.R + 127) / 128 * 128;
   Tile x;
 #pragma unroll
-  for (int i = 0; i < SR; ++i) x.load(a.x, (int64_t)(r0 + i) * a.ld + c0, i, r0 + i < a.R ? a.C - c0 : 0, a.vec);
+  for (int i = 0; i < SR; ++i) x.load(a.x, (int64_t)(r0 + i) * a.ld + c0, i, r0 + i < a.R ? a.C - c0 : 0);
   if (a.q) {
 #pragma unroll
     for (int i = 0; i < SR; ++i) {
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(SNT) void split8_many_k(HxSplit8Batch d) {
   __shared__ __attribute__((aligned(16))) Split8Lds lds;
   int i = 0;
   while (i + 1 < d.n && (int)blockIdx.x >= d.start[i + 1]) ++i;   // uniform over the workgroup
-  const HxSplit8 a{0, d.W[i], d.C[i], d.R[i], d.C[i], d.q[i], d.s[i], d.qt[i], d.st[i], nullptr, d.C[i] % 4 == 0};
+  const HxSplit8 a{0, d.W[i], d.C[i], d.R[i], d.C[i], d.q[i], d.s[i], d.qt[i], d.st[i], nullptr};
   split8_tile<TileF32>(a, blockIdx.x - d.start[i], lds);
 }
 
@@ -244,13 +244,13 @@ __device__ __forceinline__ Gelu gelu_parts(float u) {
 template <typename T>
 __global__ __launch_bounds__(NT) void gelu8_fwd_k(const T* __restrict__ y, const float* __restrict__ b,
                                                 T* __restrict__ out, uint8_t* __restrict__ q, uint8_t* __restrict__ s,
-                                                int64_t nblk, int nb, int N, int vec) {
+                                                int64_t nblk, int nb, int N) {
   const int l16 = threadIdx.x & 15;
   for (int64_t i = (blockIdx.x * (int64_t)NT + threadIdx.x) >> 4; i < nblk; i += (int64_t)gridDim.x * (NT / 16)) {
     const int64_t r = i / nb;
     const int c0 = (int)(i - r * nb) * 128 + 8 * l16, n = N - c0;
     float v[8], bb[8];
-    load_upto<T>(y + r * N + c0, n, vec, v);
+    load_upto<T>(y + r * N + c0, n, v);
     float m = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[k]));
@@ -261,13 +261,13 @@ __global__ __launch_bounds__(NT) void gelu8_fwd_k(const T* __restrict__ y, const
     if (l16 == 0) s[i] = (uint8_t)(e + 127);
 #pragma unroll
     for (int k = 0; k < 8; ++k) bb[k] = 0.f;
-    if (b) load_upto<float>(b + c0, n, vec, bb);
+    if (b) load_upto<float>(b + c0, n, bb);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const float u = v[k] + bb[k];
       v[k] = u * gelu_parts(u).cdf;
     }
-    store_upto<T>(out + r * N + c0, n, vec, v);
+    store_upto<T>(out + r * N + c0, n, v);
   }
 }
 
@@ -275,8 +275,7 @@ __global__ __launch_bounds__(NT) void gelu8_fwd_k(const T* __restrict__ y, const
 template <typename T>
 __global__ __launch_bounds__(NT) void gelu8_bwd_k(const T* __restrict__ dout, const uint8_t* __restrict__ q,
                                                 const uint8_t* __restrict__ s, const float* __restrict__ b,
-                                                T* __restrict__ dy, float* __restrict__ partial, int64_t rows, int nb,
-                                                int N, int vec) {
+                                                T* __restrict__ dy, float* __restrict__ partial, int64_t rows, int nb, int N) {
   __shared__ float red[16][128];
   const int l16 = threadIdx.x & 15, rg = threadIdx.x >> 4;
   const int cb = blockIdx.x % nb, chunk = blockIdx.x / nb, c0 = cb * 128 + 8 * l16, n = N - c0;
@@ -284,11 +283,11 @@ __global__ __launch_bounds__(NT) void gelu8_bwd_k(const T* __restrict__ dout, co
   float bb[8], sum[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) bb[k] = sum[k] = 0.f;
-  if (b) load_upto<float>(b + c0, n, vec, bb);
+  if (b) load_upto<float>(b + c0, n, bb);
   for (int64_t r = (int64_t)chunk * kRowChunk + rg; r < r1; r += 16) {
     const int64_t i = r * nb + cb;
     float d[8];
-    load_upto<T>(dout + r * N + c0, n, vec, d);
+    load_upto<T>(dout + r * N + c0, n, d);
     const uint2 w = *reinterpret_cast<const uint2*>(q + i * 128 + 8 * l16);
     const float sc = scale_of(s[i]);
 #pragma unroll
@@ -299,7 +298,7 @@ __global__ __launch_bounds__(NT) void gelu8_bwd_k(const T* __restrict__ dout, co
       d[k] *= fmaf(u * (0.5641895835477563f / 1.41421f), g.bell, g.cdf);
       sum[k] += d[k];
     }
-    store_upto<T>(dy + r * N + c0, n, vec, d);
+    store_upto<T>(dy + r * N + c0, n, d);
   }
   if (!partial) return;
 #pragma unroll
@@ -316,13 +315,13 @@ __global__ __launch_bounds__(NT) void gelu8_bwd_k(const T* __restrict__ dout, co
 // ---------------------------------------------------------------- pack8 / unpack8
 template <typename T>
 __global__ __launch_bounds__(NT) void pack8_k(const T* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ s,
-                                            int64_t nblk, int nb, int N, int vec) {
+                                            int64_t nblk, int nb, int N) {
   const int l16 = threadIdx.x & 15;
   for (int64_t i = (blockIdx.x * (int64_t)NT + threadIdx.x) >> 4; i < nblk; i += (int64_t)gridDim.x * (NT / 16)) {
     const int64_t r = i / nb;
     const int c0 = (int)(i - r * nb) * 128 + 8 * l16;
     float v[8];
-    load_upto<T>(x + r * N + c0, N - c0, vec, v);
+    load_upto<T>(x + r * N + c0, N - c0, v);
     float m = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[k]));
@@ -336,7 +335,7 @@ __global__ __launch_bounds__(NT) void pack8_k(const T* __restrict__ x, uint8_t* 
 
 template <typename T>
 __global__ __launch_bounds__(NT) void unpack8_k(const uint8_t* __restrict__ q, const uint8_t* __restrict__ s,
-                                              T* __restrict__ x, int64_t nblk, int nb, int N, int vec) {
+                                              T* __restrict__ x, int64_t nblk, int nb, int N) {
   const int l16 = threadIdx.x & 15;
   for (int64_t i = (blockIdx.x * (int64_t)NT + threadIdx.x) >> 4; i < nblk; i += (int64_t)gridDim.x * (NT / 16)) {
     const int64_t r = i / nb;
@@ -346,7 +345,7 @@ __global__ __launch_bounds__(NT) void unpack8_k(const uint8_t* __restrict__ q, c
     float v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = int8_val(k < 4 ? w.x : w.y, k & 3, sc);
-    store_upto<T>(x + r * N + c0, N - c0, vec, v);
+    store_upto<T>(x + r * N + c0, N - c0, v);
   }
 }
 
@@ -379,34 +378,34 @@ void hx_split8_many(const HxSplit8Batch& d, hipStream_t stream) {
 }
 
 void hx_gelu8_fwd(int bf16, const void* y, const float* b, void* out, uint8_t* q, uint8_t* s, int64_t rows, int N,
-                  int vec, hipStream_t stream) {
+                  hipStream_t stream) {
   const int nb = (N + 127) / 128;
   const int64_t nblk = rows * nb;
-  if (bf16) gelu8_fwd_k<uint16_t><<<stream_grid(nblk), NT, 0, stream>>>((const uint16_t*)y, b, (uint16_t*)out, q, s, nblk, nb, N, vec);
-  else gelu8_fwd_k<float><<<stream_grid(nblk), NT, 0, stream>>>((const float*)y, b, (float*)out, q, s, nblk, nb, N, vec);
+  if (bf16) gelu8_fwd_k<uint16_t><<<stream_grid(nblk), NT, 0, stream>>>((const uint16_t*)y, b, (uint16_t*)out, q, s, nblk, nb, N);
+  else gelu8_fwd_k<float><<<stream_grid(nblk), NT, 0, stream>>>((const float*)y, b, (float*)out, q, s, nblk, nb, N);
 }
 
 int hx_gelu8_chunks(int64_t rows) { return (int)((rows + kRowChunk - 1) / kRowChunk); }
 
 void hx_gelu8_bwd(int bf16, const void* dout, const uint8_t* q, const uint8_t* s, const float* b, void* dy,
-                  float* partial, float* db, int64_t rows, int N, int vec, hipStream_t stream) {
+                  float* partial, float* db, int64_t rows, int N, hipStream_t stream) {
   const int nb = (N + 127) / 128;
   const unsigned grid = (unsigned)(nb * (int64_t)hx_gelu8_chunks(rows));
-  if (bf16) gelu8_bwd_k<uint16_t><<<grid, NT, 0, stream>>>((const uint16_t*)dout, q, s, b, (uint16_t*)dy, partial, rows, nb, N, vec);
-  else gelu8_bwd_k<float><<<grid, NT, 0, stream>>>((const float*)dout, q, s, b, (float*)dy, partial, rows, nb, N, vec);
+  if (bf16) gelu8_bwd_k<uint16_t><<<grid, NT, 0, stream>>>((const uint16_t*)dout, q, s, b, (uint16_t*)dy, partial, rows, nb, N);
+  else gelu8_bwd_k<float><<<grid, NT, 0, stream>>>((const float*)dout, q, s, b, (float*)dy, partial, rows, nb, N);
   if (partial) fold_rows(partial, hx_gelu8_chunks(rows), N, N, N, db, nullptr, nullptr, 0, stream);
 }
 
-void hx_pack8(int bf16, const void* x, uint8_t* q, uint8_t* s, int64_t rows, int N, int vec, hipStream_t stream) {
+void hx_pack8(int bf16, const void* x, uint8_t* q, uint8_t* s, int64_t rows, int N, hipStream_t stream) {
   const int nb = (N + 127) / 128;
   const int64_t nblk = rows * nb;
-  if (bf16) pack8_k<uint16_t><<<stream_grid(nblk), NT, 0, stream>>>((const uint16_t*)x, q, s, nblk, nb, N, vec);
-  else pack8_k<float><<<stream_grid(nblk), NT, 0, stream>>>((const float*)x, q, s, nblk, nb, N, vec);
+  if (bf16) pack8_k<uint16_t><<<stream_grid(nblk), NT, 0, stream>>>((const uint16_t*)x, q, s, nblk, nb, N);
+  else pack8_k<float><<<stream_grid(nblk), NT, 0, stream>>>((const float*)x, q, s, nblk, nb, N);
 }
 
-void hx_unpack8(int bf16, const uint8_t* q, const uint8_t* s, void* x, int64_t rows, int N, int vec, hipStream_t stream) {
+void hx_unpack8(int bf16, const uint8_t* q, const uint8_t* s, void* x, int64_t rows, int N, hipStream_t stream) {
   const int nb = (N + 127) / 128;
   const int64_t nblk = rows * nb;
-  if (bf16) unpack8_k<uint16_t><<<stream_grid(nblk), NT, 0, stream>>>(q, s, (uint16_t*)x, nblk, nb, N, vec);
-  else unpack8_k<float><<<stream_grid(nblk), NT, 0, stream>>>(q, s, (float*)x, nblk, nb, N, vec);
+  if (bf16) unpack8_k<uint16_t><<<stream_grid(nblk), NT, 0, stream>>>(q, s, (uint16_t*)x, nblk, nb, N);
+  else unpack8_k<float><<<stream_grid(nblk), NT, 0, stream>>>(q, s, (float*)x, nblk, nb, N);
 }
