@@ -129,7 +129,6 @@ __device__ __forceinline__ uint32_t max16u(uint32_t m) {
   m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, false));   // mirrored in 8
   return max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xF, 0xF, false));   // mirrored in 16
 }
-__device__ __forceinline__ float max16(float m) { return __uint_as_float(max16u(__float_as_uint(m))); }   // m >= 0
 
 }  // namespace q8
 }  // namespace hx
