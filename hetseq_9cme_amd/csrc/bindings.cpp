@@ -1081,6 +1081,14 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
 Tensor linear_fp8(Tensor x, OptT W, OptT b, std::vector<OptT> w8, bool grad) {
   TORCH_CHECK(w8.empty() ? has(W) : w8.size() == 4 && has(w8[0]) && has(w8[1]), "linear_fp8: a weight or its codes and scales");
   if (w8.empty()) return LinearFp8::apply(x, W, b, OptT(), OptT(), OptT(), OptT(), grad);
+  const bool wanted = grad && (x.requires_grad() || (has(W) && W->requires_grad()) || (has(b) && b->requires_grad()));
+  if (!wanted) {   // inference: no node
+    at::NoGradGuard no_grad;
+    if (x.dim() == 2 && x.is_contiguous()) return linear_fp8_y(x, *w8[0], *w8[1], b, false, nullptr, nullptr);
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = w8[0]->size(0);
+    return linear_fp8_y(as_rows8(x), *w8[0], *w8[1], b, false, nullptr, nullptr).view(shape);
+  }
   return LinearFp8::apply(x, W, b, w8[0], w8[1], w8[2], w8[3], grad);
 }
 
