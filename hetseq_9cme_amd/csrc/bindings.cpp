@@ -4,6 +4,7 @@
 // and RCCL, and are capturable into HIP graphs).
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/extension.h>
 
 #include "hx_launch.h"
@@ -846,6 +847,10 @@ static void gemm8_run(const uint8_t* a, const uint8_t* as, int64_t M, const uint
                       const Tensor& out, bool beta, const float* bias) {
   const bool out_bf16 = out.scalar_type() == torch::kBFloat16;
   const int es = out_bf16 ? 2 : 4;
+  // a tile's rows of codes and an operand's scale words lie within one buffer descriptor each
+  const int64_t groups = (blocks128(K) + 3) / 4, most = 1LL << 31;
+  TORCH_CHECK(K <= (1LL << 22) && std::max(M, N) < most - 256 && (std::max(M, N) + 3) / 4 * groups * 16 < most,
+              "gemm_fp8: at most 2^22 deep, fewer than 2^31 rows and bytes of scale words (rows / 4 x depth / 512 x 16)");
   HxGemm8 g{};
   g.A = a;
   g.sa = reinterpret_cast<const uint32_t*>(as);
@@ -969,6 +974,25 @@ struct Codes8 {
   uint8_t* s(uint8_t* base) const { return bytes() ? base + qb : nullptr; }
 };
 
+// A gradient that is captured into a graph for a leaf whose accumulator was made on another stream (an
+// eager graph of the same leaf is alive): autograd would make that stream wait for the capturing one,
+// which a capture cannot hold and which ends the process.  Refused before it comes to that.
+static void refuse_stale_leaves(const Tensor& like, const char* what) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(cur_stream(like), &st) != hipSuccess || st == hipStreamCaptureStatusNone) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (const auto& e : node->next_edges()) {
+    if (!e.function || !dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get())) continue;
+    const auto s = e.function->stream();
+    TORCH_CHECK(!s || s->id() == c10::hip::getCurrentHIPStream(like.get_device()).id(), what,
+                ": a captured backward needs its leaves' eager graphs released first (one of them lives on another stream)");
+  }
+}
+static void refuse_second_derivative(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, ": first derivatives only (create_graph=True is not supported)");
+}
+
 // The whole layer as one autograd node for parameters that autograd accumulates itself (no flat gradient
 // slots, no residual mailbox).  A small layer's step is bound by the host: a node in C++ runs its
 // backward without the interpreter lock, all of a direction's codes share one workspace, and x and W
@@ -1038,6 +1062,8 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
     return y.view(shape);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    refuse_second_derivative("linear_fp8");
+    refuse_stale_leaves(g[0], "linear_fp8");
     const auto saved = ctx->get_saved_variables();
     const auto xshape = ctx->saved_data["xshape"].toIntVector();
     const int64_t N = ctx->saved_data["N"].toInt(), K = xshape.back();
@@ -1152,6 +1178,8 @@ struct BiasGelu8 : public torch::autograd::Function<BiasGelu8> {
     return r[0];
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    refuse_second_derivative("bias_act(bits=8)");
+    refuse_stale_leaves(g[0], "bias_act(bits=8)");
     const auto saved = ctx->get_saved_variables();
     const bool need_b = saved[2].defined() && ctx->needs_input_grad(1);
     std::vector<OptT> r = gelu8_bwd(g[0].contiguous(), saved[0], saved[1], saved[2].defined() ? OptT(saved[2]) : OptT(), need_b, c10::nullopt);
@@ -1171,7 +1199,7 @@ std::vector<Tensor> pack8(Tensor x) {
 }
 
 Tensor unpack8(Tensor q, Tensor s, int64_t N, bool bf16) {
-  TORCH_CHECK(q.dim() == 3 && N >= 1 && q.size(1) == blocks128(N) && q.size(2) == 128, "unpack8: codes [rows, ceil(N / 128), 128]");
+  TORCH_CHECK(q.dim() == 3 && N >= 1 && N < (1LL << 30) && q.size(1) == blocks128(N) && q.size(2) == 128, "unpack8: codes [rows, ceil(N / 128), 128]");
   const int64_t rows = q.size(0);
   check_kept(q, s, q, rows, N, "unpack8");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());

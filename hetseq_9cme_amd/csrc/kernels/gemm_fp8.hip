@@ -16,6 +16,7 @@
 //    LDS read, and v_mfma_f32_32x32x16_bf16, which sums exact products in fp32 (1e-7): the products
 //    whose result is kept in fp32 (weight gradients, fp32 activations).  Half the matrix rate.
 #include <algorithm>
+#include <atomic>
 
 #include "hx_gemm.h"
 #include "hx_launch.h"
@@ -494,10 +495,16 @@ int launch(const HxGemm8& g, hipStream_t s) {
   constexpr int NT = (BM / WM) * (BN / WN) * 64;
   constexpr int LDS = 2 * (BM + BN) * 128 + 4096 + 2048 + 1024;   // stages, scale words, biases, spare
   auto k = gemm_fp8_k<BM, BN, WM, WN, WGS, EXACT, OB>;
-  static const hipError_t ok = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-  if (ok != hipSuccess) return 1;
+  static std::atomic<uint64_t> allowed{0};   // devices on which the kernel may take this much LDS
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 1;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return 1;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   const int64_t items = (int64_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN) * g.ks;
-  if (items > 0x7fffffff) return 1;
+  if (items > 0x7ffffff0) return 1;
   // one workgroup per item, at most what the CUs hold at a time -- but where an item is one k block, which
   // leaves no room for the next one's first two stages
   const int gper = ((g.nkb + 3) / 4 + g.ks - 1) / g.ks * 4, last = g.nkb - (g.ks - 1) * gper;

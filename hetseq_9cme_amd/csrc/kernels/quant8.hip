@@ -245,7 +245,7 @@ __global__ __launch_bounds__(SNT) void split8_k(HxSplit8 a, HxSplit8 b) {
   }
 }
 
-// every weight of an encoder at once (ops.fp8_scope): one launch per forward instead of one per layer
+// every weight of an encoder at once (ops.fp8_weights): one launch per forward instead of one per layer
 __global__ __launch_bounds__(SNT) void split8_many_k(HxSplit8Batch d) {
   __shared__ __attribute__((aligned(16))) Split8Lds lds;
   int i = 0;

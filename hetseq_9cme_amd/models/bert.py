@@ -21,6 +21,7 @@ The compute path is different: every hot op goes through ``hetseq_9cme_amd.ops``
   * the MLM head only runs on the masked rows (gathered without host sync) and the
     decoder bias + softmax-cross-entropy (+ its gradient) is one kernel.
 """
+import contextlib
 import copy
 import json
 import logging
@@ -112,6 +113,7 @@ class LinearActivation(nn.Module):
     """Linear + activation; GELU/tanh with bias run as one fused epilogue kernel."""
     __constants__ = ['bias']
     fp8 = False     # set_compute_dtype(fp8=True): e4m3 products, 8-bit kept activations (encoder layers)
+    codes = None    # the weight's e4m3 codes while its encoder's forward runs (BertEncoder)
 
     def __init__(self, in_features, out_features, act='gelu', bias=True):
         super().__init__()
@@ -135,7 +137,7 @@ class LinearActivation(nn.Module):
 
     def forward(self, x, res_grad=None):
         if self.fp8:
-            y = ops.linear_fp8(x, self.weight, res_grad=res_grad)
+            y = ops.linear_fp8(x, self.weight, res_grad=res_grad, codes=self.codes)
             if self.act == 'gelu':   # the backward reads y from int8 blocks
                 return ops.bias_act(y, self.bias, 'gelu', bits=8)
         else:
@@ -189,7 +191,7 @@ _QKV_BIAS_EPILOGUE = os.environ.get('HX_QKV_BIAS_EPILOGUE', '1') != '0'
 
 
 class BertSelfAttention(nn.Module):
-    fp8 = False
+    fp8, codes = False, None
 
     def __init__(self, config):
         super().__init__()
@@ -208,7 +210,7 @@ class BertSelfAttention(nn.Module):
         bias = (self.query.bias, self.key.bias, self.value.bias)
         if self.fp8:
             qkv = ops.linear3_fp8(hidden_states, self.query.weight, self.key.weight, self.value.weight, *bias,
-                                  res_grad=res_grad, bias_grad=False)
+                                  res_grad=res_grad, bias_grad=False, codes=self.codes)
             return ops.attention(qkv, attention_mask_bias, self.num_attention_heads, self.dropout.p, self.training,
                                  bias_grad=bias)
         if _QKV_BIAS_EPILOGUE:
@@ -226,7 +228,7 @@ class BertSelfAttention(nn.Module):
 
 
 class BertSelfOutput(nn.Module):
-    fp8 = False
+    fp8, codes = False, None
 
     def __init__(self, config):
         super().__init__()
@@ -235,7 +237,8 @@ class BertSelfOutput(nn.Module):
         self.dropout = nn.Dropout(config.hidden_dropout_prob)
 
     def forward(self, hidden_states, input_tensor, res_grad=None):
-        y = (ops.linear_fp8 if self.fp8 else ops.linear)(hidden_states, self.dense.weight)
+        y = (ops.linear_fp8(hidden_states, self.dense.weight, codes=self.codes) if self.fp8
+             else ops.linear(hidden_states, self.dense.weight))
         return ops.bias_dropout_residual_ln(y, self.dense.bias, input_tensor, self.LayerNorm.weight,
                                             self.LayerNorm.bias, self.LayerNorm.variance_epsilon,
                                             self.dropout.p, self.training, res_grad=res_grad)
@@ -264,7 +267,7 @@ class BertIntermediate(nn.Module):
 
 
 class BertOutput(nn.Module):
-    fp8 = False
+    fp8, codes = False, None
 
     def __init__(self, config):
         super().__init__()
@@ -273,8 +276,9 @@ class BertOutput(nn.Module):
         self.dropout = nn.Dropout(config.hidden_dropout_prob)
 
     def forward(self, hidden_states, input_tensor, res_grad=None):
-        linear = ops.linear_fp8 if self.fp8 else ops.linear
-        return self.finish(linear(hidden_states, self.dense.weight), input_tensor, res_grad)
+        y = (ops.linear_fp8(hidden_states, self.dense.weight, codes=self.codes) if self.fp8
+             else ops.linear(hidden_states, self.dense.weight))
+        return self.finish(y, input_tensor, res_grad)
 
     def finish(self, y, input_tensor, res_grad=None):
         """dense bias -> dropout -> + residual -> LayerNorm on the bias-less projection ``y``."""
@@ -327,7 +331,7 @@ class BertEncoder(nn.Module):
     def forward(self, hidden_states, attention_mask_bias, output_all_encoded_layers=True,
                 checkpoint_activations=False):
         fp8 = len(self.layer) > 0 and self.layer[0].output.fp8
-        with (ops.fp8_scope(self._piece_weights()) if fp8 else ops.weight_pieces_scope(self._piece_weights(), hidden_states)):
+        with (self._weight_codes() if fp8 else ops.weight_pieces_scope(self._piece_weights(), hidden_states)):
             return self._forward(hidden_states, attention_mask_bias, output_all_encoded_layers,
                                  checkpoint_activations)
 
@@ -345,6 +349,26 @@ class BertEncoder(nn.Module):
                        layer.intermediate.dense_act.weight, layer.output.dense.weight]
             self.__dict__['_pw_params'] = ps
         return [ops.qkv_weight_view(*p) if isinstance(p, tuple) else p for p in ps]
+
+    @contextlib.contextmanager
+    def _weight_codes(self):
+        """The e4m3 codes of every linear weight, made in one launch and handed to the layers for this
+        forward alone (a segment recomputed in the backward makes its own)."""
+        parts = self.__dict__.get('_fp8_parts')
+        if parts is None or len(parts) != 4 * len(self.layer):
+            parts = self.__dict__['_fp8_parts'] = [
+                part for layer in self.layer for part in (layer.attention.self, layer.attention.output,
+                                                          layer.intermediate.dense_act, layer.output)]
+        # the weights as the parts hold them now (a replaced layer is not in `parts`: it makes its own codes)
+        Ws = [ops.qkv_weight_view(part.query.weight, part.key.weight, part.value.weight) if isinstance(part, BertSelfAttention)
+              else part.weight if isinstance(part, LinearActivation) else part.dense.weight for part in parts]
+        try:
+            for part, codes in zip(parts, ops.fp8_weights(Ws)):
+                part.__dict__['codes'] = codes
+            yield
+        finally:
+            for part in parts:
+                part.__dict__['codes'] = None
 
     def _forward(self, hidden_states, attention_mask_bias, output_all_encoded_layers, checkpoint_activations):
         all_encoder_layers = []

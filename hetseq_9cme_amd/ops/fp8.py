@@ -57,6 +57,11 @@ def _check_bias(b, n, like, what):
             what, n, like.device, b.dtype, tuple(b.shape), b.device))
 
 
+def _first_derivatives(what):
+    if torch.is_grad_enabled():
+        raise RuntimeError('{}: first derivatives only (create_graph=True is not supported)'.format(what))
+
+
 # ---------------------------------------------------------------- references (CPU, and the numerics oracle)
 def _blocks_ref(x, largest):
     """x / 2^e per block of the last dimension, and 2^e, as [..., blocks, 128] fp32."""
@@ -90,8 +95,9 @@ def _gelu_grad_ref(u):
 # ---------------------------------------------------------------- operands
 class Fp8Weight(object):
     """A weight's e4m3 codes for ``linear_fp8``: of W [N, K] blocked along K (the forward) and of W^T
-    blocked along N (the data gradient; ``grad=False`` leaves it out: inference).  A served model
-    builds it once; training builds it per forward (``fp8_scope`` does, for a whole encoder)."""
+    blocked along N (the data gradient; ``grad=False`` leaves it out: inference).  They are of W's
+    values when it was built: a served model builds it once, training once per forward
+    (``fp8_weights`` for a whole encoder)."""
     __slots__ = ('shape', 'dtype', 'device', 'q', 's', 'qt', 'st', 'ref')
 
     def __init__(self, W, grad=True):
@@ -116,40 +122,32 @@ class Fp8Weight(object):
         return self.qt is not None or (self.ref is not None and self.ref[1] is not None)
 
 
-class _Scope(object):
-    weights = None      # {(data_ptr, shape): Fp8Weight} of the running forward
+def fp8_weights(Ws):
+    """``Fp8Weight`` of every weight in ``Ws`` (None stays None), contiguous fp32 ones on the GPU 64 to a
+    launch: the ``codes`` of a whole encoder's layers for one forward."""
+    out, batch = [None] * len(Ws), []
+    for i, W in enumerate(Ws):
+        if W is None:
+            continue
+        if use_kernels(W) and W.dim() == 2 and W.numel() and W.dtype == torch.float32 and W.is_contiguous() and W.data_ptr() % 16 == 0:
+            batch.append(i)
+        else:
+            out[i] = Fp8Weight(W)
+    for o in range(0, len(batch), 64):
+        part = batch[o:o + 64]
+        for i, t in zip(part, C().split8_weights([Ws[j].detach() for j in part])):
+            out[i] = Fp8Weight._of(Ws[i], *t)
+    return out
 
 
-class fp8_scope(object):
-    """``Fp8Weight`` copies of every weight in ``Ws`` for the running forward, made in one launch:
-    ``linear_fp8`` / ``linear3_fp8`` find them by the weight.  A recompute outside the scope makes its
-    own."""
-
-    def __init__(self, Ws):
-        self.Ws = [W for W in Ws if W is not None]
-
-    def __enter__(self):
-        self.prev = _Scope.weights
-        d = {}
-        Ws = [W.detach() for W in self.Ws if use_kernels(W) and W.dtype == torch.float32 and W.is_contiguous() and
-              W.data_ptr() % 16 == 0]
-        for i in range(0, len(Ws), 64):
-            chunk = Ws[i:i + 64]
-            for W, t in zip(chunk, C().split8_weights(chunk)):
-                d[(W.data_ptr(), tuple(W.shape))] = Fp8Weight._of(W, *t)
-        _Scope.weights = d
-        return self
-
-    def __exit__(self, *exc):
-        _Scope.weights = self.prev
-        return False
-
-
-def _scoped(W):
-    """The running ``fp8_scope``'s copy of W, if it has one."""
-    if _Scope.weights is None:
-        return None
-    return _Scope.weights.get((W.data_ptr(), tuple(W.shape)))
+def _check_codes(codes, shape, device, need_grad, what):
+    if not isinstance(codes, Fp8Weight):
+        raise TypeError('{}: codes must be an Fp8Weight, got {}'.format(what, type(codes).__name__))
+    if codes.shape != shape or codes.device != device:
+        raise ValueError('{}: codes of a {} weight on {}, the weight is {} on {}'.format(
+            what, codes.shape, codes.device, shape, device))
+    if need_grad and not codes.has_grad:
+        raise ValueError('{}: x needs a gradient, the Fp8Weight was built with grad=False'.format(what))
 
 
 def _rows2(x):
@@ -187,6 +185,7 @@ class _LinearFp8Fn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        _first_derivatives('linear_fp8')
         xt, xs, wt, ws = ctx.saved_tensors
         n, Ws, bs = ctx.n, ctx.Ws, ctx.bs
         N, K = ctx.wshape
@@ -259,11 +258,13 @@ def _residual(dx, mbox):
     return dx if g is None else dx + g.view(dx.shape).to(dx.dtype)
 
 
-def linear_fp8(x, W, b=None, res_grad=None):
+def linear_fp8(x, W, b=None, res_grad=None, codes=None):
     """x W^T (+ b) with e4m3 operands (one power-of-two scale per block of 128; see the module's
     formulas).  ``x`` [.., K] fp32 or bf16 (the result has its type); ``W`` [N, K] a parameter, or an
     ``Fp8Weight`` (then it gets no gradient: inference, frozen layers); ``b`` fp32 [N].
-    ``res_grad``: see ``ResidualGrad``."""
+    ``codes``: the parameter's ``Fp8Weight``, where the caller has made it for this forward
+    (``fp8_weights``).  ``res_grad``: see ``ResidualGrad``.  First derivatives only; at most 2^22
+    features in or out, and in a training step 2^22 rows."""
     _check_act(x, 'linear_fp8')
     kept = isinstance(W, Fp8Weight)
     if not kept:
@@ -275,9 +276,9 @@ def linear_fp8(x, W, b=None, res_grad=None):
         raise ValueError('linear_fp8: x on {}, the weight on {}'.format(x.device, W.device))
     _check_bias(b, N, x, 'linear_fp8')
     grad = torch.is_grad_enabled()
-    w8 = W if kept else _scoped(W)
-    if grad and x.requires_grad and w8 is not None and not w8.has_grad:
-        raise ValueError('linear_fp8: x needs a gradient, the Fp8Weight was built with grad=False')
+    w8 = W if kept else codes
+    if w8 is not None:
+        _check_codes(w8, (N, K), W.device, grad and x.requires_grad, 'linear_fp8')
     if use_kernels(x) and res_grad is None and (kept or not _flat(W)) and not _flat(b):
         # autograd keeps the gradients: the whole layer is one node (bindings.cpp LinearFp8)
         return C().linear_fp8(x, None if kept else W, b, [] if w8 is None else [w8.q, w8.s, w8.qt, w8.st], grad)
@@ -292,17 +293,25 @@ def _flat(p):
     return getattr(p, '_hx_flat', None) is not None
 
 
-def linear3_fp8(x, wq, wk, wv, bq, bk, bv, res_grad=None, bias_grad=True):
-    """``linear3`` on e4m3 operands: the Q / K / V projections as one product (N = 3H)."""
+def linear3_fp8(x, wq, wk, wv, bq, bk, bv, res_grad=None, bias_grad=True, codes=None):
+    """``linear3`` on e4m3 operands: the Q / K / V projections as one product (N = 3H).  ``codes``: the
+    ``Fp8Weight`` of the three weights stacked."""
     _check_act(x, 'linear3_fp8')
     W = fused._adjacent_view([wq, wk, wv])
     W = W if W is not None else torch.cat([wq.detach(), wk.detach(), wv.detach()], 0)
+    _check_weight(W, 'linear3_fp8')
+    if x.shape[-1] != W.shape[1] or x.device != W.device:
+        raise ValueError('linear3_fp8: x {} on {}, the weights take {} features on {}'.format(
+            tuple(x.shape), x.device, W.shape[1], W.device))
     bs, bias = (), None
     if bq is not None:
         bs, bias = (bq, bk, bv), fused._adjacent_view([bq, bk, bv])
         bias = bias if bias is not None else torch.cat([t.detach() for t in bs], 0)
     _check_bias(bias, W.shape[0], x, 'linear3_fp8')
-    w8 = _scoped(W) or Fp8Weight(W, torch.is_grad_enabled() and x.requires_grad)
+    need = torch.is_grad_enabled() and x.requires_grad
+    if codes is not None:
+        _check_codes(codes, tuple(W.shape), W.device, need, 'linear3_fp8')
+    w8 = codes if codes is not None else Fp8Weight(W, need)
     return _LinearFp8Fn.apply(x, w8, bias, res_grad, bool(bias_grad), 3, wq, wk, wv, *bs)
 
 
@@ -322,6 +331,7 @@ class _BiasGelu8Fn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
+        _first_derivatives('bias_act(bits=8)')
         q, s = ctx.saved_tensors
         b, need_b = ctx.b, ctx.needs_input_grad[1]
         if use_kernels(dout):

@@ -392,3 +392,166 @@ def test_results_repeat_bit_for_bit(dev):
     for _ in range(3):
         for a, b in zip(first, torch.autograd.grad(ops.linear_fp8(x, W), (x, W), d)):
             assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- calls side by side
+def test_bias_at_any_element(dev):
+    """A bias that starts between two 16-B boundaries (a view into a larger buffer)."""
+    W = rand((130, 200), torch.float32, 2) * 0.02
+    buf = rand((140,), torch.float32, 3)
+    for dt in (torch.float32, torch.bfloat16):
+        for M in (5, 300):
+            x = rand((M, 200), dt, M)
+            for o in (0, 1, 2, 3):
+                b = buf[o:o + 130]
+                assert_product(ops.linear_fp8(x, W, b), e4m3(x), e4m3(W), bias=b)
+                y = rand((M, 130), dt, 7)
+                assert torch.equal(ops.bias_act(y, b, 'gelu', bits=8), ops.bias_act(y, b.clone(), 'gelu', bits=8))
+
+
+def test_given_codes(dev):
+    """A parameter with codes made beforehand: the same bits as without, for one weight and for a batch
+    of every kind of weight (more than one launch holds)."""
+    Ws = [(rand((64 + i, 130), torch.float32, i) * 0.02) for i in range(70)]
+    Ws[5] = Ws[5].to(torch.bfloat16)
+    Ws[9] = torch.cat([Ws[9], Ws[9]], 1)[:, :130]     # rows 260 apart
+    Ws[11] = None
+    codes = ops.fp8_weights(Ws)
+    assert codes[11] is None and len(codes) == 70
+    x = rand((200, 130), torch.bfloat16, 1).requires_grad_(True)
+    for i in (0, 5, 9, 63, 64, 69):
+        W = Ws[i].detach().requires_grad_(True)
+        d = rand((200, W.shape[0]), torch.bfloat16, 3)
+        res = []
+        for c in (codes[i], None):
+            y = ops.linear_fp8(x, W, codes=c)
+            res.append((y,) + torch.autograd.grad(y, (x, W), d))
+        assert all(torch.equal(a, b) for a, b in zip(*res)), i
+    q = [(rand((128, 128), torch.float32, i) * 0.02).requires_grad_(True) for i in range(3)]
+    x = rand((200, 128), torch.bfloat16, 1)
+    c = ops.Fp8Weight(torch.cat(q))
+    assert torch.equal(ops.linear3_fp8(x, *q, None, None, None, codes=c), ops.linear3_fp8(x, *q, None, None, None))
+
+
+def test_two_streams_at_once(dev):
+    """Training passes on two streams, none waiting for the other: each as when it runs alone."""
+    def data(i):
+        return ((rand((300 + 50 * i, 256), torch.bfloat16, i)).requires_grad_(True),
+                (rand((512, 256), torch.float32, 10 + i) * 0.03).requires_grad_(True), rand((512,), torch.float32, 20 + i).requires_grad_(True),
+                (rand((256, 512), torch.float32, 30 + i) * 0.03).requires_grad_(True), rand((256,), torch.float32, 40 + i).requires_grad_(True))
+
+    def step(t, d):
+        y = layer(*t)
+        return (y,) + torch.autograd.grad(y, t, d)
+    sets = [data(0), data(1)]
+    ds = [rand(t[0].shape, torch.bfloat16, 50) for t in sets]
+    alone = [step(t, d) for t, d in zip(sets, ds)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(step(sets[i], ds[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, alone[i]))
+
+
+def _captured(step):
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        step()
+    torch.cuda.current_stream().wait_stream(st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    return graph, [t.detach() for t in out]
+
+
+def test_two_captured_graphs(dev):
+    """Two captured passes over the same weights, replayed by turns: neither touches the other's memory."""
+    W = (rand((384, 256), torch.float32, 1) * 0.03).requires_grad_(True)
+    b = rand((384,), torch.float32, 2).requires_grad_(True)
+    xs = [rand((M, 256), torch.bfloat16, M).requires_grad_(True) for M in (41, 500)]
+    ds = [rand((x.shape[0], 384), torch.bfloat16, 5) for x in xs]
+
+    def step(i):
+        y = ops.bias_act(ops.linear_fp8(xs[i], W), b, 'gelu', bits=8)
+        return (y,) + torch.autograd.grad(y, (xs[i], W, b), ds[i])
+    graphs = [_captured(lambda i=i: step(i)) for i in (0, 1)]
+    for turn in (0, 1, 0, 0, 1, 1):
+        with torch.no_grad():
+            xs[turn].copy_(rand(xs[turn].shape, torch.bfloat16, 100 + turn))
+        graphs[turn][0].replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in graphs[turn][1]]
+        assert all(torch.equal(a, c) for a, c in zip(got, step(turn))), turn
+
+
+def test_second_derivatives_are_refused(dev):
+    x = rand((30, 128), torch.bfloat16, 1).requires_grad_(True)
+    W = (rand((64, 128), torch.float32, 2) * 0.02).requires_grad_(True)
+    for y in (ops.linear_fp8(x, W), ops.bias_act(x, None, 'gelu', bits=8)):
+        with pytest.raises(RuntimeError, match='first derivatives only'):
+            torch.autograd.grad(y.float().sum(), x, create_graph=True)
+
+
+def test_rows_past_two_to_the_31st_element(dev):
+    """x of 2.3e9 elements: the last rows of the results, and the codes and sums over all of them."""
+    M, K, N = 560_000, 4096, 64
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device=dev)
+    tail = rand((300, K), torch.bfloat16, 1)
+    x[-300:] = tail
+    x.requires_grad_(True)
+    W = (rand((N, K), torch.float32, 2) * 0.02).requires_grad_(True)
+    y = ops.linear_fp8(x, W)
+    dy = torch.zeros(M, N, dtype=torch.bfloat16, device=dev)
+    dy[-300:] = rand((300, N), torch.bfloat16, 3)
+    dx, dW = torch.autograd.grad(y, (x, W), dy)
+    with torch.no_grad():
+        assert not y[:-300].any() and not dx[:-300].any()
+        assert_product(y[-300:], e4m3(tail), e4m3(W))
+        assert_product(dx[-300:], e4m3(dy[-300:]), e4m3(W.t().contiguous()))
+        # 560 000 = 4375 blocks of 128: the last 300 rows are the end of block 4372 and blocks 4373, 4374
+        cut = M - 384
+        assert_product(dW, e4m3(dy[cut:].t().contiguous()), e4m3(x[cut:].detach().t().contiguous()))
+        del y, dx, dW
+        got = ops.unpack8(ops.pack8(x))
+        assert not got[:-300].any() and torch.equal(got[-300:], ops.unpack8(ops.pack8(tail)))
+        del got
+    g = ops.bias_act(x, None, 'gelu', bits=8)
+    one = ops.bias_act(tail.requires_grad_(True), None, 'gelu', bits=8)
+    assert torch.equal(g[-300:], one)
+    d = rand((300, K), torch.bfloat16, 4)
+    dg = torch.zeros_like(g)
+    dg[-300:] = d
+    a, = torch.autograd.grad(g, x, dg)
+    b, = torch.autograd.grad(one, tail, d)
+    assert torch.equal(a[-300:], b) and not a[:-300].any()
+
+
+def test_capture_is_refused_while_an_eager_graph_lives(dev):
+    """A leaf's gradient accumulator that an eager graph on another stream holds cannot take part in a
+    capture: an error from the layer's backward, and the same capture works once that graph is gone."""
+    x = rand((100, 128), torch.bfloat16, 1)
+    W = (rand((64, 128), torch.float32, 2) * 0.02).requires_grad_(True)
+    d = rand((100, 64), torch.bfloat16, 3)
+    alive = ops.linear_fp8(x, W)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        y = ops.linear_fp8(x, W)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match='eager graphs released first'):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(ops.linear_fp8(x, W), W, d)
+    del alive, y
+    graph, out = _captured(lambda: torch.autograd.grad(ops.linear_fp8(x, W), W, d))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], torch.autograd.grad(ops.linear_fp8(x, W), W, d)[0])
