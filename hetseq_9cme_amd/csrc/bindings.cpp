@@ -919,7 +919,7 @@ Tensor gemm_fp8(Tensor a, Tensor as, Tensor b, Tensor bs, int64_t K, bool out_bf
 // gradient's operand).  Few rows that need no such copy go through one launch (fp8_rows_k).
 static Tensor linear_fp8_y(const Tensor& x2, const Tensor& wq, const Tensor& ws, const OptT& bias, bool keep, OptT* qt, OptT* st) {
   const int64_t M = x2.size(0), K = x2.size(1), N = wq.size(0);
-  if (!keep && M > 0 && M <= hx_fp8_rows_max()) {
+  if (!keep && hx_fp8_rows_fit(M, blocks128(K), act_bf16(x2))) {
     check_rows8(x2, "linear_fp8");
     TORCH_CHECK(wq.is_cuda() && wq.device() == x2.device() && wq.size(1) == blocks128(K) * 128 && wq.is_contiguous() && aligned16(wq.data_ptr()) &&
                     ws.numel() == (blocks128(K) + 3) / 4 * ((N + 3) / 4 * 4) * 4, "linear_fp8: the weight's codes do not fit x");

@@ -288,7 +288,7 @@ void hx_gemm_fp8_plan(int M, int N, int nkb, int exact, int* cfg, int* ks);   //
 int hx_gemm_fp8(const HxGemm8& g, int cfg, int exact, int out_bf16, hipStream_t s);
 void hx_gemm_fp8_slabs(const float* part, void* out, int out_bf16, int64_t ldc, int M, int N, int ks, const float* bias,
                        int beta, int vec, hipStream_t s);
-// y [M, N] (x's type, contiguous) = Q(x) B^T (+ bias) for M <= hx_fp8_rows_max() rows of fp32 or bf16 x
+// y [M, N] (x's type, contiguous) = Q(x) B^T (+ bias) for few rows (hx_fp8_rows_fit) of fp32 or bf16 x
 // (row stride ldx), B as in HxGemm8
 struct HxRows8 {
   const void* x;
@@ -300,5 +300,5 @@ struct HxRows8 {
   const float* bias;
   int M, N, K, nkb;
 };
-int hx_fp8_rows_max();
+int hx_fp8_rows_fit(int64_t M, int64_t nkb, int bf16);   // rows and k blocks it is the faster way for (M <= 64)
 int hx_fp8_rows(const HxRows8& g, int bf16, hipStream_t s);
