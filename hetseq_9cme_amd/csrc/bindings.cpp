@@ -842,9 +842,15 @@ std::vector<std::vector<Tensor>> split8_weights(std::vector<Tensor> Ws) {
   return out;
 }
 
-// out [M, N] (fp32 or bf16, unit column stride) (+)= A . B^T (+ bias) from split8's codes and scale words
+// what a layer's products leave to add up, and the memory it is in
+struct Finish8 {
+  HxFinish f{};
+  Tensor part[2];
+};
+// out [M, N] (fp32 or bf16, unit column stride) (+)= A . B^T (+ bias) from split8's codes and scale words;
+// with `fin`, the slabs of a split reduction are left to it
 static void gemm8_run(const uint8_t* a, const uint8_t* as, int64_t M, const uint8_t* b, const uint8_t* bs, int64_t N, int64_t K,
-                      const Tensor& out, bool beta, const float* bias) {
+                      const Tensor& out, bool beta, const float* bias, Finish8* fin = nullptr) {
   const bool out_bf16 = out.scalar_type() == torch::kBFloat16;
   const int es = out_bf16 ? 2 : 4;
   // a tile's rows of codes and an operand's scale words lie within one buffer descriptor each
@@ -879,8 +885,12 @@ static void gemm8_run(const uint8_t* a, const uint8_t* as, int64_t M, const uint
     p.beta = 0;
     p.vec = N % 4 == 0 && 1024 * N < (1LL << 31);
     TORCH_CHECK(hx_gemm_fp8(p, cfg, out_bf16 ? 0 : 1, 0, stream) == 0, "gemm_fp8: split-K launch failed");
-    hx_gemm_fp8_slabs(part.data_ptr<float>(), g.C, out_bf16, g.ldc, g.M, g.N, g.ks, g.bias, g.beta,
-                      N % 4 == 0 && aligned16(g.C) && g.ldc % 4 == 0 && (!out_bf16 || g.ldc % 8 == 0), stream);
+    Finish8 own;
+    Finish8& f = fin ? *fin : own;
+    f.f.slabs[f.f.n] = HxSlabs{part.data_ptr<float>(), g.C, g.ldc, g.bias, g.M, g.N, g.ks, g.beta,
+                               N % 4 == 0 && aligned16(g.C) && g.ldc % 4 == 0, out_bf16};
+    f.part[f.f.n++] = part;
+    if (!fin) hx_fp8_finish(f.f, stream);
   } else {
     TORCH_CHECK(hx_gemm_fp8(g, cfg, out_bf16 ? 0 : 1, out_bf16 ? 1 : 0, stream) == 0, "gemm_fp8: launch failed");
   }
@@ -1085,17 +1095,24 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
       uint8_t *pd = tmp.data_ptr<uint8_t>(), *pt = pd + cd.bytes(), *pp = pt + cdt.bytes();
       const HxSplit8 job = split8_job(dy, cd.q(pd), cd.s(pd), cdt.q(pt), cdt.s(pt), need_b ? reinterpret_cast<float*>(pp) : nullptr);
       hx_split8(&job, 1, cur_stream(dy));
-      if (need_b) hx_fold_cols(reinterpret_cast<float*>(pp), hx_split8_row_tiles(M), (int)N, db.data_ptr<float>(), 0, cur_stream(dy));
+      Finish8 fin;
+      if (need_b) {
+        fin.f.part = reinterpret_cast<float*>(pp);
+        fin.f.sum = db.data_ptr<float>();
+        fin.f.rows = hx_split8_row_tiles(M);
+        fin.f.cols = (int)N;
+      }
       if (need_w) {
         uint8_t* pk = saved[0].data_ptr<uint8_t>();
-        gemm8_run(cdt.q(pt), cdt.s(pt), N, cxt.q(pk), cxt.s(pk), K, M, dW, false, nullptr);
-        dbg_finite(dW, "linear_fp8 weight gradient");
+        gemm8_run(cdt.q(pt), cdt.s(pt), N, cxt.q(pk), cxt.s(pk), K, M, dW, false, nullptr, &fin);
       }
       if (need_x) {
         TORCH_CHECK(saved[1].defined(), "linear_fp8: the weight's codes were made without those of its transpose");
-        gemm8_run(cd.q(pd), cd.s(pd), M, saved[1].data_ptr<uint8_t>(), saved[2].data_ptr<uint8_t>(), K, N, dx, false, nullptr);
-        dbg_finite(dx, "linear_fp8 input gradient");
+        gemm8_run(cd.q(pd), cd.s(pd), M, saved[1].data_ptr<uint8_t>(), saved[2].data_ptr<uint8_t>(), K, N, dx, false, nullptr, &fin);
       }
+      hx_fp8_finish(fin.f, cur_stream(dy));
+      if (need_w) dbg_finite(dW, "linear_fp8 weight gradient");
+      if (need_x) dbg_finite(dx, "linear_fp8 input gradient");
     }
     if (need_x) dx = dx.view(xshape);
     if (need_w && ctx->saved_data["wbf16"].toBool()) dW = dW.to(torch::kBFloat16);

@@ -286,8 +286,22 @@ struct HxGemm8 {
 };
 void hx_gemm_fp8_plan(int M, int N, int nkb, int exact, int* cfg, int* ks);   // tile configuration, split-K slabs
 int hx_gemm_fp8(const HxGemm8& g, int cfg, int exact, int out_bf16, hipStream_t s);
-void hx_gemm_fp8_slabs(const float* part, void* out, int out_bf16, int64_t ldc, int M, int N, int ks, const float* bias,
-                       int beta, int vec, hipStream_t s);
+// slabs [ks][M][N] of a split reduction -> out (+ bias) (+ out); vec: N, ldc and out allow 4 elements at a time
+struct HxSlabs {
+  const float* part;
+  void* out;
+  int64_t ldc;
+  const float* bias;
+  int M, N, ks, beta, vec, bf16;
+};
+// in one launch: n (<= 2) slab sums, and sum[cols] = the sum of part's [rows][cols] (sum null: none)
+struct HxFinish {
+  HxSlabs slabs[2];
+  const float* part;
+  float* sum;
+  int n, rows, cols, end[2];
+};
+void hx_fp8_finish(HxFinish f, hipStream_t s);
 // y [M, N] (x's type, contiguous) = Q(x) B^T (+ bias) for few rows (hx_fp8_rows_fit) of fp32 or bf16 x
 // (row stride ldx), B as in HxGemm8
 struct HxRows8 {
