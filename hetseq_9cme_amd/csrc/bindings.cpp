@@ -3,6 +3,7 @@
 // stream of the tensor's device (so kernels order correctly with hipBLASLt GEMMs
 // and RCCL, and are capturable into HIP graphs).
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/extension.h>
@@ -842,21 +843,35 @@ std::vector<std::vector<Tensor>> split8_weights(std::vector<Tensor> Ws) {
   return out;
 }
 
-// what a layer's products leave to add up, and the memory it is in
-struct Finish8 {
-  HxFinish f{};
-  Tensor part[2];
+// memory for the call alone, without a tensor around it (0.5 us instead of 1.3): returned to the stream's
+// allocator when it goes out of scope, as a tensor's would be
+struct Scratch8 {
+  c10::DataPtr p;
+  explicit Scratch8(int64_t bytes) { if (bytes) p = c10::hip::HIPCachingAllocator::get()->allocate((size_t)bytes); }
+  uint8_t* get() const { return static_cast<uint8_t*>(p.get()); }
+};
+inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// the tile, the split and the bytes of slabs of a product [M, N] over K
+struct Plan8 {
+  int cfg = 0, ks = 1;
+  int64_t bytes = 0;
+  Plan8() = default;
+  Plan8(int64_t M, int64_t N, int64_t K, bool out_bf16) {
+    // a tile's rows of codes and an operand's scale words lie within one buffer descriptor each
+    const int64_t groups = (blocks128(K) + 3) / 4, most = 1LL << 31;
+    TORCH_CHECK(K <= (1LL << 22) && std::max(M, N) < most - 256 && (std::max(M, N) + 3) / 4 * groups * 16 < most,
+                "gemm_fp8: at most 2^22 deep, fewer than 2^31 rows and bytes of scale words (rows / 4 x depth / 512 x 16)");
+    hx_gemm_fp8_plan((int)M, (int)N, (int)blocks128(K), out_bf16 ? 0 : 1, &cfg, &ks);
+    bytes = ks > 1 ? up256(ks * M * N * 4) : 0;
+  }
 };
 // out [M, N] (fp32 or bf16, unit column stride) (+)= A . B^T (+ bias) from split8's codes and scale words;
-// with `fin`, the slabs of a split reduction are left to it
-static void gemm8_run(const uint8_t* a, const uint8_t* as, int64_t M, const uint8_t* b, const uint8_t* bs, int64_t N, int64_t K,
-                      const Tensor& out, bool beta, const float* bias, Finish8* fin = nullptr) {
+// slabs: the plan's bytes; with `fin`, the sum over a split reduction's slabs is left to it
+static void gemm8_run(const Plan8& plan, uint8_t* slabs, const uint8_t* a, const uint8_t* as, int64_t M, const uint8_t* b, const uint8_t* bs,
+                      int64_t N, int64_t K, const Tensor& out, bool beta, const float* bias, HxFinish* fin = nullptr) {
   const bool out_bf16 = out.scalar_type() == torch::kBFloat16;
   const int es = out_bf16 ? 2 : 4;
-  // a tile's rows of codes and an operand's scale words lie within one buffer descriptor each
-  const int64_t groups = (blocks128(K) + 3) / 4, most = 1LL << 31;
-  TORCH_CHECK(K <= (1LL << 22) && std::max(M, N) < most - 256 && (std::max(M, N) + 3) / 4 * groups * 16 < most,
-              "gemm_fp8: at most 2^22 deep, fewer than 2^31 rows and bytes of scale words (rows / 4 x depth / 512 x 16)");
   HxGemm8 g{};
   g.A = a;
   g.sa = reinterpret_cast<const uint32_t*>(as);
@@ -870,27 +885,25 @@ static void gemm8_run(const uint8_t* a, const uint8_t* as, int64_t M, const uint
   g.N = (int)N;
   g.nkb = (int)blocks128(K);
   g.beta = beta ? 1 : 0;
-  int cfg = 0;
-  hx_gemm_fp8_plan(g.M, g.N, g.nkb, out_bf16 ? 0 : 1, &cfg, &g.ks);
+  g.ks = plan.ks;
+  const int cfg = plan.cfg;
   // 16-B stores, and a tile's 256 rows within one buffer descriptor
   g.vec = aligned16(g.C) && g.ldc * es % 16 == 0 && N * es % 16 == 0 && 256 * g.ldc * es < (1LL << 31);
   const hipStream_t stream = cur_stream(out);
   if (g.ks > 1) {
-    Tensor part = torch::empty({g.ks, M, N}, out.options().dtype(torch::kFloat32));
+    float* part = reinterpret_cast<float*>(slabs);
     HxGemm8 p = g;
-    p.C = part.data_ptr();
+    p.C = part;
     p.ldc = N;
     p.c_zs = M * N;
     p.bias = nullptr;
     p.beta = 0;
     p.vec = N % 4 == 0 && 1024 * N < (1LL << 31);
     TORCH_CHECK(hx_gemm_fp8(p, cfg, out_bf16 ? 0 : 1, 0, stream) == 0, "gemm_fp8: split-K launch failed");
-    Finish8 own;
-    Finish8& f = fin ? *fin : own;
-    f.f.slabs[f.f.n] = HxSlabs{part.data_ptr<float>(), g.C, g.ldc, g.bias, g.M, g.N, g.ks, g.beta,
-                               N % 4 == 0 && aligned16(g.C) && g.ldc % 4 == 0, out_bf16};
-    f.part[f.f.n++] = part;
-    if (!fin) hx_fp8_finish(f.f, stream);
+    HxFinish own{};
+    HxFinish& f = fin ? *fin : own;
+    f.slabs[f.n++] = HxSlabs{part, g.C, g.ldc, g.bias, g.M, g.N, g.ks, g.beta, N % 4 == 0 && aligned16(g.C) && g.ldc % 4 == 0, out_bf16};
+    if (!fin) hx_fp8_finish(f, stream);
   } else {
     TORCH_CHECK(hx_gemm_fp8(g, cfg, out_bf16 ? 0 : 1, out_bf16 ? 1 : 0, stream) == 0, "gemm_fp8: launch failed");
   }
@@ -919,7 +932,9 @@ Tensor gemm_fp8(Tensor a, Tensor as, Tensor b, Tensor bs, int64_t K, bool out_bf
                   (out.stride(1) == 1 || N == 1) && (M <= 1 || out.stride(0) >= N),
               "gemm_fp8: out must be [M, N] of the result type with unit column stride");
   if (M == 0 || N == 0) return out;
-  gemm8_run(a.data_ptr<uint8_t>(), as.data_ptr<uint8_t>(), M, b.data_ptr<uint8_t>(), bs.data_ptr<uint8_t>(), N, K, out, beta,
+  const Plan8 plan(M, N, K, out_bf16);
+  const Scratch8 slabs(plan.bytes);
+  gemm8_run(plan, slabs.get(), a.data_ptr<uint8_t>(), as.data_ptr<uint8_t>(), M, b.data_ptr<uint8_t>(), bs.data_ptr<uint8_t>(), N, K, out, beta,
             ptr_or_null<float>(bias));
   dbg_finite(out, "gemm_fp8");
   return out;
@@ -974,7 +989,6 @@ std::vector<OptT> linear_fp8_fwd(Tensor x2, Tensor wq, Tensor ws, OptT bias, boo
 }
 
 // codes and scale words of an operand [rows, n] inside a workspace
-inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 struct Codes8 {
   int64_t rows, n, qb, sb;   // bytes of the codes and of the scale words, 256-B steps
   Codes8(int64_t rows_, int64_t n_, bool on = true)
@@ -1036,7 +1050,8 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
       c10::hip::HIPGuardMasqueradingAsCUDA guard(x2.device());
       const auto u8 = x2.options().dtype(torch::kUInt8);
       const Codes8 cx(M, K), cxt(K, M, keep), cw(N, K, own);
-      Tensor tmp = torch::empty({cx.bytes() + cw.bytes()}, u8);
+      const Plan8 plan = M > 0 ? Plan8(M, N, K, x2.scalar_type() == torch::kBFloat16) : Plan8();
+      const Scratch8 tmp(cx.bytes() + cw.bytes() + plan.bytes);
       if (keep && M > 0) kept = torch::empty({cxt.bytes()}, u8);
       if (own && wt) {
         // of the shapes that an Fp8Weight has: a checkpointed segment may run with one and be recomputed
@@ -1044,7 +1059,7 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
         wtq = torch::empty({K, blocks128(N) * 128}, u8);
         wts = scale_words(K, N, x2);
       }
-      uint8_t *px = tmp.data_ptr<uint8_t>(), *pw = px + cx.bytes();
+      uint8_t *px = tmp.get(), *pw = px + cx.bytes(), *slabs = pw + cw.bytes();
       uint8_t* pk = kept.defined() ? kept.data_ptr<uint8_t>() : nullptr;
       uint8_t* pt = own && wt ? wtq.data_ptr<uint8_t>() : nullptr;
       HxSplit8 jobs[2];
@@ -1057,27 +1072,27 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
         if (!own)
           TORCH_CHECK(wq->is_cuda() && wq->device() == x2.device() && wq->size(1) == blocks128(K) * 128 && wq->is_contiguous(),
                       "linear_fp8: the weight's codes do not fit x");
-        gemm8_run(cx.q(px), cx.s(px), M, own ? cw.q(pw) : wq->data_ptr<uint8_t>(), own ? cw.s(pw) : ws->data_ptr<uint8_t>(), N, K, y,
+        gemm8_run(plan, slabs, cx.q(px), cx.s(px), M, own ? cw.q(pw) : wq->data_ptr<uint8_t>(), own ? cw.s(pw) : ws->data_ptr<uint8_t>(), N, K, y,
                   false, ptr_or_null<float>(bias));
         dbg_finite(y, "linear_fp8");
       }
     }
     ctx->save_for_backward({kept, wtq, wts});
-    ctx->saved_data["xshape"] = x.sizes().vec();
-    ctx->saved_data["N"] = N;
-    ctx->saved_data["wbf16"] = has(W) && W->scalar_type() == torch::kBFloat16;
-    // the inputs that are there have the first edges, in order
-    ctx->saved_data["ew"] = has(W) ? 1 : 0;
-    ctx->saved_data["eb"] = has(b) ? (has(W) ? 2 : 1) : 0;
+    // in one list: N, whether W is bf16, the edges of W and b (the inputs that are there have the first
+    // edges, in order), then x's shape
+    std::vector<int64_t> kept_ints{N, has(W) && W->scalar_type() == torch::kBFloat16, has(W) ? 1 : 0, has(b) ? (has(W) ? 2 : 1) : 0};
+    kept_ints.insert(kept_ints.end(), x.sizes().begin(), x.sizes().end());
+    ctx->saved_data["ints"] = std::move(kept_ints);
+    if (x.dim() == 2) return y;
     return y.view(shape);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
     refuse_second_derivative("linear_fp8");
     refuse_stale_leaves(g[0], "linear_fp8");
     const auto saved = ctx->get_saved_variables();
-    const auto xshape = ctx->saved_data["xshape"].toIntVector();
-    const int64_t N = ctx->saved_data["N"].toInt(), K = xshape.back();
-    const int64_t ew = ctx->saved_data["ew"].toInt(), eb = ctx->saved_data["eb"].toInt();
+    const auto ints = ctx->saved_data["ints"].toIntVector();
+    const int64_t N = ints[0], K = ints.back(), ew = ints[2], eb = ints[3];
+    const c10::IntArrayRef xshape = c10::IntArrayRef(ints).slice(4);
     const bool need_x = ctx->needs_input_grad(0), need_w = ew && ctx->needs_input_grad(ew), need_b = eb && ctx->needs_input_grad(eb);
     Tensor dy = as_rows8(g[0]);
     check_rows8(dy, "linear_fp8 output gradient");
@@ -1091,31 +1106,33 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
     if (M > 0) {
       const Codes8 cd(M, N, need_x), cdt(N, M, need_w), cxt(K, M, need_w);
       const int64_t part = need_b ? up256(hx_split8_row_tiles(M) * N * 4) : 0;
-      Tensor tmp = torch::empty({cd.bytes() + cdt.bytes() + part}, dy.options().dtype(torch::kUInt8));
-      uint8_t *pd = tmp.data_ptr<uint8_t>(), *pt = pd + cd.bytes(), *pp = pt + cdt.bytes();
+      const Plan8 px = need_x ? Plan8(M, K, N, dy.scalar_type() == torch::kBFloat16) : Plan8();
+      const Plan8 pw = need_w ? Plan8(N, K, M, false) : Plan8();
+      const Scratch8 tmp(cd.bytes() + cdt.bytes() + part + pw.bytes + px.bytes);
+      uint8_t *pd = tmp.get(), *pt = pd + cd.bytes(), *pp = pt + cdt.bytes(), *slabs = pp + part;
       const HxSplit8 job = split8_job(dy, cd.q(pd), cd.s(pd), cdt.q(pt), cdt.s(pt), need_b ? reinterpret_cast<float*>(pp) : nullptr);
       hx_split8(&job, 1, cur_stream(dy));
-      Finish8 fin;
+      HxFinish fin{};
       if (need_b) {
-        fin.f.part = reinterpret_cast<float*>(pp);
-        fin.f.sum = db.data_ptr<float>();
-        fin.f.rows = hx_split8_row_tiles(M);
-        fin.f.cols = (int)N;
+        fin.part = reinterpret_cast<float*>(pp);
+        fin.sum = db.data_ptr<float>();
+        fin.rows = hx_split8_row_tiles(M);
+        fin.cols = (int)N;
       }
       if (need_w) {
         uint8_t* pk = saved[0].data_ptr<uint8_t>();
-        gemm8_run(cdt.q(pt), cdt.s(pt), N, cxt.q(pk), cxt.s(pk), K, M, dW, false, nullptr, &fin);
+        gemm8_run(pw, slabs, cdt.q(pt), cdt.s(pt), N, cxt.q(pk), cxt.s(pk), K, M, dW, false, nullptr, &fin);
       }
       if (need_x) {
         TORCH_CHECK(saved[1].defined(), "linear_fp8: the weight's codes were made without those of its transpose");
-        gemm8_run(cd.q(pd), cd.s(pd), M, saved[1].data_ptr<uint8_t>(), saved[2].data_ptr<uint8_t>(), K, N, dx, false, nullptr, &fin);
+        gemm8_run(px, slabs + pw.bytes, cd.q(pd), cd.s(pd), M, saved[1].data_ptr<uint8_t>(), saved[2].data_ptr<uint8_t>(), K, N, dx, false, nullptr, &fin);
       }
-      hx_fp8_finish(fin.f, cur_stream(dy));
+      hx_fp8_finish(fin, cur_stream(dy));
       if (need_w) dbg_finite(dW, "linear_fp8 weight gradient");
       if (need_x) dbg_finite(dx, "linear_fp8 input gradient");
     }
-    if (need_x) dx = dx.view(xshape);
-    if (need_w && ctx->saved_data["wbf16"].toBool()) dW = dW.to(torch::kBFloat16);
+    if (need_x && xshape.size() != 2) dx = dx.view(xshape);
+    if (need_w && ints[1]) dW = dW.to(torch::kBFloat16);
     return {dx, dW, db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
