@@ -798,13 +798,14 @@ std::vector<OptT> split8(Tensor x, bool by_rows, bool by_cols, bool want_sum, Op
     check_f32(*sum, "split8 column sums");
     TORCH_CHECK(sum->numel() == C && sum->device() == x.device(), "split8: column sums [C]");
     if (R == 0) sum->zero_();
-    else part = torch::empty({hx_split8_row_tiles(R), C}, f32);
+    else part = hx_split8_row_tiles(R) == 1 ? *sum : torch::empty({hx_split8_row_tiles(R), C}, f32);   // one tile's sums are the sums
   }
   if (R > 0 && (by_rows || by_cols || want_sum)) {
     const HxSplit8 job = split8_job(x, ptr_or_null<uint8_t>(q), ptr_or_null<uint8_t>(s), ptr_or_null<uint8_t>(qt),
                                     ptr_or_null<uint8_t>(st), want_sum ? part.data_ptr<float>() : nullptr);
     hx_split8(&job, 1, cur_stream(x));
-    if (want_sum) hx_fold_cols(part.data_ptr<float>(), hx_split8_row_tiles(R), (int)C, sum->data_ptr<float>(), 0, cur_stream(x));
+    if (want_sum && hx_split8_row_tiles(R) > 1)
+      hx_fold_cols(part.data_ptr<float>(), hx_split8_row_tiles(R), (int)C, sum->data_ptr<float>(), 0, cur_stream(x));
   }
   return {q, s, qt, st, sum};
 }
@@ -976,7 +977,7 @@ static Tensor linear_fp8_y(const Tensor& x2, const Tensor& wq, const Tensor& ws,
 }
 // [.., K] -> [rows, K] with unit column stride (a contiguous copy if it has none)
 static Tensor as_rows8(const Tensor& x) {
-  Tensor x2 = x.reshape({-1, x.size(-1)});
+  Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
   const bool ok = (x2.stride(1) == 1 || x2.size(1) == 1) && (x2.stride(0) >= x2.size(1) || x2.size(0) <= 1);
   return ok ? x2 : x2.contiguous();
 }
@@ -1027,10 +1028,10 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
                         bool grad) {
     const bool own = !has(wq);   // W's codes are made here
     const int64_t K = x.size(-1), N = own ? W->size(0) : wq->size(0);
-    Tensor x2 = as_rows8(x.detach());
+    Tensor x2 = as_rows8(x);
     const int64_t M = x2.size(0);
     const bool keep = grad && has(W) && W->requires_grad(), wt = grad && x.requires_grad();
-    OptT bias = has(b) ? OptT(b->detach()) : OptT();
+    const OptT& bias = b;   // (no gradient is recorded here: apply() turns it off)
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = N;
     Tensor y, kept, wtq, wts;   // what the backward needs: x's codes; the codes of W^T and their scales
@@ -1043,7 +1044,7 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
     } else {
       check_rows8(x2, "linear_fp8");
       check_bias8(bias, N, x2, "linear_fp8 bias");
-      Tensor W2 = own ? as_rows8(W->detach()) : Tensor();
+      Tensor W2 = own ? as_rows8(*W) : Tensor();
       if (own) check_rows8(W2, "linear_fp8 weight");
       TORCH_CHECK(!keep || M <= (1LL << 22), "linear_fp8: at most 2^22 rows in a training step");
       TORCH_CHECK(!own || N <= (1LL << 22), "linear_fp8: at most 2^22 output features");
@@ -1105,15 +1106,17 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
     if (need_b) db = M > 0 ? torch::empty({N}, f32) : torch::zeros({N}, f32);
     if (M > 0) {
       const Codes8 cd(M, N, need_x), cdt(N, M, need_w), cxt(K, M, need_w);
-      const int64_t part = need_b ? up256(hx_split8_row_tiles(M) * N * 4) : 0;
+      const bool fold = need_b && hx_split8_row_tiles(M) > 1;   // (one tile's column sums are the sums)
+      const int64_t part = fold ? up256(hx_split8_row_tiles(M) * N * 4) : 0;
       const Plan8 px = need_x ? Plan8(M, K, N, dy.scalar_type() == torch::kBFloat16) : Plan8();
       const Plan8 pw = need_w ? Plan8(N, K, M, false) : Plan8();
       const Scratch8 tmp(cd.bytes() + cdt.bytes() + part + pw.bytes + px.bytes);
       uint8_t *pd = tmp.get(), *pt = pd + cd.bytes(), *pp = pt + cdt.bytes(), *slabs = pp + part;
-      const HxSplit8 job = split8_job(dy, cd.q(pd), cd.s(pd), cdt.q(pt), cdt.s(pt), need_b ? reinterpret_cast<float*>(pp) : nullptr);
+      const HxSplit8 job = split8_job(dy, cd.q(pd), cd.s(pd), cdt.q(pt), cdt.s(pt),
+                                      fold ? reinterpret_cast<float*>(pp) : need_b ? db.data_ptr<float>() : nullptr);
       hx_split8(&job, 1, cur_stream(dy));
       HxFinish fin{};
-      if (need_b) {
+      if (fold) {
         fin.part = reinterpret_cast<float*>(pp);
         fin.sum = db.data_ptr<float>();
         fin.rows = hx_split8_row_tiles(M);
@@ -1188,17 +1191,18 @@ std::vector<OptT> gelu8_bwd(Tensor dout, Tensor q, Tensor s, OptT b, bool want_d
   check_bias8(b, N, dout, "gelu8_bwd bias");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(dout.device());
   auto f32 = dout.options().dtype(torch::kFloat32);
-  Tensor dy = torch::empty_like(dout), part;
+  Tensor dy = torch::empty_like(dout);
+  const int chunks = want_db ? hx_gelu8_chunks(rows) : 0;
+  const Scratch8 part(chunks > 1 ? chunks * N * 4 : 0);   // (one chunk's sums are the sums)
   OptT db;
   if (want_db) {
     db = has(db_out) ? *db_out : torch::empty({N}, f32);
     check_bias8(db, N, dout, "gelu8_bwd bias gradient");
     if (rows == 0) db->zero_();
-    else part = torch::empty({hx_gelu8_chunks(rows), N}, f32);
   }
   if (rows > 0)
     hx_gelu8_bwd(act_bf16(dout), dout.data_ptr(), q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), ptr_or_null<float>(b),
-                 dy.data_ptr(), want_db ? part.data_ptr<float>() : nullptr, ptr_or_null<float>(db), rows, (int)N,
+                 dy.data_ptr(), chunks > 1 ? reinterpret_cast<float*>(part.get()) : ptr_or_null<float>(db), ptr_or_null<float>(db), rows, (int)N,
                  cur_stream(dout));
   dbg_finite(dy, "gelu8_bwd");
   return {dy, db};
@@ -1207,8 +1211,8 @@ std::vector<OptT> gelu8_bwd(Tensor dout, Tensor q, Tensor s, OptT b, bool want_d
 // bias + GELU as one autograd node (see LinearFp8)
 struct BiasGelu8 : public torch::autograd::Function<BiasGelu8> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor y, OptT b) {
-    std::vector<Tensor> r = gelu8_fwd(y.detach(), has(b) ? OptT(b->detach()) : OptT());
-    ctx->save_for_backward({r[1], r[2], has(b) ? b->detach() : Tensor()});
+    std::vector<Tensor> r = gelu8_fwd(y, b);
+    ctx->save_for_backward({r[1], r[2], has(b) ? *b : Tensor()});
     return r[0];
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {

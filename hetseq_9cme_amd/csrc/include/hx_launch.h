@@ -264,7 +264,7 @@ void hx_split8_many(const HxSplit8Batch& d, hipStream_t stream);
 // int8 blocks along contiguous rows of N: codes [rows][nb][128], scale bytes [rows][nb], nb = ceil(N / 128)
 void hx_gelu8_fwd(int bf16, const void* y, const float* b, void* out, uint8_t* q, uint8_t* s, int64_t rows, int N,
                   hipStream_t stream);
-int hx_gelu8_chunks(int64_t rows);
+int hx_gelu8_chunks(int64_t rows);   // rows of partial [chunks][N]; of one chunk it is db itself; null, as db: no sums
 void hx_gelu8_bwd(int bf16, const void* dout, const uint8_t* q, const uint8_t* s, const float* b, void* dy,
                   float* partial, float* db, int64_t rows, int N, hipStream_t stream);
 void hx_pack8(int bf16, const void* x, uint8_t* q, uint8_t* s, int64_t rows, int N, hipStream_t stream);

@@ -419,7 +419,7 @@ void hx_gelu8_bwd(int bf16, const void* dout, const uint8_t* q, const uint8_t* s
   const unsigned grid = (unsigned)(nb * (int64_t)hx_gelu8_chunks(rows));
   if (bf16) gelu8_bwd_k<uint16_t><<<grid, NT, 0, stream>>>((const uint16_t*)dout, q, s, b, (uint16_t*)dy, partial, rows, nb, N);
   else gelu8_bwd_k<float><<<grid, NT, 0, stream>>>((const float*)dout, q, s, b, (float*)dy, partial, rows, nb, N);
-  if (partial) fold_rows(partial, hx_gelu8_chunks(rows), N, N, N, db, nullptr, nullptr, 0, stream);
+  if (partial != db) fold_rows(partial, hx_gelu8_chunks(rows), N, N, N, db, nullptr, nullptr, 0, stream);
 }
 
 void hx_pack8(int bf16, const void* x, uint8_t* q, uint8_t* s, int64_t rows, int N, hipStream_t stream) {
