@@ -1139,19 +1139,31 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
     return {dx, dW, db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
+// Inference with a kept weight's codes (of K input features), arguments checked here: a single token's call
+// is bound by the host
+Tensor linear_fp8_infer(Tensor x, Tensor wq, Tensor ws, int64_t K, OptT b) {
+  TORCH_CHECK_TYPE(x.scalar_type() == torch::kFloat32 || x.scalar_type() == torch::kBFloat16, "linear_fp8: an fp32 or bf16 tensor, got ",
+                   x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == K, "linear_fp8: x of shape ", x.sizes(), ", the weight takes ", K, " features");
+  TORCH_CHECK_VALUE(x.device() == wq.device(), "linear_fp8: x on ", x.device(), ", the weight on ", wq.device());
+  if (has(b))
+    TORCH_CHECK_VALUE(b->scalar_type() == torch::kFloat32 && b->dim() == 1 && b->size(0) == wq.size(0) && b->device() == x.device(),
+                      "linear_fp8: the bias must be fp32 [", wq.size(0), "] on ", x.device(), ", got ", b->scalar_type(), " ", b->sizes(),
+                      " on ", b->device());
+  at::NoGradGuard no_grad;
+  if (x.dim() == 2 && x.is_contiguous()) return linear_fp8_y(x, wq, ws, b, false, nullptr, nullptr);
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = wq.size(0);
+  return linear_fp8_y(as_rows8(x), wq, ws, b, false, nullptr, nullptr).view(shape);
+}
+
 // W: the parameter whose gradient is wanted (or none); w8: its codes and scales (wq, ws, wqt, wst -- the
 // last two may be absent), or empty: they are made from W
 Tensor linear_fp8(Tensor x, OptT W, OptT b, std::vector<OptT> w8, bool grad) {
   TORCH_CHECK(w8.empty() ? has(W) : w8.size() == 4 && has(w8[0]) && has(w8[1]), "linear_fp8: a weight or its codes and scales");
   if (w8.empty()) return LinearFp8::apply(x, W, b, OptT(), OptT(), OptT(), OptT(), grad);
   const bool wanted = grad && (x.requires_grad() || (has(W) && W->requires_grad()) || (has(b) && b->requires_grad()));
-  if (!wanted) {   // inference: no node
-    at::NoGradGuard no_grad;
-    if (x.dim() == 2 && x.is_contiguous()) return linear_fp8_y(x, *w8[0], *w8[1], b, false, nullptr, nullptr);
-    std::vector<int64_t> shape = x.sizes().vec();
-    shape.back() = w8[0]->size(0);
-    return linear_fp8_y(as_rows8(x), *w8[0], *w8[1], b, false, nullptr, nullptr).view(shape);
-  }
+  if (!wanted) return linear_fp8_infer(x, *w8[0], *w8[1], x.size(-1), b);   // no node
   return LinearFp8::apply(x, W, b, w8[0], w8[1], w8[2], w8[3], grad);
 }
 
@@ -1227,6 +1239,8 @@ struct BiasGelu8 : public torch::autograd::Function<BiasGelu8> {
 Tensor bias_gelu8(Tensor y, OptT b) { return BiasGelu8::apply(y.contiguous(), b); }
 
 std::vector<Tensor> pack8(Tensor x) {
+  at::NoGradGuard no_grad;
+  if (!x.is_contiguous()) x = x.contiguous();
   const auto [rows, N] = rows_cols8(x, "pack8 x");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
   Tensor q = torch::empty({rows, blocks128(N), 128}, x.options().dtype(torch::kUInt8));
@@ -1236,12 +1250,17 @@ std::vector<Tensor> pack8(Tensor x) {
   return {q, s};
 }
 
-Tensor unpack8(Tensor q, Tensor s, int64_t N, bool bf16) {
-  TORCH_CHECK(q.dim() == 3 && N >= 1 && N < (1LL << 30) && q.size(1) == blocks128(N) && q.size(2) == 128, "unpack8: codes [rows, ceil(N / 128), 128]");
+// codes [rows, nb, 128] and scale bytes -> their values, a tensor of `shape`
+Tensor unpack8(Tensor q, Tensor s, std::vector<int64_t> shape, bool bf16) {
+  TORCH_CHECK(!shape.empty(), "unpack8: a shape of at least one dimension");
+  const int64_t N = shape.back();
+  TORCH_CHECK(q.dim() == 3 && N >= 1 && N < (1LL << 30) && q.size(1) == blocks128(N) && q.size(2) == 128,
+              "unpack8: codes [rows, ceil(N / 128), 128]");
   const int64_t rows = q.size(0);
   check_kept(q, s, q, rows, N, "unpack8");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
-  Tensor x = torch::empty({rows, N}, q.options().dtype(bf16 ? torch::kBFloat16 : torch::kFloat32));
+  Tensor x = torch::empty(shape, q.options().dtype(bf16 ? torch::kBFloat16 : torch::kFloat32));
+  TORCH_CHECK(x.numel() == rows * N, "unpack8: codes of ", rows, " rows for another shape");
   if (rows > 0)
     hx_unpack8(bf16, q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), x.data_ptr(), rows, (int)N, cur_stream(q));
   return x;
@@ -1623,6 +1642,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("out") = py::none(), py::arg("beta") = false, py::arg("bias") = py::none());
   m.def("linear_fp8_fwd", &linear_fp8_fwd, py::arg("x"), py::arg("wq"), py::arg("ws"), py::arg("bias"), py::arg("keep"));
   m.def("linear_fp8", &linear_fp8, py::arg("x"), py::arg("W"), py::arg("bias"), py::arg("w8"), py::arg("grad"));
+  m.def("linear_fp8_infer", &linear_fp8_infer, py::arg("x"), py::arg("wq"), py::arg("ws"), py::arg("K"), py::arg("bias"));
   m.def("bias_gelu8", &bias_gelu8, py::arg("y"), py::arg("bias"));
   m.def("gelu8_fwd", &gelu8_fwd);
   m.def("gelu8_bwd", &gelu8_bwd, py::arg("dout"), py::arg("q"), py::arg("s"), py::arg("bias"), py::arg("want_db"),

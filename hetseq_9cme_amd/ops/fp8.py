@@ -118,6 +118,10 @@ class Fp8Weight(object):
         return w
 
     @property
+    def is_cuda(self):
+        return self.device.type == 'cuda'
+
+    @property
     def has_grad(self):
         return self.qt is not None or (self.ref is not None and self.ref[1] is not None)
 
@@ -146,6 +150,8 @@ def _check_codes(codes, shape, device, need_grad, what):
     if codes.shape != shape or codes.device != device:
         raise ValueError('{}: codes of a {} weight on {}, the weight is {} on {}'.format(
             what, codes.shape, codes.device, shape, device))
+    if (codes.ref is None) != use_kernels(codes):
+        raise ValueError('{}: the Fp8Weight was built with the GPU kernels switched {}'.format(what, 'on' if codes.ref is None else 'off'))
     if need_grad and not codes.has_grad:
         raise ValueError('{}: x needs a gradient, the Fp8Weight was built with grad=False'.format(what))
 
@@ -265,8 +271,10 @@ def linear_fp8(x, W, b=None, res_grad=None, codes=None):
     ``codes``: the parameter's ``Fp8Weight``, where the caller has made it for this forward
     (``fp8_weights``).  ``res_grad``: see ``ResidualGrad``.  First derivatives only; at most 2^22
     features in or out, and in a training step 2^22 rows."""
-    _check_act(x, 'linear_fp8')
     kept = isinstance(W, Fp8Weight)
+    if kept and codes is None and torch.is_tensor(x) and use_kernels(x) and W.q is not None and not torch.is_grad_enabled():
+        return C().linear_fp8_infer(x, W.q, W.s, W.shape[1], b)   # (checks its arguments as below)
+    _check_act(x, 'linear_fp8')
     if not kept:
         _check_weight(W, 'linear_fp8')
     N, K = W.shape
@@ -276,6 +284,8 @@ def linear_fp8(x, W, b=None, res_grad=None, codes=None):
         raise ValueError('linear_fp8: x on {}, the weight on {}'.format(x.device, W.device))
     _check_bias(b, N, x, 'linear_fp8')
     grad = torch.is_grad_enabled()
+    if kept and codes is not None:
+        raise ValueError('linear_fp8: codes go with a parameter; W is an Fp8Weight itself')
     w8 = W if kept else codes
     if w8 is not None:
         _check_codes(w8, (N, K), W.device, grad and x.requires_grad, 'linear_fp8')
@@ -366,11 +376,7 @@ class Packed8(object):
 def pack8(x):
     """``x`` (fp32 or bf16) as int8 blocks along its last dimension: 1 + 1/128 bytes per element."""
     _check_act(x, 'pack8')
-    x = x.detach()
-    if use_kernels(x):
-        q, s = C().pack8(x.contiguous())
-    else:
-        q, s = _pack8_ref(x)
+    q, s = C().pack8(x) if use_kernels(x) else _pack8_ref(x.detach())
     return Packed8(q, s, x.shape, x.dtype)
 
 
@@ -385,7 +391,7 @@ def unpack8(p):
     if not isinstance(p, Packed8):
         raise TypeError('unpack8: a Packed8 (ops.pack8), got {}'.format(type(p).__name__))
     if use_kernels(p.q):
-        return C().unpack8(p.q, p.s, p.shape[-1], p.dtype == torch.bfloat16).view(p.shape)
+        return C().unpack8(p.q, p.s, p.shape, p.dtype == torch.bfloat16)
     c = p.q.view(torch.int8).float()
     v = c * (p.s.to(torch.int32) << 23).view(torch.float32).unsqueeze(-1)
     v = torch.where(c == -128, torch.full_like(v, float('nan')), v)

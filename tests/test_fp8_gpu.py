@@ -556,3 +556,25 @@ def test_capture_is_refused_while_an_eager_graph_lives(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out[0], torch.autograd.grad(ops.linear_fp8(x, W), W, d)[0])
+
+
+def test_inference_refusals(dev):
+    """The one-call inference path refuses what the general one does."""
+    w8, x = ops.Fp8Weight(rand((64, 130), torch.float32, 1)), rand((3, 130), torch.bfloat16, 2)
+    with torch.no_grad():
+        assert ops.linear_fp8(x[0], w8).shape == (64,) and ops.linear_fp8(x.view(3, 1, 130), w8).shape == (3, 1, 64)
+        for bad, error in ((lambda: ops.linear_fp8(x.half(), w8), TypeError), (lambda: ops.linear_fp8(x[:, :128], w8), ValueError),
+                           (lambda: ops.linear_fp8(x.cpu(), w8), ValueError),
+                           (lambda: ops.linear_fp8(x, w8, torch.zeros(64, device=dev, dtype=torch.bfloat16)), ValueError),
+                           (lambda: ops.linear_fp8(x, w8, torch.zeros(65, device=dev)), ValueError),
+                           (lambda: ops.linear_fp8(x, w8, torch.zeros(64)), ValueError),
+                           (lambda: ops.linear_fp8(x, w8, codes=torch.zeros(3)), (TypeError, ValueError))):
+            with pytest.raises(error):
+                bad()
+        assert torch.equal(ops.linear_fp8(x[:0], w8), torch.zeros(0, 64, device=dev, dtype=torch.bfloat16))
+        ops.set_fused(False)
+        try:
+            with pytest.raises(ValueError, match='switched on'):
+                ops.linear_fp8(x, w8)
+        finally:
+            ops.set_fused(True)
