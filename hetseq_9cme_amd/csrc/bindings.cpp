@@ -1220,6 +1220,66 @@ std::vector<OptT> gelu8_bwd(Tensor dout, Tensor q, Tensor s, OptT b, bool want_d
   return {dy, db};
 }
 
+// gelu(y + b) of a feed-forward layer straight to the second product's operand: (q, s, qt, st) as split8 (qt, st
+// for by_cols), and y's int8 blocks (kept: codes, scale bytes)
+std::vector<OptT> gelu8_split_fwd(Tensor y, OptT b, bool by_cols, bool keep) {
+  check_rows8(y, "gelu8_split_fwd");
+  const int64_t R = y.size(0), C = y.size(1);
+  check_bias8(b, C, y, "gelu8_split_fwd bias");
+  TORCH_CHECK(!by_cols || R <= (1LL << 22), "gelu8_split_fwd: at most 2^22 rows blocked along the rows");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(y.device());
+  auto u8 = y.options().dtype(torch::kUInt8);
+  Tensor q = torch::empty({R, blocks128(C) * 128}, u8), s = scale_words(R, C, y);
+  OptT qt, st, kq, ks;
+  if (by_cols) {
+    qt = torch::empty({C, blocks128(R) * 128}, u8);
+    st = scale_words(C, R, y);
+  }
+  if (keep) {
+    kq = torch::empty({R, blocks128(C), 128}, u8);
+    ks = torch::empty({R, blocks128(C)}, u8);
+  }
+  if (R > 0)
+    hx_gelu8_split_fwd(split8_job(y, q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), ptr_or_null<uint8_t>(qt), ptr_or_null<uint8_t>(st), nullptr),
+                       ptr_or_null<float>(b), ptr_or_null<uint8_t>(kq), ptr_or_null<uint8_t>(ks), cur_stream(y));
+  return {q, s, qt, st, kq, ks};
+}
+
+// dout gelu'(y + b) straight to the operands of the first product's gradients: (q, s) by_rows, (qt, st) by_cols, and
+// the bias gradient
+std::vector<OptT> gelu8_split_bwd(Tensor dout, Tensor kq, Tensor ks, OptT b, bool by_rows, bool by_cols, bool want_db, OptT db_out) {
+  check_rows8(dout, "gelu8_split_bwd");
+  const int64_t R = dout.size(0), C = dout.size(1);
+  check_kept(kq, ks, dout, R, C, "gelu8_split_bwd");
+  check_bias8(b, C, dout, "gelu8_split_bwd bias");
+  TORCH_CHECK(!by_cols || R <= (1LL << 22), "gelu8_split_bwd: at most 2^22 rows blocked along the rows");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dout.device());
+  auto u8 = dout.options().dtype(torch::kUInt8);
+  OptT q, s, qt, st, db;
+  if (by_rows) {
+    q = torch::empty({R, blocks128(C) * 128}, u8);
+    s = scale_words(R, C, dout);
+  }
+  if (by_cols) {
+    qt = torch::empty({C, blocks128(R) * 128}, u8);
+    st = scale_words(C, R, dout);
+  }
+  const int tiles = want_db ? hx_split8_row_tiles(R) : 0;
+  const Scratch8 part(tiles > 1 ? tiles * C * 4 : 0);
+  if (want_db) {
+    db = has(db_out) ? *db_out : torch::empty({C}, dout.options().dtype(torch::kFloat32));
+    check_bias8(db, C, dout, "gelu8_split_bwd bias gradient");
+    if (R == 0) db->zero_();
+  }
+  if (R > 0 && (by_rows || by_cols || want_db)) {
+    float* sums = tiles > 1 ? reinterpret_cast<float*>(part.get()) : ptr_or_null<float>(db);
+    hx_gelu8_split_bwd(split8_job(dout, ptr_or_null<uint8_t>(q), ptr_or_null<uint8_t>(s), ptr_or_null<uint8_t>(qt), ptr_or_null<uint8_t>(st), sums),
+                       ptr_or_null<float>(b), kq.data_ptr<uint8_t>(), ks.data_ptr<uint8_t>(), cur_stream(dout));
+    if (tiles > 1) hx_fold_cols(sums, tiles, (int)C, db->data_ptr<float>(), 0, cur_stream(dout));
+  }
+  return {q, s, qt, st, db};
+}
+
 // bias + GELU as one autograd node (see LinearFp8)
 struct BiasGelu8 : public torch::autograd::Function<BiasGelu8> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor y, OptT b) {
@@ -1647,6 +1707,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gelu8_fwd", &gelu8_fwd);
   m.def("gelu8_bwd", &gelu8_bwd, py::arg("dout"), py::arg("q"), py::arg("s"), py::arg("bias"), py::arg("want_db"),
         py::arg("db_out") = py::none());
+  m.def("gelu8_split_fwd", &gelu8_split_fwd, py::arg("y"), py::arg("bias"), py::arg("by_cols"), py::arg("keep"));
+  m.def("gelu8_split_bwd", &gelu8_split_bwd, py::arg("dout"), py::arg("kept"), py::arg("scales"), py::arg("bias"), py::arg("by_rows"),
+        py::arg("by_cols"), py::arg("want_db"), py::arg("db_out") = py::none());
   m.def("pack8", &pack8);
   m.def("unpack8", &unpack8);
   m.def("weight_bf16_t", &weight_bf16_t);

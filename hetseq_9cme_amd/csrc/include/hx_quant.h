@@ -69,6 +69,24 @@ __device__ __forceinline__ float int8_val(uint32_t w, int j, float s) {
   return c == -128 ? __uint_as_float(0x7fc00000u) : (float)c * s;
 }
 
+// 8 int8 codes -> their values times s: a code plus 128 is a byte (one conversion) and b s - 128 s is exact, so
+// one fma each; codes of -128 and scales so large that 128 s is not finite take the careful way
+__device__ __forceinline__ void int8_vals(uint2 w, float s, float (&v)[8]) {
+  const uint32_t a = w.x ^ 0x80808080u, b = w.y ^ 0x80808080u;
+  const uint32_t zero = (((a - 0x01010101u) & ~a) | ((b - 0x01010101u) & ~b)) & 0x80808080u;   // some byte is 0
+  if (__builtin_expect(zero != 0 || s > 1.329227995784916e36f, 0)) {   // 2^120
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = int8_val(k < 4 ? w.x : w.y, k & 3, s);
+    return;
+  }
+  const float o = -128.f * s;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[k] = fmaf((float)((a >> (8 * k)) & 0xffu), s, o);
+    v[4 + k] = fmaf((float)((b >> (8 * k)) & 0xffu), s, o);
+  }
+}
+
 // two fp32 values -> packed bf16 (one v_cvt_pk_bf16_f32: nearest even, NaN kept)
 __device__ __forceinline__ uint32_t bf16x2(float a, float b) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));

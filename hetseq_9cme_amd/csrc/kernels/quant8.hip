@@ -61,6 +61,10 @@ struct TileF32 {
     }
   }
   __device__ float at(int i, int k) const { return v[i][k]; }
+  __device__ void set_row(int i, const float (&f)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[i][k] = f[k];
+  }
   __device__ uint2 row_codes(int i, float s) const {
     return make_uint2(e4m3x4(v[i][0], v[i][1], v[i][2], v[i][3], s), e4m3x4(v[i][4], v[i][5], v[i][6], v[i][7], s));
   }
@@ -99,6 +103,10 @@ struct TileBf16 {
       m[2 * j + 1] = (uint32_t)a[1] << 16;
     }
   }
+  __device__ void set_row(int i, const float (&f)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[i][j] = bf16x2(f[2 * j], f[2 * j + 1]);
+  }
   __device__ float at(int i, int k) const { return __uint_as_float(k & 1 ? w[i][k >> 1] & 0xffff0000u : w[i][k >> 1] << 16); }
   __device__ uint2 row_codes(int i, float s) const { return make_uint2(e4m3x4(w[i][0], w[i][1], s), e4m3x4(w[i][2], w[i][3], s)); }
   __device__ uint32_t col_codes(int k, float s) const {
@@ -109,24 +117,24 @@ struct TileBf16 {
 
 template <typename T>
 using Row8 = std::conditional_t<sizeof(T) == 4, TileF32<1>, TileBf16<1>>;
-// a lane's 8 entries of a block (16 lanes) -> their int8 codes; e: the block's exponent
+// a lane's 8 entries of a block (row i of 16 lanes) -> their int8 codes; e: the block's exponent
 template <typename Row>
-__device__ __forceinline__ uint2 int8_block(const Row& x, int& e) {
-  uint32_t m = max16u(x.row_max(0));
+__device__ __forceinline__ uint2 int8_block(const Row& x, int i, int& e) {
+  uint32_t m = max16u(x.row_max(i));
   if (__builtin_expect(m >= kInf, 0)) {   // (the 16 lanes agree)
     m = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(finite_abs(x.at(0, k))));
+    for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(finite_abs(x.at(i, k))));
     e = block_exp<Int8>(__uint_as_float(max16u(m)));
     const float is = exp2i(-e);
-    return make_uint2(int8x4(x.at(0, 0) * is, x.at(0, 1) * is, x.at(0, 2) * is, x.at(0, 3) * is),
-                      int8x4(x.at(0, 4) * is, x.at(0, 5) * is, x.at(0, 6) * is, x.at(0, 7) * is));
+    return make_uint2(int8x4(x.at(i, 0) * is, x.at(i, 1) * is, x.at(i, 2) * is, x.at(i, 3) * is),
+                      int8x4(x.at(i, 4) * is, x.at(i, 5) * is, x.at(i, 6) * is, x.at(i, 7) * is));
   }
   e = block_exp<Int8>(__uint_as_float(m));
   const float is = exp2i(-e);
   float f[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) f[k] = fmaf(x.at(0, k), is, kWhole);
+  for (int k = 0; k < 8; ++k) f[k] = fmaf(x.at(i, k), is, kWhole);
   return make_uint2(low_bytes(f[0], f[1], f[2], f[3]), low_bytes(f[4], f[5], f[6], f[7]));
 }
 
@@ -138,8 +146,15 @@ struct Split8Lds {
   float reds[SNT / 64][128];
 };
 
-template <typename Tile>
-__device__ __forceinline__ void split8_tile(const HxSplit8& a, int bid, Split8Lds& lds) {
+// `Step`: what is done to a tile between its load and its codes (rows r0 .., columns c0 .. of a thread's);
+// it may give the column sums of its own
+struct NoStep {
+  static constexpr bool sums = false;
+  template <typename Tile>
+  __device__ void operator()(Tile&, int, int, const HxSplit8&, float (&)[8]) const {}
+};
+template <typename Tile, typename Step = NoStep>
+__device__ __forceinline__ void split8_tile(const HxSplit8& a, int bid, Split8Lds& lds, const Step& step = {}) {
   auto& tile = lds.tile;
   auto& redm = lds.redm;
   auto& reds = lds.reds;
@@ -152,6 +167,8 @@ __device__ __forceinline__ void split8_tile(const HxSplit8& a, int bid, Split8Ld
   Tile x;
 #pragma unroll
   for (int i = 0; i < SR; ++i) x.load(a.x, (int64_t)(r0 + i) * a.ld + c0, i, r0 + i < a.R ? a.C - c0 : 0);
+  float own[8];
+  step(x, r0, c0, a, own);
   if (a.q) {
 #pragma unroll
     for (int i = 0; i < SR; ++i) {
@@ -192,7 +209,7 @@ __device__ __forceinline__ void split8_tile(const HxSplit8& a, int bid, Split8Ld
   if (a.colpart) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      float s = (x.at(0, k) + x.at(1, k)) + (x.at(2, k) + x.at(3, k));
+      float s = Step::sums ? own[k] : (x.at(0, k) + x.at(1, k)) + (x.at(2, k) + x.at(3, k));
       s += __shfl_xor(s, 16, 64);
       s += __shfl_xor(s, 32, 64);
       if ((t & 63) < 16) reds[w][8 * cg + k] = s;
@@ -260,8 +277,8 @@ __global__ __launch_bounds__(SNT) void split8_many_k(HxSplit8Batch d) {
 // gelu(u) = u Phi(u), Phi(u) = (1 + erf(z)) / 2 with z = u / 1.41421 (the model's truncated constant).
 // erfc by Abramowitz & Stegun 7.1.26 (a degree-5 polynomial in 1 / (1 + p |z|) times exp(-z^2), error at
 // most 1.5e-7), its constants taken with u: the exponential is the derivative's too.  Both directions move
-// 5 bytes per bf16 element; 16384 x 4096 takes 68 us forward (4.9 TB/s; a large copy runs at 5.1) and 76
-// us back (4.4: the derivative's arithmetic on what int8 decodes to takes what is left), 41 x 4096 3.0 and 5.1.
+// 5 bytes per bf16 element; 16384 x 4096 takes 68 us forward (4.9 TB/s; a large copy runs at 5.1) and 74
+// us back (4.5: the derivative's arithmetic on what int8 decodes to takes what is left), 41 x 4096 3.0 and 5.1.
 // Back, a workgroup takes 128 columns of kRowChunk rows: 512 columns at a time left 41 rows with 8
 // workgroups (11 us); every row loaded before the first is used took 87 us (registers).
 struct Gelu {
@@ -291,7 +308,7 @@ __global__ __launch_bounds__(NT) void gelu8_fwd_k(const T* __restrict__ y, const
     Row8<T> x;
     x.load(y, r * N + c0, 0, n);
     int e;
-    *reinterpret_cast<uint2*>(q + i * 128 + 8 * l16) = int8_block(x, e);
+    *reinterpret_cast<uint2*>(q + i * 128 + 8 * l16) = int8_block(x, 0, e);
     if (l16 == 0) s[i] = (uint8_t)(e + 127);
     float v[8], bb[8];
 #pragma unroll
@@ -324,10 +341,11 @@ __global__ __launch_bounds__(NT) void gelu8_bwd_k(const T* __restrict__ dout, co
     float d[8];
     load_upto<T>(dout + r * N + c0, n, d);
     const uint2 w = *reinterpret_cast<const uint2*>(q + i * 128 + 8 * l16);
-    const float sc = scale_of(s[i]);
+    float yv[8];
+    int8_vals(w, scale_of(s[i]), yv);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float u = int8_val(k < 4 ? w.x : w.y, k & 3, sc) + bb[k];
+      const float u = yv[k] + bb[k];
       const Gelu g = gelu_parts(u);
       // d/du u Phi(u) = Phi + u exp(-z^2) / (1.41421 sqrt(pi))
       d[k] *= fmaf(u * (0.5641895835477563f / 1.41421f), g.bell, g.cdf);
@@ -347,6 +365,87 @@ __global__ __launch_bounds__(NT) void gelu8_bwd_k(const T* __restrict__ dout, co
   }
 }
 
+// ---------------------------------------------------------------- GELU on the way to a product's operand
+// Between the two products of a feed-forward layer the GELU's result is read by the second one only, and
+// its input's gradient by the first one's gradient products only: they go straight to e4m3 codes (both
+// blockings, as split8) and the tensors themselves are never written.  Same arithmetic, and the same
+// rounding to T in between, as gelu8 and split8 one after the other: equal bits.  5 bytes per bf16 element
+// each way where those move 9; 16384 x 4096 takes 85 us forward and 105 back (118 and 125 one after the
+// other), bound by the vector arithmetic of both.  64 registers for a fourth workgroup per CU spill (91, 122).
+struct GeluStep {   // y -> gelu(y + b), y's int8 blocks kept (q null: not kept)
+  static constexpr bool sums = false;
+  const float* b;
+  uint8_t *q, *s;
+  template <typename Tile>
+  __device__ void operator()(Tile& x, int r0, int c0, const HxSplit8& a, float (&)[8]) const {
+    const int nb = (a.C + 127) / 128, l16 = threadIdx.x & 15;
+    float bb[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) bb[k] = 0.f;
+    if (b) load_upto<float>(b + c0, a.C - c0, bb);
+#pragma unroll
+    for (int i = 0; i < SR; ++i) {
+      const bool in = r0 + i < a.R;
+      if (q) {
+        int e;
+        const uint2 codes = int8_block(x, i, e);
+        const int64_t blk = (int64_t)(r0 + i) * nb + c0 / 128;
+        if (in) {
+          *reinterpret_cast<uint2*>(q + blk * 128 + 8 * l16) = codes;
+          if (l16 == 0) s[blk] = (uint8_t)(e + 127);
+        }
+      }
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float u = x.at(i, k) + bb[k];
+        v[k] = in ? u * gelu_parts(u).cdf : 0.f;   // (columns past the last: gelu(0) = 0)
+      }
+      x.set_row(i, v);
+    }
+  }
+};
+struct GeluBackStep {   // dout -> dout gelu'(y^ + b), and its column sums (of the values before their rounding to T)
+  static constexpr bool sums = true;
+  const float* b;
+  const uint8_t *q, *s;
+  template <typename Tile>
+  __device__ void operator()(Tile& x, int r0, int c0, const HxSplit8& a, float (&sum)[8]) const {
+    const int nb = (a.C + 127) / 128, l16 = threadIdx.x & 15;
+    uint2 w[SR];
+    float sc[SR];
+#pragma unroll
+    for (int i = 0; i < SR; ++i) {
+      const int64_t blk = (int64_t)(r0 + i) * nb + c0 / 128;
+      const bool in = r0 + i < a.R;
+      w[i] = in ? *reinterpret_cast<const uint2*>(q + blk * 128 + 8 * l16) : make_uint2(0, 0);
+      sc[i] = in ? scale_of(s[blk]) : 1.f;
+    }
+    float bb[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) bb[k] = sum[k] = 0.f;
+    if (b) load_upto<float>(b + c0, a.C - c0, bb);
+#pragma unroll
+    for (int i = 0; i < SR; ++i) {
+      float d[8], yv[8];
+      int8_vals(w[i], sc[i], yv);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float u = yv[k] + bb[k];
+        const Gelu g = gelu_parts(u);
+        d[k] = x.at(i, k) * fmaf(u * (0.5641895835477563f / 1.41421f), g.bell, g.cdf);
+        sum[k] += d[k];
+      }
+      x.set_row(i, d);
+    }
+  }
+};
+template <typename Tile, typename Step>
+__global__ __launch_bounds__(SNT) void gelu8_split_k(HxSplit8 a, Step step) {
+  __shared__ __attribute__((aligned(16))) Split8Lds lds;
+  split8_tile<Tile>(a, blockIdx.x, lds, step);
+}
+
 // ---------------------------------------------------------------- pack8 / unpack8
 // One pass, 16 lanes to a block; bound by memory: 16384 x 1024 fp32 (84 MB) 16 us each way (5.3 TB/s, part
 // of it from the last level cache), 1312 x 768 bf16 2.5 us.
@@ -360,7 +459,7 @@ __global__ __launch_bounds__(NT) void pack8_k(const T* __restrict__ x, uint8_t* 
     Row8<T> v;
     v.load(x, r * N + c0, 0, N - c0);
     int e;
-    *reinterpret_cast<uint2*>(q + i * 128 + 8 * l16) = int8_block(v, e);
+    *reinterpret_cast<uint2*>(q + i * 128 + 8 * l16) = int8_block(v, 0, e);
     if (l16 == 0) s[i] = (uint8_t)(e + 127);
   }
 }
@@ -373,10 +472,8 @@ __global__ __launch_bounds__(NT) void unpack8_k(const uint8_t* __restrict__ q, c
     const int64_t r = i / nb;
     const int c0 = (int)(i - r * nb) * 128 + 8 * l16;
     const uint2 w = *reinterpret_cast<const uint2*>(q + i * 128 + 8 * l16);
-    const float sc = scale_of(s[i]);
     float v[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = int8_val(k < 4 ? w.x : w.y, k & 3, sc);
+    int8_vals(w, scale_of(s[i]), v);
     store_upto<T>(x + r * N + c0, N - c0, v);
   }
 }
@@ -403,6 +500,20 @@ void hx_split8(const HxSplit8* jobs, int n, hipStream_t stream) {
   else if (a.bf16) split8_k<TileBf16<SR>, TileF32<SR>><<<grid, SNT, 0, stream>>>(a, b);
   else if (b.bf16) split8_k<TileF32<SR>, TileBf16<SR>><<<grid, SNT, 0, stream>>>(a, b);
   else split8_k<TileF32<SR>, TileF32<SR>><<<grid, SNT, 0, stream>>>(a, b);
+}
+
+void hx_gelu8_split_fwd(const HxSplit8& a, const float* b, uint8_t* q, uint8_t* s, hipStream_t stream) {
+  const unsigned grid = (unsigned)(((a.C + 127) / 128) * (int64_t)((a.R + 127) / 128));
+  const GeluStep step{b, q, s};
+  if (a.bf16) gelu8_split_k<TileBf16<SR>><<<grid, SNT, 0, stream>>>(a, step);
+  else gelu8_split_k<TileF32<SR>><<<grid, SNT, 0, stream>>>(a, step);
+}
+
+void hx_gelu8_split_bwd(const HxSplit8& a, const float* b, const uint8_t* q, const uint8_t* s, hipStream_t stream) {
+  const unsigned grid = (unsigned)(((a.C + 127) / 128) * (int64_t)((a.R + 127) / 128));
+  const GeluBackStep step{b, q, s};
+  if (a.bf16) gelu8_split_k<TileBf16<SR>><<<grid, SNT, 0, stream>>>(a, step);
+  else gelu8_split_k<TileF32<SR>><<<grid, SNT, 0, stream>>>(a, step);
 }
 
 void hx_split8_many(const HxSplit8Batch& d, hipStream_t stream) {

@@ -298,6 +298,9 @@ class BertLayer(nn.Module):
         attention_output = self.attention(hidden_states, attention_mask_bias)
         rg = ops.ResidualGrad()     # residual grad of attention_output -> FFN-up dgrad GEMM
         up = self.intermediate.dense_act
+        if up.fp8 and up.act == 'gelu' and self.output.fp8:
+            y = ops.ffn_fp8(attention_output, up.weight, up.bias, self.output.dense.weight, rg, codes=(up.codes, self.output.codes))
+            return self.output.finish(y, attention_output, rg)
         if not up.fp8 and up.act == 'gelu' and ops.ffn_fusable(attention_output, up.weight, up.bias, self.output.dense.weight):
             # fp32 runs: bias + GELU in the FFN-up GEMM's epilogue, the GELU backward in the
             # FFN-down data gradient's (ops.ffn)

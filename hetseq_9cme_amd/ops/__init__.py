@@ -12,7 +12,7 @@ from .fused import (  # noqa: F401
     set_side_stream, active_side_stream, side_join, ffn, ffn_fusable, qkv_weight_view, weight_pieces_scope,
 )
 from .fp8 import (  # noqa: F401
-    linear_fp8, linear3_fp8, Fp8Weight, fp8_weights, pack8, unpack8, Packed8, checkpoint8,
+    linear_fp8, linear3_fp8, ffn_fp8, Fp8Weight, fp8_weights, pack8, unpack8, Packed8, checkpoint8,
 )
 
 

@@ -208,27 +208,38 @@ class _LinearFp8Fn(torch.autograd.Function):
                     *_parts(dW, Ws, None), *_parts(db, bs, None))
         bslots, bview = _slots(bs) if need_b else (None, None)
         q, s, qt, st, db = C().split8(dy2, need_x, need_w and M > 0, need_b, bview)
-        gW = (None,) * len(Ws)
-        if need_w:
-            slots, view = _slots(Ws)
-            side = fused.side_begin(dy2.device, M) if view is not None and M > 0 else None
-            with fused.side_ctx(side):
-                if M == 0:
-                    dW = view.zero_() if view is not None else torch.zeros(N, K, device=dy.device)
-                else:
-                    dW = C().gemm_fp8(qt, st, xt, xs, M, False, out=view)
-                gW = _parts(dW, Ws, slots, view is not None)
-            fused._record(side, qt, st, xt, xs)
-        dx = None
-        if need_x:
-            acc = other = None
-            if ctx.mbox is not None:
-                acc, other = ctx.mbox.take(dy.dtype)
-            acc = acc.view(M, K) if acc is not None else None
-            dx = C().gemm_fp8(q, s, wt, ws, N, dy.dtype == torch.bfloat16, out=acc, beta=acc is not None).view(ctx.xshape)
-            if other is not None:
-                dx = dx + other.view(ctx.xshape).to(dx.dtype)
+        gW = _weight_grads(Ws, (N, K), qt, st, xt, xs, M) if need_w else (None,) * len(Ws)
+        dx = _input_grad(q, s, wt, ws, N, M, ctx.xshape, dy.dtype == torch.bfloat16, ctx.mbox) if need_x else None
         return (dx, None, None, None, None, None, *gW, *_parts(db, bs, bslots, bview is not None))
+
+
+def _weight_grads(Ws, shape, qt, st, xt, xs, M):
+    """The stacked weights' gradients from the token-blocked codes of dy (qt, st) and of x (xt, xs): into
+    their flat slots, on the side stream, where they have them."""
+    slots, view = _slots(Ws)
+    side = fused.side_begin(Ws[0].device, M) if view is not None and M > 0 else None
+    with fused.side_ctx(side):
+        if M == 0:
+            dW = view.zero_() if view is not None else torch.zeros(shape, device=Ws[0].device)
+        else:
+            dW = C().gemm_fp8(qt, st, xt, xs, M, False, out=view)
+        g = _parts(dW, Ws, slots, view is not None)
+    fused._record(side, qt, st, xt, xs)
+    return g
+
+
+def _weight_grad(W, qt, st, xt, xs, M):
+    return _weight_grads((W,), tuple(W.shape), qt, st, xt, xs, M)[0]
+
+
+def _input_grad(q, s, wt, ws, N, M, xshape, bf16, mbox):
+    """dx from the codes of dy (q, s) and of W^T (wt, ws), onto the residual gradient in ``mbox``."""
+    acc = other = None
+    if mbox is not None:
+        acc, other = mbox.take(torch.bfloat16 if bf16 else torch.float32)
+    acc = acc.view(M, xshape[-1]) if acc is not None else None
+    dx = C().gemm_fp8(q, s, wt, ws, N, bf16, out=acc, beta=acc is not None).view(xshape)
+    return dx if other is None else dx + other.view(xshape).to(dx.dtype)
 
 
 def _slots(params):
@@ -358,6 +369,73 @@ def bias_gelu8(y, b):
     if use_kernels(y) and not _flat(b):
         return C().bias_gelu8(y, b)
     return _BiasGelu8Fn.apply(y.contiguous(), b)
+
+
+# ---------------------------------------------------------------- feed-forward
+class _FfnFp8Fn(torch.autograd.Function):
+    """gelu(x W1^T + b1) W2^T with the GELU's result and its input's gradient going straight to e4m3 codes
+    (quant8.hip gelu8_split_k): neither tensor is written."""
+
+    @staticmethod
+    def forward(ctx, x, c1, c2, mbox, W1, b1, W2):
+        need_x, _, _, _, need_1, need_b, need_2 = ctx.needs_input_grad
+        ctx.xshape, ctx.mbox, ctx.W1, ctx.b1, ctx.W2 = x.shape, mbox, W1, b1, W2
+        ctx.need_u = need_u = need_x or need_1 or need_b   # anything behind the GELU
+        x2, bf16 = _rows2(x), x.dtype == torch.bfloat16
+        q, s, xt, xs, _ = C().split8(x2, True, need_1)
+        y = C().gemm_fp8(q, s, c1.q, c1.s, W1.shape[1], bf16)
+        q, s, at, as_, kq, ks = C().gelu8_split_fwd(y, b1, need_2, need_u)
+        out = C().gemm_fp8(q, s, c2.q, c2.s, W2.shape[1], bf16)
+        w1 = (c1.qt, c1.st) if need_x else (None, None)
+        w2 = (c2.qt, c2.st) if need_u else (None, None)
+        ctx.save_for_backward(xt, xs, at, as_, kq, ks, *w1, *w2)
+        return out.view(*x.shape[:-1], W2.shape[0])
+
+    @staticmethod
+    def backward(ctx, dy):
+        _first_derivatives('ffn_fp8')
+        xt, xs, at, as_, kq, ks, w1, w1s, w2, w2s = ctx.saved_tensors
+        need_x, _, _, _, need_1, need_b, need_2 = ctx.needs_input_grad
+        W1, b1, W2 = ctx.W1, ctx.b1, ctx.W2
+        dy2, bf16 = _rows2(dy), dy.dtype == torch.bfloat16
+        M = dy2.shape[0]
+        q, s, qt, st, _ = C().split8(dy2, ctx.need_u, need_2 and M > 0)
+        g2 = _weight_grad(W2, qt, st, at, as_, M) if need_2 else None
+        dx = g1 = db = None
+        if ctx.need_u:
+            da = C().gemm_fp8(q, s, w2, w2s, W2.shape[0], bf16)
+            q, s, qt, st, db = C().gelu8_split_bwd(da, kq, ks, b1, need_x, need_1 and M > 0, need_b,
+                                                   fused.grad_slot(b1) if need_b else None)
+            g1 = _weight_grad(W1, qt, st, xt, xs, M) if need_1 else None
+            if need_x:
+                dx = _input_grad(q, s, w1, w1s, W1.shape[0], M, ctx.xshape, bf16, ctx.mbox)
+        return dx, None, None, None, g1, db, g2
+
+
+def ffn_fp8(x, W1, b1, W2, res_grad=None, codes=(None, None)):
+    """gelu(x W1^T + b1) W2^T on e4m3 operands: ``linear_fp8(bias_act(linear_fp8(x, W1), b1, 'gelu', bits=8),
+    W2)`` -- the same roundings, b1's gradient summed in another order -- without writing the GELU's result
+    or the gradient of its input.  ``W1`` [F, K], ``b1`` fp32 [F] or None, ``W2`` [N, F]; ``codes``: the ``Fp8Weight``
+    of each where the caller has made it for this forward; ``res_grad`` as in ``linear_fp8``."""
+    _check_act(x, 'ffn_fp8')
+    for W in (W1, W2):
+        _check_weight(W, 'ffn_fp8')
+    if x.shape[-1] != W1.shape[1] or W2.shape[1] != W1.shape[0]:
+        raise ValueError('ffn_fp8: x {}, weights {} and {}'.format(tuple(x.shape), tuple(W1.shape), tuple(W2.shape)))
+    if x.device != W1.device or x.device != W2.device:
+        raise ValueError('ffn_fp8: x on {}, the weights on {} and {}'.format(x.device, W1.device, W2.device))
+    _check_bias(b1, W1.shape[0], x, 'ffn_fp8')
+    if not use_kernels(x):
+        return linear_fp8(bias_gelu8(linear_fp8(x, W1, res_grad=res_grad, codes=codes[0]), b1), W2, codes=codes[1])
+    grad = torch.is_grad_enabled()
+    need_x = grad and x.requires_grad
+    need_u = need_x or grad and (W1.requires_grad or b1 is not None and b1.requires_grad)
+    c = []
+    for W, given, need in ((W1, codes[0], need_x), (W2, codes[1], need_u)):
+        if given is not None:
+            _check_codes(given, tuple(W.shape), W.device, need, 'ffn_fp8')
+        c.append(given if given is not None else Fp8Weight(W, need))
+    return _FfnFp8Fn.apply(x, c[0], c[1], res_grad, W1, b1, W2)
 
 
 # ---------------------------------------------------------------- kept activations

@@ -161,6 +161,10 @@ def test_residual_gradient():
     (lambda: ops.linear_fp8(torch.zeros(2, 4), torch.zeros(3, 4), codes=ops.Fp8Weight(torch.zeros(4, 4))), ValueError),
     (lambda: ops.linear_fp8(torch.zeros(2, 4, requires_grad=True), torch.zeros(3, 4),
                             codes=ops.Fp8Weight(torch.zeros(3, 4), grad=False)), ValueError),
+    (lambda: ops.ffn_fp8(torch.zeros(2, 4), torch.zeros(6, 4), None, torch.zeros(3, 5)), ValueError),
+    (lambda: ops.ffn_fp8(torch.zeros(2, 4), torch.zeros(6, 5), None, torch.zeros(3, 6)), ValueError),
+    (lambda: ops.ffn_fp8(torch.zeros(2, 4), torch.zeros(6, 4), torch.zeros(3), torch.zeros(3, 6)), ValueError),
+    (lambda: ops.ffn_fp8(torch.zeros(2, 4, dtype=torch.float16), torch.zeros(6, 4), None, torch.zeros(3, 6)), TypeError),
     (lambda: ops.linear3_fp8(torch.zeros(2, 100), *[torch.zeros(4, 128)] * 3, None, None, None), ValueError),
     (lambda: ops.linear3_fp8(torch.zeros(2, 128), *[torch.zeros(4, 128)] * 3, None, None, None,
                              codes=ops.Fp8Weight(torch.zeros(4, 128))), ValueError),

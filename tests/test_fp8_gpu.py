@@ -395,6 +395,79 @@ def test_results_repeat_bit_for_bit(dev):
             assert torch.equal(a, b)
 
 
+# ---------------------------------------------------------------- feed-forward
+def _ffn_data(M, K, F, N, dt):
+    x = rand((M, K), dt, M + F).requires_grad_(True)
+    W1, W2 = (rand((F, K), torch.float32, 2) * 0.05).requires_grad_(True), (rand((N, F), torch.float32, 3) * 0.05).requires_grad_(True)
+    return x, W1, rand((F,), torch.float32, 4).requires_grad_(True), W2, rand((M, N), dt, 5)
+
+
+@pytest.mark.parametrize('dt', ['fp32', 'bf16'])
+@pytest.mark.parametrize('M,K,F,N', [(1, 1, 1, 1), (3, 130, 257, 5), (65, 128, 512, 128), (130, 96, 1001, 33), (700, 256, 384, 130)])
+def test_ffn_fp8_equals_its_parts(dev, M, K, F, N, dt):
+    """The same arithmetic and roundings as linear, GELU and linear one after the other: equal bits; b1's
+    gradient, summed over 128 rows at a time instead of 64, within (M + 8) steps of the sum of magnitudes
+    of what is summed (half a step per addition, twice)."""
+    x, W1, b1, W2, d = _ffn_data(M, K, F, N, DT[dt])
+    y = ops.ffn_fp8(x, W1, b1, W2)
+    h = ops.linear_fp8(x, W1)
+    a = ops.bias_act(h, b1, 'gelu', bits=8)
+    r = ops.linear_fp8(a, W2)
+    assert y.dtype == x.dtype and torch.equal(y, r)
+    got = torch.autograd.grad(y, (x, W1, W2, b1), d)
+    da, = torch.autograd.grad(r, a, d, retain_graph=True)
+    ref = torch.autograd.grad(r, (x, W1, W2, b1), d)
+    for n, p, q in zip(('dx', 'dW1', 'dW2'), got, ref):
+        assert torch.equal(p, q), n
+    u = int8(h.detach()) + b1.detach().double()
+    mag = (da.double() * gelu_slope64(u)).abs().sum(0)
+    assert ((got[3] - ref[3]).double().abs() <= (M + 8) * 2.0 ** -23 * mag + 1e-37).all()
+    with torch.no_grad():
+        assert torch.equal(ops.ffn_fp8(x, W1, b1, W2), y)
+        both = ops.fp8_weights([W1, W2])
+        assert torch.equal(ops.ffn_fp8(x, W1, b1, W2, codes=both), y)
+        assert torch.equal(ops.ffn_fp8(x.view(1, M, K), W1, b1, W2, codes=both), y.view(1, M, N))
+
+
+def test_ffn_fp8_parts_of_the_gradient(dev):
+    """Each leaf alone, no bias, a residual gradient, no rows."""
+    x, W1, b1, W2, d = _ffn_data(200, 128, 384, 96, torch.bfloat16)
+    full = torch.autograd.grad(ops.ffn_fp8(x, W1, b1, W2), (x, W1, b1, W2), d)
+    for i in range(4):
+        leaves = [t.detach().requires_grad_(j == i) for j, t in enumerate((x, W1, b1, W2))]
+        g, = torch.autograd.grad(ops.ffn_fp8(*leaves), leaves[i], d)
+        assert torch.equal(g, full[i]), i
+    y = ops.ffn_fp8(x, W1, None, W2)
+    r = ops.linear_fp8(ops.bias_act(ops.linear_fp8(x, W1), None, 'gelu', bits=8), W2)
+    assert torch.equal(y, r)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (x, W1, W2), d), torch.autograd.grad(r, (x, W1, W2), d)))
+    res = rand((200, 128), torch.bfloat16, 9)
+    out = []
+    for f in (lambda m: ops.ffn_fp8(x, W1, b1, W2, m),
+              lambda m: ops.linear_fp8(ops.bias_act(ops.linear_fp8(x, W1, res_grad=m), b1, 'gelu', bits=8), W2)):
+        m = ops.ResidualGrad()
+        y = f(m)
+        assert m.deposit(res.clone())
+        out.append(torch.autograd.grad(y, x, d)[0])
+    assert torch.equal(*out)
+    e = torch.zeros(0, 128, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    y = ops.ffn_fp8(e, W1, b1, W2)
+    g = torch.autograd.grad(y, (e, W1, b1, W2), torch.zeros(0, 96, dtype=torch.bfloat16, device=dev))
+    assert y.shape == (0, 96) and g[0].shape == (0, 128) and not any(t.any() for t in g)
+
+
+def test_ffn_fp8_nonfinite(dev):
+    x, W1, b1, W2, d = _ffn_data(200, 128, 384, 96, torch.float32)
+    x = x.detach().clone()
+    x[7, 3], x[150, 100] = float('inf'), float('nan')
+    y = ops.ffn_fp8(x, W1, b1, W2)
+    bad = torch.zeros(200, dtype=torch.bool, device=dev)
+    bad[[7, 150]] = True
+    assert torch.equal(torch.isnan(y).any(1), bad)
+    gb, = torch.autograd.grad(y, b1, d)
+    assert torch.isnan(gb).all()
+
+
 # ---------------------------------------------------------------- calls side by side
 def test_bias_at_any_element(dev):
     """A bias that starts between two 16-B boundaries (a view into a larger buffer)."""
