@@ -1002,7 +1002,7 @@ struct Codes8 {
 // A gradient that is captured into a graph for a leaf whose accumulator was made on another stream (an
 // eager graph of the same leaf is alive): autograd would make that stream wait for the capturing one,
 // which a capture cannot hold and which ends the process.  Refused before it comes to that.
-static void refuse_stale_leaves(const Tensor& like, const char* what) {
+static void refuse_stale_leaves(const Tensor& like, const std::string& what) {
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(cur_stream(like), &st) != hipSuccess || st == hipStreamCaptureStatusNone) return;
   const auto node = torch::autograd::get_current_node();
@@ -1703,6 +1703,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_fp8_fwd", &linear_fp8_fwd, py::arg("x"), py::arg("wq"), py::arg("ws"), py::arg("bias"), py::arg("keep"));
   m.def("linear_fp8", &linear_fp8, py::arg("x"), py::arg("W"), py::arg("bias"), py::arg("w8"), py::arg("grad"));
   m.def("linear_fp8_infer", &linear_fp8_infer, py::arg("x"), py::arg("wq"), py::arg("ws"), py::arg("K"), py::arg("bias"));
+  m.def("refuse_stale_leaves", &refuse_stale_leaves);
   m.def("bias_gelu8", &bias_gelu8, py::arg("y"), py::arg("bias"));
   m.def("gelu8_fwd", &gelu8_fwd);
   m.def("gelu8_bwd", &gelu8_bwd, py::arg("dout"), py::arg("q"), py::arg("s"), py::arg("bias"), py::arg("want_db"),

@@ -57,9 +57,11 @@ def _check_bias(b, n, like, what):
             what, n, like.device, b.dtype, tuple(b.shape), b.device))
 
 
-def _first_derivatives(what):
+def _backward_checks(what, dy):
     if torch.is_grad_enabled():
         raise RuntimeError('{}: first derivatives only (create_graph=True is not supported)'.format(what))
+    if use_kernels(dy):
+        C().refuse_stale_leaves(dy, what)   # (captures only)
 
 
 # ---------------------------------------------------------------- references (CPU, and the numerics oracle)
@@ -191,7 +193,7 @@ class _LinearFp8Fn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        _first_derivatives('linear_fp8')
+        _backward_checks('linear_fp8', dy)
         xt, xs, wt, ws = ctx.saved_tensors
         n, Ws, bs = ctx.n, ctx.Ws, ctx.bs
         N, K = ctx.wshape
@@ -352,7 +354,7 @@ class _BiasGelu8Fn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        _first_derivatives('bias_act(bits=8)')
+        _backward_checks('bias_act(bits=8)', dout)
         q, s = ctx.saved_tensors
         b, need_b = ctx.b, ctx.needs_input_grad[1]
         if use_kernels(dout):
@@ -393,7 +395,7 @@ class _FfnFp8Fn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        _first_derivatives('ffn_fp8')
+        _backward_checks('ffn_fp8', dy)
         xt, xs, at, as_, kq, ks, w1, w1s, w2, w2s = ctx.saved_tensors
         need_x, _, _, _, need_1, need_b, need_2 = ctx.needs_input_grad
         W1, b1, W2 = ctx.W1, ctx.b1, ctx.W2

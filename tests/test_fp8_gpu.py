@@ -607,28 +607,33 @@ def test_rows_past_two_to_the_31st_element(dev):
     assert torch.equal(a[-300:], b) and not a[:-300].any()
 
 
-def test_capture_is_refused_while_an_eager_graph_lives(dev):
+@pytest.mark.parametrize('what', ['linear', 'mailbox', 'gelu', 'ffn'])
+def test_capture_is_refused_while_an_eager_graph_lives(dev, what):
     """A leaf's gradient accumulator that an eager graph on another stream holds cannot take part in a
     capture: an error from the layer's backward, and the same capture works once that graph is gone."""
     x = rand((100, 128), torch.bfloat16, 1)
     W = (rand((64, 128), torch.float32, 2) * 0.02).requires_grad_(True)
-    d = rand((100, 64), torch.bfloat16, 3)
-    alive = ops.linear_fp8(x, W)
+    W2 = rand((128, 64), torch.float32, 5) * 0.02
+    b = rand((128,), torch.float32, 4).requires_grad_(True)
+    leaf, d = (b, rand((100, 128), torch.bfloat16, 3)) if what == 'gelu' else (W, rand((100, 128 if what == 'ffn' else 64), torch.bfloat16, 3))
+    run = {'linear': lambda: ops.linear_fp8(x, W), 'mailbox': lambda: ops.linear_fp8(x, W, res_grad=ops.ResidualGrad()),
+           'gelu': lambda: ops.bias_act(x, b, 'gelu', bits=8), 'ffn': lambda: ops.ffn_fp8(x, W, None, W2)}[what]
+    alive = run()
     st = torch.cuda.Stream()
     st.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(st):
-        y = ops.linear_fp8(x, W)
+        y = run()
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with pytest.raises(RuntimeError, match='eager graphs released first'):
         with torch.cuda.graph(graph):
-            torch.autograd.grad(ops.linear_fp8(x, W), W, d)
+            torch.autograd.grad(run(), leaf, d)
     del alive, y
-    graph, out = _captured(lambda: torch.autograd.grad(ops.linear_fp8(x, W), W, d))
+    graph, out = _captured(lambda: torch.autograd.grad(run(), leaf, d))
     for _ in range(3):
         graph.replay()
         torch.cuda.synchronize()
-        assert torch.equal(out[0], torch.autograd.grad(ops.linear_fp8(x, W), W, d)[0])
+        assert torch.equal(out[0], torch.autograd.grad(run(), leaf, d)[0])
 
 
 def test_inference_refusals(dev):
