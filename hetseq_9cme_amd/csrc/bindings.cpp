@@ -810,12 +810,12 @@ std::vector<OptT> split8(Tensor x, bool by_rows, bool by_cols, bool want_sum, Op
   return {q, s, qt, st, sum};
 }
 
-// both blockings of every weight, one launch: [(q, s, qt, st)] as split8 makes them
-std::vector<std::vector<Tensor>> split8_weights(std::vector<Tensor> Ws) {
+// every weight's codes, one launch: [(q, s, qt, st)] as split8 makes them (by_cols: qt and st, else undefined)
+std::vector<std::vector<OptT>> split8_weights(std::vector<Tensor> Ws, bool by_cols) {
   TORCH_CHECK(!Ws.empty() && Ws.size() <= HX_WBATCH, "split8_weights: 1..64 weights");
   HxSplit8Batch d{};
   d.n = (int)Ws.size();
-  std::vector<std::vector<Tensor>> out;
+  std::vector<std::vector<OptT>> out;
   c10::hip::HIPGuardMasqueradingAsCUDA guard(Ws[0].device());
   auto u8 = Ws[0].options().dtype(torch::kUInt8);
   int64_t tiles = 0;
@@ -826,13 +826,17 @@ std::vector<std::vector<Tensor>> split8_weights(std::vector<Tensor> Ws) {
     TORCH_CHECK(W.size(0) >= 1 && W.size(0) <= (1LL << 22) && aligned16(W.data_ptr()) && W.device() == Ws[0].device(),
                 "split8_weights: contiguous fp32 [1 .. 2^22, K] weights with 16-B aligned storage on one device");
     const int64_t N = W.size(0), K = W.size(1);
-    out.push_back({torch::empty({N, blocks128(K) * 128}, u8), scale_words(N, K, W), torch::empty({K, blocks128(N) * 128}, u8),
-                   scale_words(K, N, W)});
+    std::vector<OptT> w{torch::empty({N, blocks128(K) * 128}, u8), scale_words(N, K, W), c10::nullopt, c10::nullopt};
+    if (by_cols) {
+      w[2] = torch::empty({K, blocks128(N) * 128}, u8);
+      w[3] = scale_words(K, N, W);
+    }
     d.W[i] = W.data_ptr<float>();
-    d.q[i] = out[i][0].data_ptr<uint8_t>();
-    d.s[i] = out[i][1].data_ptr<uint8_t>();
-    d.qt[i] = out[i][2].data_ptr<uint8_t>();
-    d.st[i] = out[i][3].data_ptr<uint8_t>();
+    d.q[i] = ptr_or_null<uint8_t>(w[0]);
+    d.s[i] = ptr_or_null<uint8_t>(w[1]);
+    d.qt[i] = ptr_or_null<uint8_t>(w[2]);
+    d.st[i] = ptr_or_null<uint8_t>(w[3]);
+    out.push_back(std::move(w));
     d.R[i] = (int)N;
     d.C[i] = (int)K;
     d.start[i] = (int)tiles;
@@ -1697,7 +1701,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("bias") = py::none(), py::arg("out_bf16") = true);
   m.def("split8", &split8, py::arg("x"), py::arg("by_rows"), py::arg("by_cols"), py::arg("want_sum") = false,
         py::arg("sum_out") = py::none());
-  m.def("split8_weights", &split8_weights);
+  m.def("split8_weights", &split8_weights, py::arg("Ws"), py::arg("by_cols") = true);
   m.def("gemm_fp8", &gemm_fp8, py::arg("a"), py::arg("as"), py::arg("b"), py::arg("bs"), py::arg("K"), py::arg("out_bf16"),
         py::arg("out") = py::none(), py::arg("beta") = false, py::arg("bias") = py::none());
   m.def("linear_fp8_fwd", &linear_fp8_fwd, py::arg("x"), py::arg("wq"), py::arg("ws"), py::arg("bias"), py::arg("keep"));

@@ -256,7 +256,7 @@ void hx_split8(const HxSplit8* jobs, int n, hipStream_t stream);
 void hx_gelu8_split_fwd(const HxSplit8& a, const float* b, uint8_t* q, uint8_t* s, hipStream_t stream);
 // the same of a.x gelu'(y + b), y from its int8 blocks
 void hx_gelu8_split_bwd(const HxSplit8& a, const float* b, const uint8_t* q, const uint8_t* s, hipStream_t stream);
-// up to HX_WBATCH contiguous fp32 weights [R, C], both blockings of each, in one launch; tile t of weight
+// up to HX_WBATCH contiguous fp32 weights [R, C], both blockings of each (or q, s alone), in one launch; tile t of weight
 // i is workgroup start[i] + t
 struct HxSplit8Batch {
   int n;

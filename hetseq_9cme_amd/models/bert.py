@@ -353,21 +353,45 @@ class BertEncoder(nn.Module):
             self.__dict__['_pw_params'] = ps
         return [ops.qkv_weight_view(*p) if isinstance(p, tuple) else p for p in ps]
 
-    @contextlib.contextmanager
-    def _weight_codes(self):
-        """The e4m3 codes of every linear weight, made in one launch and handed to the layers for this
-        forward alone (a segment recomputed in the backward makes its own)."""
+    def _parts(self):
+        """The layers' modules that hold a linear weight, in order."""
         parts = self.__dict__.get('_fp8_parts')
         if parts is None or len(parts) != 4 * len(self.layer):
             parts = self.__dict__['_fp8_parts'] = [
                 part for layer in self.layer for part in (layer.attention.self, layer.attention.output,
                                                           layer.intermediate.dense_act, layer.output)]
-        # the weights as the parts hold them now (a replaced layer is not in `parts`: it makes its own codes)
-        Ws = [ops.qkv_weight_view(part.query.weight, part.key.weight, part.value.weight) if isinstance(part, BertSelfAttention)
-              else part.weight if isinstance(part, LinearActivation) else part.dense.weight for part in parts]
+        return parts
+
+    def _fp8_codes(self, grad):
+        # the weights as the parts hold them now (a replaced layer is not among the parts: it makes its own codes)
+        Ws = []
+        for part in self._parts():
+            if isinstance(part, BertSelfAttention):
+                qkv = [part.query.weight, part.key.weight, part.value.weight]
+                W = ops.qkv_weight_view(*qkv)
+                Ws.append(W if W is not None else torch.cat([w.detach() for w in qkv], 0))
+            else:
+                Ws.append(part.weight if isinstance(part, LinearActivation) else part.dense.weight)
+        return ops.fp8_weights(Ws, grad)
+
+    def keep_fp8_weights(self, keep=True):
+        """For serving at fp8: the layers' weights are brought to 8 bits now, and every forward without
+        gradients reads those until the next call (``keep=False``: codes once per forward again).  A
+        forward with gradients always takes the weights as they are."""
+        self.__dict__['_fp8_kept'] = self._fp8_codes(False) if keep else None
+
+    @contextlib.contextmanager
+    def _weight_codes(self):
+        """The e4m3 codes of every linear weight, made in one launch (or kept: ``keep_fp8_weights``) and
+        handed to the layers for this forward alone: a segment recomputed in the backward makes its
+        own."""
+        parts, grad = self._parts(), torch.is_grad_enabled()
+        codes = None if grad else self.__dict__.get('_fp8_kept')
+        if codes is None or len(codes) != len(parts):
+            codes = self._fp8_codes(grad)
         try:
-            for part, codes in zip(parts, ops.fp8_weights(Ws)):
-                part.__dict__['codes'] = codes
+            for part, c in zip(parts, codes):
+                part.__dict__['codes'] = c
             yield
         finally:
             for part in parts:

@@ -128,9 +128,9 @@ class Fp8Weight(object):
         return self.qt is not None or (self.ref is not None and self.ref[1] is not None)
 
 
-def fp8_weights(Ws):
+def fp8_weights(Ws, grad=True):
     """``Fp8Weight`` of every weight in ``Ws`` (None stays None), contiguous fp32 ones on the GPU 64 to a
-    launch: the ``codes`` of a whole encoder's layers for one forward."""
+    launch: the ``codes`` of a whole encoder's layers."""
     out, batch = [None] * len(Ws), []
     for i, W in enumerate(Ws):
         if W is None:
@@ -138,10 +138,10 @@ def fp8_weights(Ws):
         if use_kernels(W) and W.dim() == 2 and W.numel() and W.dtype == torch.float32 and W.is_contiguous() and W.data_ptr() % 16 == 0:
             batch.append(i)
         else:
-            out[i] = Fp8Weight(W)
+            out[i] = Fp8Weight(W, grad)
     for o in range(0, len(batch), 64):
         part = batch[o:o + 64]
-        for i, t in zip(part, C().split8_weights([Ws[j].detach() for j in part])):
+        for i, t in zip(part, C().split8_weights([Ws[j].detach() for j in part], bool(grad))):
             out[i] = Fp8Weight._of(Ws[i], *t)
     return out
 
@@ -320,22 +320,24 @@ def linear3_fp8(x, wq, wk, wv, bq, bk, bv, res_grad=None, bias_grad=True, codes=
     """``linear3`` on e4m3 operands: the Q / K / V projections as one product (N = 3H).  ``codes``: the
     ``Fp8Weight`` of the three weights stacked."""
     _check_act(x, 'linear3_fp8')
-    W = fused._adjacent_view([wq, wk, wv])
-    W = W if W is not None else torch.cat([wq.detach(), wk.detach(), wv.detach()], 0)
-    _check_weight(W, 'linear3_fp8')
-    if x.shape[-1] != W.shape[1] or x.device != W.device:
-        raise ValueError('linear3_fp8: x {} on {}, the weights take {} features on {}'.format(
-            tuple(x.shape), x.device, W.shape[1], W.device))
+    for W in (wq, wk, wv):
+        _check_weight(W, 'linear3_fp8')
+        if x.shape[-1] != W.shape[1] or x.device != W.device:
+            raise ValueError('linear3_fp8: x {} on {}, a weight takes {} features on {}'.format(
+                tuple(x.shape), x.device, W.shape[1], W.device))
+    shape = (wq.shape[0] + wk.shape[0] + wv.shape[0], x.shape[-1])
     bs, bias = (), None
     if bq is not None:
         bs, bias = (bq, bk, bv), fused._adjacent_view([bq, bk, bv])
         bias = bias if bias is not None else torch.cat([t.detach() for t in bs], 0)
-    _check_bias(bias, W.shape[0], x, 'linear3_fp8')
+    _check_bias(bias, shape[0], x, 'linear3_fp8')
     need = torch.is_grad_enabled() and x.requires_grad
     if codes is not None:
-        _check_codes(codes, tuple(W.shape), W.device, need, 'linear3_fp8')
-    w8 = codes if codes is not None else Fp8Weight(W, need)
-    return _LinearFp8Fn.apply(x, w8, bias, res_grad, bool(bias_grad), 3, wq, wk, wv, *bs)
+        _check_codes(codes, shape, x.device, need, 'linear3_fp8')
+    else:
+        W = fused._adjacent_view([wq, wk, wv])
+        codes = Fp8Weight(W if W is not None else torch.cat([wq.detach(), wk.detach(), wv.detach()], 0), need)
+    return _LinearFp8Fn.apply(x, codes, bias, res_grad, bool(bias_grad), 3, wq, wk, wv, *bs)
 
 
 # ---------------------------------------------------------------- bias + GELU with an int8 checkpoint

@@ -258,3 +258,31 @@ def test_encoder_reads_the_weights_it_has_now():
     assert not torch.equal(first, second)
     assert torch.equal(second, enc(x, mask, output_all_encoded_layers=False)[-1])
     assert all(p.codes is None for p in enc.modules() if hasattr(p, 'codes'))
+
+
+def test_kept_weights_serve_until_told_otherwise():
+    """keep_fp8_weights: the same outputs without gradients; the codes are those of the weights when they
+    were kept; a forward with gradients takes the weights as they are; checkpoints recompute with theirs."""
+    from hetseq_9cme_amd.models.bert import BertConfig, BertEncoder, BertLayer
+    torch.manual_seed(0)
+    enc = BertEncoder(BertConfig(64, hidden_size=64, num_hidden_layers=2, num_attention_heads=1, intermediate_size=128,
+                                 hidden_dropout_prob=0.0, attention_probs_dropout_prob=0.0))
+    for m in enc.modules():
+        if isinstance(m, BertLayer):
+            for part in (m.attention.self, m.attention.output, m.intermediate.dense_act, m.output):
+                part.fp8 = True
+    x, mask = torch.randn(2, 7, 64), torch.zeros(2, 7)
+    run = lambda **kw: enc(x, mask, output_all_encoded_layers=False, **kw)[-1]
+    with torch.no_grad():
+        first = run()
+        enc.keep_fp8_weights()
+        assert torch.equal(run(), first)
+        enc.layer[0].output.dense.weight.mul_(1.5)
+        assert torch.equal(run(), first)
+    now = run(checkpoint_activations=8)
+    assert not torch.equal(now, first)
+    now.sum().backward()
+    assert enc.layer[0].output.dense.weight.grad.abs().sum() > 0
+    with torch.no_grad():
+        enc.keep_fp8_weights(False)
+        assert torch.equal(run(), now)

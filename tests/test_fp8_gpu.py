@@ -501,6 +501,9 @@ def test_given_codes(dev):
             y = ops.linear_fp8(x, W, codes=c)
             res.append((y,) + torch.autograd.grad(y, (x, W), d))
         assert all(torch.equal(a, b) for a, b in zip(*res)), i
+    with torch.no_grad():
+        for a, b in zip(ops.fp8_weights(Ws, grad=False), codes):
+            assert a is b is None or (torch.equal(a.q, b.q) and not a.has_grad and b.has_grad)
     q = [(rand((128, 128), torch.float32, i) * 0.02).requires_grad_(True) for i in range(3)]
     x = rand((200, 128), torch.bfloat16, 1)
     c = ops.Fp8Weight(torch.cat(q))

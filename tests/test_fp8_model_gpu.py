@@ -131,7 +131,7 @@ def test_engine_updates(dev, tmp_path):
             f = getattr(ops.C(), name)
             if name != 'split8_weights':
                 return f
-            return lambda Ws: seen.append(len(Ws)) or split(Ws)
+            return lambda Ws, grad: seen.append(len(Ws)) or split(Ws, grad)
     old, fp8.C = fp8.C, lambda: Spy()
     try:
         for _ in range(3):
@@ -203,3 +203,29 @@ def test_graph_captured_updates_match_eager(dev, tmp_path):
     # other side of a rounding border then moves by an e4m3 step, as in two eager runs: the bound of the
     # bf16 engine (2e-3 of lr-sized updates) widened by the e4m3 step over the bf16 one, capped at 2 %
     _compare(eager, graph, 2e-2)
+
+
+def test_kept_weights_serve_captured_and_alone(dev):
+    """Serving with weights brought to 8 bits once: the outputs of a forward that makes its own codes, for a
+    batch and for one short sentence, and from a captured forward replayed on new inputs."""
+    enc = _encoder().eval()
+    with torch.no_grad():
+        ins = [_inputs()[:2], tuple(t[:1, :5].contiguous() for t in _inputs()[:2])]
+        ref = [enc(x, b, output_all_encoded_layers=False)[-1] for x, b in ins]
+        enc.keep_fp8_weights()
+        for (x, b), r in zip(ins, ref):
+            assert torch.equal(enc(x, b, output_all_encoded_layers=False)[-1], r)
+        x, b = ins[0]
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            enc(x, b, output_all_encoded_layers=False)
+        torch.cuda.current_stream().wait_stream(st)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = enc(x, b, output_all_encoded_layers=False)[-1]
+        for i in range(3):
+            x.copy_(torch.randn(x.shape, generator=torch.Generator(device='cuda').manual_seed(i), device=dev))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, enc(x, b, output_all_encoded_layers=False)[-1]), i
