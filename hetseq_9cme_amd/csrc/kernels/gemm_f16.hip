@@ -1713,8 +1713,17 @@ __global__ __launch_bounds__(256) void amax_cols_k(const float* __restrict__ x, 
   }
 }
 
+// Cleared by a kernel: callers are captured into graphs, whose replays have run memset nodes out of order
+// with the kernels after them (a replayed forward then scaled its weights by the wrong maxima).
+__global__ __launch_bounds__(256) void clear_k(float* p, int64_t n) {
+  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) p[i] = 0.f;
+}
+static void clear_floats(float* p, int64_t n, hipStream_t s) {
+  if (n > 0) clear_k<<<(unsigned)std::min<int64_t>((n + 255) / 256, 1024), 256, 0, s>>>(p, n);
+}
+
 void hx_amax_cols(const float* x, int64_t rows, int cols, int64_t ld, float* out, hipStream_t s) {
-  (void)hipMemsetAsync(out, 0, (size_t)cols * 4, s);
+  clear_floats(out, cols, s);
   if (rows < 1) return;
   const int cb = (cols / 4 + 63) / 64;
   // ~4 workgroups per CU over the row slabs
@@ -1785,7 +1794,7 @@ __global__ __launch_bounds__(256) void amax_rows_cols_k(const float* __restrict_
 int hx_amax_rows_cols(const float* x, int64_t rows, int cols, int64_t ld, float* rowmax, float* colmax,
                       hipStream_t s) {
   if (cols % 4 || cols > 4 * 64 * kRcMaxQ) return -1;
-  (void)hipMemsetAsync(colmax, 0, (size_t)cols * 4, s);
+  clear_floats(colmax, cols, s);
   if (rows < 1) return 0;
   amax_rows_cols_k<<<(unsigned)((rows + kRcRows - 1) / kRcRows), 256, (size_t)cols * 16, s>>>(x, rows, cols, ld,
                                                                                               rowmax, colmax);
@@ -1799,7 +1808,7 @@ void hx_amax_rows(const float* x, int64_t rows, int cols, int64_t ld, float* out
 
 void hx_split_weight_f16(const HxWeightBatch& d, float* rc, int64_t rc_floats, hipStream_t s) {
   if (d.n < 1) return;
-  (void)hipMemsetAsync(rc, 0, (size_t)rc_floats * 4, s);
+  clear_floats(rc, rc_floats, s);
   amax_weights_k<<<d.start[d.n], 256, 0, s>>>(d, rc);
   split_weight_f16_k<<<d.start[d.n], 256, 0, s>>>(d, rc);
 }
