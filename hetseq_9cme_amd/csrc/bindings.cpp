@@ -945,30 +945,51 @@ Tensor gemm_fp8(Tensor a, Tensor as, Tensor b, Tensor bs, int64_t K, bool out_bf
   return out;
 }
 
+// codes and scale words of an operand [rows, n] inside a workspace
+struct Codes8 {
+  int64_t rows, n, qb, sb;   // bytes of the codes and of the scale words, 256-B steps
+  Codes8(int64_t rows_, int64_t n_, bool on = true)
+      : rows(rows_), n(n_), qb(on ? up256(rows_ * blocks128(n_) * 128) : 0), sb(on ? up256((blocks128(n_) + 3) / 4 * ((rows_ + 3) / 4) * 16) : 0) {}
+  int64_t bytes() const { return qb + sb; }
+  uint8_t* q(uint8_t* base) const { return bytes() ? base : nullptr; }
+  uint8_t* s(uint8_t* base) const { return bytes() ? base + qb : nullptr; }
+};
+
 // x [M, K] W^T (+ bias) from W's codes; with `keep`, also x's codes blocked along the rows (the weight
 // gradient's operand).  Few rows that need no such copy go through one launch (fp8_rows_k).
 static Tensor linear_fp8_y(const Tensor& x2, const Tensor& wq, const Tensor& ws, const OptT& bias, bool keep, OptT* qt, OptT* st) {
   const int64_t M = x2.size(0), K = x2.size(1), N = wq.size(0);
-  if (!keep && hx_fp8_rows_fit(M, blocks128(K), act_bf16(x2))) {
+  if (!keep && M > 0) {
     check_rows8(x2, "linear_fp8");
     TORCH_CHECK(wq.is_cuda() && wq.device() == x2.device() && wq.size(1) == blocks128(K) * 128 && wq.is_contiguous() && aligned16(wq.data_ptr()) &&
                     ws.numel() == (blocks128(K) + 3) / 4 * ((N + 3) / 4 * 4) * 4, "linear_fp8: the weight's codes do not fit x");
     check_bias8(bias, N, x2, "linear_fp8 bias");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(x2.device());
+    const int bf16 = act_bf16(x2);
     Tensor y = torch::empty({M, N}, x2.options());
-    HxRows8 g{};
-    g.x = x2.data_ptr();
-    g.ldx = M > 1 ? x2.stride(0) : K;
-    g.B = wq.data_ptr<uint8_t>();
-    g.ldb = wq.size(1);
-    g.sb = reinterpret_cast<const uint32_t*>(ws.data_ptr());
-    g.y = y.data_ptr();
-    g.bias = ptr_or_null<float>(bias);
-    g.M = (int)M;
-    g.N = (int)N;
-    g.K = (int)K;
-    g.nkb = (int)blocks128(K);
-    TORCH_CHECK(hx_fp8_rows(g, act_bf16(x2), cur_stream(x2)) == 0, "linear_fp8: launch failed");
+    if (hx_fp8_rows_fit(M, blocks128(K), bf16)) {
+      HxRows8 g{};
+      g.x = x2.data_ptr();
+      g.ldx = M > 1 ? x2.stride(0) : K;
+      g.B = wq.data_ptr<uint8_t>();
+      g.ldb = wq.size(1);
+      g.sb = reinterpret_cast<const uint32_t*>(ws.data_ptr());
+      g.y = y.data_ptr();
+      g.bias = ptr_or_null<float>(bias);
+      g.M = (int)M;
+      g.N = (int)N;
+      g.K = (int)K;
+      g.nkb = (int)blocks128(K);
+      TORCH_CHECK(hx_fp8_rows(g, bf16, cur_stream(x2)) == 0, "linear_fp8: launch failed");
+    } else {
+      const Plan8 plan(M, N, K, bf16);
+      const Codes8 cx(M, K);
+      const Scratch8 tmp(cx.bytes() + plan.bytes);
+      uint8_t* px = tmp.get();
+      const HxSplit8 job = split8_job(x2, cx.q(px), cx.s(px), nullptr, nullptr, nullptr);
+      hx_split8(&job, 1, cur_stream(x2));
+      gemm8_run(plan, px + cx.bytes(), cx.q(px), cx.s(px), M, wq.data_ptr<uint8_t>(), ws.data_ptr<uint8_t>(), N, K, y, false, ptr_or_null<float>(bias));
+    }
     dbg_finite(y, "linear_fp8");
     return y;
   }
@@ -992,16 +1013,6 @@ std::vector<OptT> linear_fp8_fwd(Tensor x2, Tensor wq, Tensor ws, OptT bias, boo
   Tensor y = linear_fp8_y(x2, wq, ws, bias, keep, &qt, &st);
   return {y, qt, st};
 }
-
-// codes and scale words of an operand [rows, n] inside a workspace
-struct Codes8 {
-  int64_t rows, n, qb, sb;   // bytes of the codes and of the scale words, 256-B steps
-  Codes8(int64_t rows_, int64_t n_, bool on = true)
-      : rows(rows_), n(n_), qb(on ? up256(rows_ * blocks128(n_) * 128) : 0), sb(on ? up256((blocks128(n_) + 3) / 4 * ((rows_ + 3) / 4) * 16) : 0) {}
-  int64_t bytes() const { return qb + sb; }
-  uint8_t* q(uint8_t* base) const { return bytes() ? base : nullptr; }
-  uint8_t* s(uint8_t* base) const { return bytes() ? base + qb : nullptr; }
-};
 
 // A gradient that is captured into a graph for a leaf whose accumulator was made on another stream (an
 // eager graph of the same leaf is alive): autograd would make that stream wait for the capturing one,
