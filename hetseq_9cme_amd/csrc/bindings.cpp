@@ -956,7 +956,7 @@ struct Codes8 {
 };
 
 // x [M, K] W^T (+ bias) from W's codes; with `keep`, also x's codes blocked along the rows (the weight
-// gradient's operand).  Few rows that need no such copy go through one launch (fp8_rows_k).
+// gradient's operand).  Small products that need no such copy go through one launch (fp8_rows_k).
 static Tensor linear_fp8_y(const Tensor& x2, const Tensor& wq, const Tensor& ws, const OptT& bias, bool keep, OptT* qt, OptT* st) {
   const int64_t M = x2.size(0), K = x2.size(1), N = wq.size(0);
   if (!keep && M > 0) {
@@ -967,7 +967,7 @@ static Tensor linear_fp8_y(const Tensor& x2, const Tensor& wq, const Tensor& ws,
     c10::hip::HIPGuardMasqueradingAsCUDA guard(x2.device());
     const int bf16 = act_bf16(x2);
     Tensor y = torch::empty({M, N}, x2.options());
-    if (hx_fp8_rows_fit(M, blocks128(K), bf16)) {
+    if (hx_fp8_rows_fit(M, N, blocks128(K), bf16)) {
       HxRows8 g{};
       g.x = x2.data_ptr();
       g.ldx = M > 1 ? x2.stride(0) : K;

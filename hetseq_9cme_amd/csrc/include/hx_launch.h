@@ -318,5 +318,5 @@ struct HxRows8 {
   const float* bias;
   int M, N, K, nkb;
 };
-int hx_fp8_rows_fit(int64_t M, int64_t nkb, int bf16);   // rows and k blocks it is the faster way for (M <= 64)
+int hx_fp8_rows_fit(int64_t M, int64_t N, int64_t nkb, int bf16);   // sizes that it is the faster way for
 int hx_fp8_rows(const HxRows8& g, int bf16, hipStream_t s);

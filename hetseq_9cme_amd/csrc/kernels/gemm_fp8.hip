@@ -446,14 +446,14 @@ __global__ __launch_bounds__(256) void fp8_finish_k(HxFinish f) {
 }
 
 // ---------------------------------------------------------------- few rows
-// y = Q(x) W^T (+ bias) for up to 16 MB MG rows of unquantised x, in one launch: 16 output features per
-// workgroup, the k blocks dealt over its waves (and groups of 16 MB rows over MG sets of them).  A wave
-// reads its W codes straight into registers (32 B of a row per lane: a whole 128-B line per row), rounds
-// its 32 x values per lane and row block to e4m3 (the block's maximum is 4 lanes), runs both through
-// exact bf16 MFMAs, and the waves' sums are added in LDS in wave order.  Bound by latency (one token
-// through 768 x 2304: 1.8 MB of codes, 3.6 us; 41 rows through 1024 x 1024: 6.9 us, most of it one wave's
-// chain of load, maximum, rounding and products): splitting the reduction inside the workgroup keeps up to
-// 16 waves of loads in flight where a tile per wave would leave one.
+// y = Q(x) W^T (+ bias) of unquantised x, in one launch: 16 rows and 16 output features per workgroup, the k
+// blocks dealt over its waves.  A wave reads its W codes straight into registers (32 B of a row per lane: a
+// whole 128-B line per row), rounds its 32 x values per lane to e4m3 (the block's maximum is 4 lanes), runs
+// both through exact bf16 MFMAs, and the waves' sums are added in LDS in wave order.  Bound by latency (one
+// token through 768 x 2304: 1.8 MB of codes, 3.5 us; 41 rows through 1024 x 1024: 3.7) and, as rows are
+// added, by the rounding, which every workgroup does for itself: groups of rows in one workgroup share the W
+// codes but leave CUs idle (41 rows, 64 workgroups of 16 waves: 6.9 us).  Splitting the reduction inside
+// the workgroup keeps up to 16 waves of loads in flight where a tile per wave would leave one.
 template <typename T>
 struct Row32;   // 32 consecutive values of a row, of which n are inside
 template <>
@@ -506,18 +506,15 @@ struct Row32<uint16_t> {
   __device__ uint32_t code(int j, float s) const { return hx::q8::e4m3x4(w[2 * j], w[2 * j + 1], s); }
 };
 
-template <typename T, int MB, int MG>
+template <typename T>
 __global__ __launch_bounds__(1024) void fp8_rows_k(HxRows8 g) {
-  __shared__ float red[16][MB][256];   // a wave's sums
-  const int nw = blockDim.x / 64, nk = nw / MG;   // waves; of them along k
+  __shared__ float red[16][256];   // a wave's sums
+  const int nk = blockDim.x / 64;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, h = lane >> 4;
-  const int wk = MG == 1 ? wv : wv / MG, r0 = MG == 1 ? 0 : wv % MG * (16 * MB);
-  const int n0 = blockIdx.x * 16, n = n0 + l16;
+  const int n0 = blockIdx.x * 16, n = n0 + l16, r0 = blockIdx.y * 16, r = r0 + l16;
   const int64_t sbn = (g.N + 3) & ~3;
-  f32x4 acc[MB];
-#pragma unroll
-  for (int m = 0; m < MB; ++m) acc[m] = f32x4{0, 0, 0, 0};
-  for (int kb = wk; kb < g.nkb; kb += nk) {
+  f32x4 acc = {0, 0, 0, 0};
+  for (int kb = wv; kb < g.nkb; kb += nk) {
     const int k0 = kb * 128 + 32 * h;
     uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
     uint32_t sw = 0x7f7f7f7fu;
@@ -527,49 +524,40 @@ __global__ __launch_bounds__(1024) void fp8_rows_k(HxRows8 g) {
       w1 = p[1];
       sw = g.sb[(kb >> 2) * sbn + n];
     }
-    Row32<T> x[MB];
-#pragma unroll
-    for (int m = 0; m < MB; ++m) {
-      const int r = r0 + 16 * m + l16;
-      x[m].load((const T*)g.x + (int64_t)r * g.ldx + k0, r < g.M ? g.K - k0 : 0);
-    }
+    Row32<T> x;
+    x.load((const T*)g.x + (int64_t)r * g.ldx + k0, r < g.M ? g.K - k0 : 0);
     const float ws = hx::q8::scale_of((sw >> (8 * (kb & 3))) & 0xffu);
     const uint32_t wc[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
     bf16x8v wd[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) wd[q] = decode8(wc[2 * q], wc[2 * q + 1], ws);
+    uint32_t a = x.top();
+    a = max(a, (uint32_t)__shfl_xor((int)a, 16, 64));
+    a = max(a, (uint32_t)__shfl_xor((int)a, 32, 64));
+    if (__builtin_expect(a >= 0x7f800000u, 0)) {   // something not finite (the row's 4 lanes agree): the maximum of the rest
+      a = 0;
 #pragma unroll
-    for (int m = 0; m < MB; ++m) {
-      if (r0 + 16 * m >= g.M) break;   // (uniform over the wave)
-      uint32_t a = x[m].top();
+      for (int i = 0; i < 32; ++i) a = max(a, __float_as_uint(hx::q8::finite_abs(x.at(i))));
       a = max(a, (uint32_t)__shfl_xor((int)a, 16, 64));
       a = max(a, (uint32_t)__shfl_xor((int)a, 32, 64));
-      if (__builtin_expect(a >= 0x7f800000u, 0)) {   // something not finite: the maximum of the rest
-        a = 0;
+    }
+    const float xs = hx::q8::exp2i(hx::q8::block_exp<hx::q8::E4M3>(__uint_as_float(a)));
 #pragma unroll
-        for (int i = 0; i < 32; ++i) a = max(a, __float_as_uint(hx::q8::finite_abs(x[m].at(i))));
-        a = max(a, (uint32_t)__shfl_xor((int)a, 16, 64));
-        a = max(a, (uint32_t)__shfl_xor((int)a, 32, 64));
-      }
-      const float xs = hx::q8::exp2i(hx::q8::block_exp<hx::q8::E4M3>(__uint_as_float(a)));
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const bf16x8v xd = decode8((int)x[m].code(2 * q, xs), (int)x[m].code(2 * q + 1, xs), xs);
-        acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wd[q], xd, acc[m], 0, 0, 0);
-      }
+    for (int q = 0; q < 4; ++q) {
+      const bf16x8v xd = decode8((int)x.code(2 * q, xs), (int)x.code(2 * q + 1, xs), xs);
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wd[q], xd, acc, 0, 0, 0);
     }
   }
-#pragma unroll
-  for (int m = 0; m < MB; ++m) *reinterpret_cast<f32x4*>(&red[wv][m][4 * lane]) = acc[m];
+  *reinterpret_cast<f32x4*>(&red[wv][4 * lane]) = acc;
   __syncthreads();
-  for (int t = threadIdx.x; t < 256 * MB * MG; t += blockDim.x) {
-    const int mg = t / (256 * MB), m = t / 256 % MB, e = t & 255;   // element e of a 16 x 16 block: lane e / 4, register e % 4
+  const int e = threadIdx.x;   // element e of the 16 x 16 block: lane e / 4, register e % 4
+  if (e < 256) {
     float v = 0.f;
-    for (int k = 0; k < nk; ++k) v += red[k * MG + mg][m][e];
-    const int r = 16 * (mg * MB + m) + ((e >> 2) & 15), c = n0 + 4 * (e >> 6) + (e & 3);
-    if (r < g.M && c < g.N) {
+    for (int k = 0; k < nk; ++k) v += red[k][e];
+    const int rr = r0 + ((e >> 2) & 15), c = n0 + 4 * (e >> 6) + (e & 3);
+    if (rr < g.M && c < g.N) {
       if (g.bias) v += g.bias[c];
-      hx::io<T>::st((T*)g.y + (int64_t)r * g.N + c, v);
+      hx::io<T>::st((T*)g.y + (int64_t)rr * g.N + c, v);
     }
   }
 }
@@ -649,26 +637,20 @@ void hx_gemm_fp8_plan(int M, int N, int nkb, int exact, int* cfg, int* ks) {
   }
 }
 
-// Whether fp8_rows_k takes the product: every workgroup rounds all of x, so its time grows with the 16 x 128
-// blocks of x (split8 and gemm_fp8_k, two launches: 9 - 14 us whatever the rows).  bf16, us here / there:
-// 1 x 4096 x 1024 6.9 / 11.8, 41 x 1024 x 1024 6.9 / 9.8, 64 x 2048 x 1024 11.4 / 11.6, 64 x 4096 x 1024 21 / 13.6;
-// fp32: 41 x 1024 x 1024 8.2 / 10.5, 64 x 1024 x 1024 10.6 / 10.5, 32 x 4096 x 1024 21 / 13.4.
-int hx_fp8_rows_fit(int64_t M, int64_t nkb, int bf16) { return M >= 1 && M <= 64 && (M + 15) / 16 * nkb <= (bf16 ? 64 : 32); }
+// Whether fp8_rows_k takes the product: its time grows with the 16 x 16 x 128 blocks of work, and with the depth
+// (16 waves take it by turns); split8 and gemm_fp8_k, two launches, are 8 - 14 us at these sizes.  bf16, us here /
+// there: 1 x 4096 x 1024 7.1 / 12.1, 100 x 768 x 768 4.6 / 9.0, 256 x 1024 x 1024 (8192 blocks) 8.0 / 10.1, 512 x 768 x 768 (9216) 9.8 /
+// 9.4, 1 x 16384 x 1024 20 / 17; fp32: 256 x 768 x 768 (4608) 7.6 / 9.5, 128 x 768 x 2304 (6912) 11.0 / 9.8.
+int hx_fp8_rows_fit(int64_t M, int64_t N, int64_t nkb, int bf16) {
+  return nkb <= 64 && (M + 15) / 16 * ((N + 15) / 16) * nkb <= (bf16 ? 8192 : 5632);
+}
 
 int hx_fp8_rows(const HxRows8& g, int bf16, hipStream_t s) {
-  const unsigned grid = (unsigned)((g.N + 15) / 16);
-  if (g.M < 1 || g.M > 64) return 1;
-  // two sets of waves over the rows where there are more than 16; 16 waves where the k blocks keep them busy
-  const unsigned nt = g.M > 16 || g.nkb > 8 ? 1024 : 512;
-  if (bf16) {
-    if (g.M <= 16) fp8_rows_k<uint16_t, 1, 1><<<grid, nt, 0, s>>>(g);
-    else if (g.M <= 32) fp8_rows_k<uint16_t, 1, 2><<<grid, nt, 0, s>>>(g);
-    else fp8_rows_k<uint16_t, 2, 2><<<grid, nt, 0, s>>>(g);
-  } else {
-    if (g.M <= 16) fp8_rows_k<float, 1, 1><<<grid, nt, 0, s>>>(g);
-    else if (g.M <= 32) fp8_rows_k<float, 1, 2><<<grid, nt, 0, s>>>(g);
-    else fp8_rows_k<float, 2, 2><<<grid, nt, 0, s>>>(g);
-  }
+  if (g.M < 1 || g.M > 65535 * 16) return 1;   // (grid)
+  const dim3 grid((unsigned)((g.N + 15) / 16), (unsigned)((g.M + 15) / 16));
+  const unsigned nt = g.nkb > 8 ? 1024 : 512;   // waves that the k blocks keep busy
+  if (bf16) fp8_rows_k<uint16_t><<<grid, nt, 0, s>>>(g);
+  else fp8_rows_k<float><<<grid, nt, 0, s>>>(g);
   return 0;
 }
 

@@ -158,7 +158,8 @@ def test_linear_fp8(dev, M, K, N, dt):
 
 @pytest.mark.parametrize('dt', ['fp32', 'bf16'])
 @pytest.mark.parametrize('M,K,N', [(1, 768, 2304), (5, 130, 33), (33, 1024, 1001), (64, 4096, 128), (129, 96, 64), (3000, 256, 512),
-                                   (1, 8192, 40), (16, 4096, 33), (17, 2050, 16), (32, 1000, 50), (33, 2048, 31), (48, 300, 96), (49, 129, 5), (64, 2048, 48)])
+                                   (1, 8192, 40), (16, 4096, 33), (17, 2050, 16), (32, 1000, 50), (33, 2048, 31), (48, 300, 96), (49, 129, 5), (64, 2048, 48),
+                                   (1, 9000, 40), (200, 768, 770), (257, 1000, 1030), (512, 256, 256), (600, 130, 1001), (4000, 100, 30)])
 def test_linear_fp8_kept_weight(dev, M, K, N, dt):
     x, W, b = rand((M, K), DT[dt], 1), rand((N, K), torch.float32, 2) * 0.02, rand((N,), torch.float32, 3)
     w8 = ops.Fp8Weight(W, grad=False)
