@@ -74,8 +74,11 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) *
   static_assert((KA + KB) % NW == 0, "whole DMA pieces per wave");
   static_assert(BM <= 256 && BN <= 256 && NW >= 3, "one DMA piece of scale words per operand");
   // LDS: two stages, two slots of scale words (A 1 KiB, B 1 KiB; one word = 4 k blocks of a row), the
-  // biases of two tiles, and where idle DMA pieces land
-  constexpr int STAGE = (BM + BN) * 128, SCALES = 2 * STAGE, BIAS = SCALES + 4096, SPARE = BIAS + 2048;
+  // biases of three tiles, and where idle DMA pieces land.  Tile i's bias lies in slot i % 3.  It is fetched
+  // in tile i - 1, of up to 4 k blocks before that tile's first barrier, when a slower wave may still be
+  // reading the bias of tile i - 2 in its epilogue: two slots would give it tile i's.  The slot's tile before,
+  // i - 3, was read by every wave before the barriers of tile i - 2.
+  constexpr int STAGE = (BM + BN) * 128, SCALES = 2 * STAGE, BIAS = SCALES + 4096, SPARE = BIAS + 3072;
   constexpr int STORES = MB * NB * (OB ? 2 : 4);   // of a lane in the epilogue
   static_assert(STORES < 63, "counted by vmcnt");
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -348,7 +351,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) *
         read_scales(gslot);
         gslot ^= 1;
         const bool here = kb + 4 < t.n;
-        dma_scales(pick(here, src.x, nxt.x), here ? src.so : nxt.so, here ? (kb >> 2) + 1 : 0, gslot, tslot ^ 1);
+        dma_scales(pick(here, src.x, nxt.x), here ? src.so : nxt.so, here ? (kb >> 2) + 1 : 0, gslot, tslot == 2 ? 0 : tslot + 1);
       } else {
 #pragma unroll
         for (int a = 0; a < MB; ++a) wa[a] >>= 8;
@@ -366,7 +369,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) *
     store(t, tslot);
     if (!more) break;
     w += step;
-    tslot ^= 1;
+    tslot = tslot == 2 ? 0 : tslot + 1;
     t = u;
     src = nxt;
     more = w + step < end;
@@ -565,7 +568,7 @@ __global__ __launch_bounds__(1024) void fp8_rows_k(HxRows8 g) {
 template <int BM, int BN, int WM, int WN, int WGS, bool EXACT, bool OB>
 int launch(const HxGemm8& g, hipStream_t s) {
   constexpr int NT = (BM / WM) * (BN / WN) * 64;
-  constexpr int LDS = 2 * (BM + BN) * 128 + 4096 + 2048 + 1024;   // stages, scale words, biases, spare
+  constexpr int LDS = 2 * (BM + BN) * 128 + 4096 + 3072 + 1024;   // stages, scale words, biases, spare
   auto k = gemm_fp8_k<BM, BN, WM, WN, WGS, EXACT, OB>;
   static std::atomic<uint64_t> allowed{0};   // devices on which the kernel may take this much LDS
   int dev = 0;

@@ -660,3 +660,48 @@ def test_inference_refusals(dev):
                 ops.linear_fp8(x, w8)
         finally:
             ops.set_fused(True)
+
+
+# ---------------------------------------------------------------- several tiles per workgroup
+def assert_biased(y, x8, w8, b):
+    """y = x8 w8^T + b for exact operand values, the bias held to its own rounding: half a step of the result
+    (fp32: and the rounding of each of K / 16 + 8 sums; bf16: and 2^-11 of sum |x8||w8|)."""
+    prod, mag = x8 @ w8.t(), x8.abs() @ w8.abs().t()
+    ref = prod + b.double()
+    if y.dtype == torch.float32:
+        tol = (x8.shape[1] / 16 + 8) * 2.0 ** -23 * (mag + b.double().abs())
+    else:
+        tol = HALF[y.dtype] * ref.abs() + 2.0 ** -11 * mag * (1 + 2.0 ** -8) + 2.0 ** -22 * b.double().abs()
+    bad = (y.double() - ref).abs() > tol
+    assert not bad.any(), bad.nonzero()[:4].tolist()
+
+
+@pytest.mark.parametrize('dt', ['fp32', 'bf16'])
+@pytest.mark.parametrize('M,K,N', [(16384, 512, 2048), (16384, 512, 1536), (16390, 130, 2050), (8200, 256, 4097), (16384, 384, 2304),
+                                   (20000, 640, 1100), (4100, 256, 1030), (33000, 250, 600), (16384, 512, 2304)])
+def test_bias_where_a_workgroup_takes_several_tiles(dev, M, K, N, dt):
+    """2 .. 5 blocks deep, more tiles than the chip holds at a time, a bias 4 .. 40 apart from one 64 columns to the
+    next: every tile has its own bias, on a kept weight and in training, again and again."""
+    x, W = rand((M, K), DT[dt], 1, 0.5), rand((N, K), torch.float32, 2, 0.5) * 0.02
+    n = torch.arange(N, device=dev)
+    b = (4.0 * ((n // 64 * 3) % 11 - 5) + (n % 64) / 64).float()
+    x8, w8 = e4m3(x), e4m3(W)
+    kept = ops.Fp8Weight(W, grad=False)
+    with torch.no_grad():
+        y = ops.linear_fp8(x, kept, b)
+        assert_biased(y, x8, w8, b)
+        for _ in range(4):
+            assert torch.equal(ops.linear_fp8(x, kept, b), y)
+    assert torch.equal(ops.linear_fp8(x, W.requires_grad_(True), b), y)
+
+
+def test_linear3_bias_where_a_workgroup_takes_several_tiles(dev):
+    x = rand((32768, 512), torch.bfloat16, 1, 0.5)
+    ws = [(rand((512, 512), torch.float32, 2 + i, 0.5) * 0.02).requires_grad_(True) for i in range(3)]
+    n = torch.arange(1536, device=dev)
+    b = (4.0 * ((n // 64 * 3) % 11 - 5) + (n % 64) / 64).float()
+    bs = [t.clone().requires_grad_(True) for t in b.split(512)]
+    with torch.no_grad():
+        W8 = e4m3(torch.cat(ws))
+    for _ in range(2):
+        assert_biased(ops.linear3_fp8(x, *ws, *bs).detach(), e4m3(x), W8, b)
