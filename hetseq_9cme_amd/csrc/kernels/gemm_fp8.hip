@@ -8,10 +8,12 @@
 //
 // Two ways through the matrix cores:
 //  * fast: v_mfma_scale_f32_32x32x64_f8f6f4 on the codes, the block scales as its E8M0 operands (no
-//    vector instruction at all for the scaling).  The instruction keeps about 16 bits below the
-//    largest product of a small group: relative error 1.5e-5 (normal data) to 3e-5 (spread over
-//    decades) of the result, whatever the depth -- 1/100 of a bf16 rounding, so it carries every
-//    product whose result is rounded to bf16.
+//    vector instruction at all for the scaling).  The instruction sums 8 consecutive products at a time
+//    and cuts each of them, towards zero, at 2^-13 of the largest 2^(ea + eb) among the 8 (ea, eb: the
+//    codes' exponents); the sums of 8 are added in fp32.  That is 1.3e-5 (normal data) to 6e-5 (widths spread
+//    over decades) of a result in the mean, whatever the depth -- 1/300 to 1/65 of half a bf16 step, so it
+//    carries every product whose result is rounded to bf16 -- and, for codes that are not subnormal, at most
+//    2^-10 of sum |a||b|.
 //  * exact: the codes decoded to bf16 with their scale (v_cvt_scalef32_pk_bf16_fp8, exact) after the
 //    LDS read, and v_mfma_f32_32x32x16_bf16, which sums exact products in fp32 (1e-7): the products
 //    whose result is kept in fp32 (weight gradients, fp32 activations).  Half the matrix rate, and a

@@ -705,3 +705,43 @@ def test_linear3_bias_where_a_workgroup_takes_several_tiles(dev):
         W8 = e4m3(torch.cat(ws))
     for _ in range(2):
         assert_biased(ops.linear3_fp8(x, *ws, *bs).detach(), e4m3(x), W8, b)
+
+
+# ---------------------------------------------------------------- the e4m3 instruction's own rounding
+def cut_steps(x, w):
+    """x [K], w [N, K] -> what the e4m3 instruction's sums may cut off, per product (64 bits): of 8 consecutive
+    products each is cut towards zero at 2^-13 of the largest 2^(ea + eb) among them (ea, eb: the exponents
+    of the codes, at least -6), so by less than that step, and at most by all of it."""
+    def exps(t):
+        v, s = scaled(t, 448.0)
+        q = (e4m3(t) / s).abs()
+        return torch.frexp(q.clamp(min=2.0 ** -6))[1] - 1, torch.log2(s).long()
+    (ea, sa), (eb, sb) = exps(x[None]), exps(w)
+    step = (ea + eb + sa + sb).double()
+    N, K = w.shape
+    step = torch.nn.functional.pad(step, (0, -K % 8), value=-1e4).view(N, -1, 8).amax(-1).repeat_interleave(8, 1)[:, :K]
+    return torch.minimum(torch.exp2(step - 13), (e4m3(x[None]) * e4m3(w)).abs()), torch.exp2(step - 13)
+
+
+@pytest.mark.parametrize('spread', [0.0, 0.8, 2.5])
+@pytest.mark.parametrize('M,K,N', [(4096, 130, 512), (600, 1024, 512), (640, 4096, 520)])
+def test_e4m3_sums_lose_what_the_instruction_cuts(dev, M, K, N, spread):
+    """A bias of minus the exact product leaves the error of the products alone.  Each result within the sum of its
+    products' cuts (and fp32 sums: 9 terms a step of 64, each to 2^-24 of sum |a||b|); over the columns the mean square no
+    more than that of cuts spread evenly over a step with signs at random, 1/3 of a step squared (512 columns: 5
+    standard deviations are 0.31).  The bound is 2^-11 .. 2^-10 of sum |a||b|, the mean 1e-5 .. 6e-5 of a result."""
+    x = rand((1, K), torch.bfloat16, 1, spread)
+    W = rand((N, K), torch.float32, 2, spread) * 0.02
+    a, w = e4m3(x)[0], e4m3(W)
+    ref, mag = w @ a, w.abs() @ a.abs()
+    b = (-ref).float()
+    with torch.no_grad():
+        y = ops.linear_fp8(x.expand(M, K).contiguous(), ops.Fp8Weight(W, grad=False), b).double()
+    assert torch.equal(y, y[:1].expand_as(y))
+    err = y[0] - (ref + b.double())
+    cut, step = cut_steps(x[0], W)
+    fp32 = (K / 8 + 8) * 2.0 ** -24 * mag + 2.0 ** -23 * ref.abs()
+    assert (err.abs() <= (cut.sum(1) + fp32) * (1 + 2.0 ** -8)).all()
+    # fp32: K / 64 + 8 roundings to 2^-24 of a running sum, itself about the root of sum (a b)^2, twice that allowed
+    var = torch.where(cut < step, cut ** 2, step ** 2 / 3).sum(1) + (K / 64 + 8) * 2.0 ** -46 * (w * a).square().sum(1)
+    assert (err ** 2 / var).mean() <= 1.31 * (1 + 2.0 ** -7)
