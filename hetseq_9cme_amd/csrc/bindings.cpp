@@ -1029,6 +1029,9 @@ static void refuse_stale_leaves(const Tensor& like, const std::string& what) {
                 ": a captured backward needs its leaves' eager graphs released first (one of them lives on another stream)");
   }
 }
+static void refuse_tangent(const OptT& t, const char* what) {
+  TORCH_CHECK(!has(t) || !t->_fw_grad(/*level=*/0).defined(), what, ": no forward-mode derivatives (an argument is a dual tensor)");
+}
 static void refuse_second_derivative(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": first derivatives only (create_graph=True is not supported)");
 }
@@ -1165,6 +1168,8 @@ Tensor linear_fp8_infer(Tensor x, Tensor wq, Tensor ws, int64_t K, OptT b) {
     TORCH_CHECK_VALUE(b->scalar_type() == torch::kFloat32 && b->dim() == 1 && b->size(0) == wq.size(0) && b->device() == x.device(),
                       "linear_fp8: the bias must be fp32 [", wq.size(0), "] on ", x.device(), ", got ", b->scalar_type(), " ", b->sizes(),
                       " on ", b->device());
+  refuse_tangent(x, "linear_fp8");
+  refuse_tangent(b, "linear_fp8");
   at::NoGradGuard no_grad;
   if (x.dim() == 2 && x.is_contiguous()) return linear_fp8_y(x, wq, ws, b, false, nullptr, nullptr);
   std::vector<int64_t> shape = x.sizes().vec();

@@ -28,6 +28,7 @@ Sites of the reference model: hetseq/bert_modeling.py:104-116 (bias_gelu), :334-
 (linear layers), :428-446 (checkpointed segments).
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import fused
 from ._ext import C, use_kernels
@@ -36,11 +37,19 @@ BLOCK = 128
 _DTYPES = (torch.float32, torch.bfloat16)
 
 
-def _check_act(x, what):
+def _refuse_tangents(what, *ts):
+    for t in ts:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError('{}: no forward-mode derivatives (an argument is a dual tensor)'.format(what))
+
+
+def _check_act(x, what, tangents=False):
     if not torch.is_tensor(x) or x.dtype not in _DTYPES:
         raise TypeError('{}: an fp32 or bf16 tensor, got {}'.format(what, getattr(x, 'dtype', type(x).__name__)))
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError('{}: needs a last dimension of at least 1, got shape {}'.format(what, tuple(x.shape)))
+    if not tangents:
+        _refuse_tangents(what, x)
 
 
 def _check_weight(W, what):
@@ -55,6 +64,7 @@ def _check_bias(b, n, like, what):
     if b.dtype != torch.float32 or tuple(b.shape) != (n,) or b.device != like.device:
         raise ValueError('{}: the bias must be fp32 [{}] on {}, got {} {} on {}'.format(
             what, n, like.device, b.dtype, tuple(b.shape), b.device))
+    _refuse_tangents(what, b)
 
 
 def _backward_checks(what, dy):
@@ -135,6 +145,7 @@ def fp8_weights(Ws, grad=True):
     for i, W in enumerate(Ws):
         if W is None:
             continue
+        _refuse_tangents('fp8_weights', W)
         if use_kernels(W) and W.dim() == 2 and W.numel() and W.dtype == torch.float32 and W.is_contiguous() and W.data_ptr() % 16 == 0:
             batch.append(i)
         else:
@@ -328,6 +339,7 @@ def linear3_fp8(x, wq, wk, wv, bq, bk, bv, res_grad=None, bias_grad=True, codes=
     shape = (wq.shape[0] + wk.shape[0] + wv.shape[0], x.shape[-1])
     bs, bias = (), None
     if bq is not None:
+        _refuse_tangents('linear3_fp8', bq, bk, bv)
         bs, bias = (bq, bk, bv), fused._adjacent_view([bq, bk, bv])
         bias = bias if bias is not None else torch.cat([t.detach() for t in bs], 0)
     _check_bias(bias, shape[0], x, 'linear3_fp8')
@@ -456,7 +468,8 @@ class Packed8(object):
 
 
 def pack8(x):
-    """``x`` (fp32 or bf16) as int8 blocks along its last dimension: 1 + 1/128 bytes per element."""
+    """``x`` (fp32 or bf16) as int8 blocks along its last dimension: 1 + 1/128 bytes per element.  The blocks are
+    values: no gradient flows back through ``unpack8(pack8(x))`` (``checkpoint8`` passes one through)."""
     _check_act(x, 'pack8')
     q, s = C().pack8(x) if use_kernels(x) else _pack8_ref(x.detach())
     return Packed8(q, s, x.shape, x.dtype)
@@ -512,7 +525,7 @@ def checkpoint8(fn, x, *rest):
     """``fn(x, *rest)`` keeping only ``x`` in 8 bits (``pack8``) and ``rest`` as it is: the forward runs
     on ``x`` itself; the backward recomputes the segment from the decoded copy and passes x's
     gradient straight through the rounding.  ``fn`` returns a tensor or a tuple of them."""
-    _check_act(x, 'checkpoint8')
+    _check_act(x, 'checkpoint8', tangents=not torch.is_grad_enabled())
     if not torch.is_grad_enabled():
         return fn(x, *rest)
     from torch.utils.checkpoint import checkpoint

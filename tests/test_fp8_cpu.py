@@ -286,3 +286,38 @@ def test_kept_weights_serve_until_told_otherwise():
     with torch.no_grad():
         enc.keep_fp8_weights(False)
         assert torch.equal(run(), now)
+
+
+def tangent_calls(dev):
+    """Calls of every entry point with one dual argument: (name, call); inside a dual level."""
+    from torch.autograd import forward_ad
+    t = lambda *s: torch.ones(*s, device=dev)
+    dual = lambda *s: forward_ad.make_dual(t(*s), t(*s))
+    w8 = lambda: ops.Fp8Weight(t(8, 130))
+    return [('pack8', lambda: ops.pack8(dual(3, 130))), ('kept', lambda: ops.linear_fp8(dual(3, 130), w8())),
+            ('kept, bias', lambda: ops.linear_fp8(t(3, 130), w8(), dual(8))), ('x', lambda: ops.linear_fp8(dual(3, 130), t(8, 130))),
+            ('W', lambda: ops.linear_fp8(t(3, 130), dual(8, 130))), ('bias', lambda: ops.linear_fp8(t(3, 130), t(8, 130), dual(8))),
+            ('Fp8Weight', lambda: ops.Fp8Weight(dual(8, 130))), ('fp8_weights', lambda: ops.fp8_weights([None, dual(8, 128)])),
+            ('gelu', lambda: ops.bias_act(dual(3, 130), None, 'gelu', bits=8)),
+            ('gelu bias', lambda: ops.bias_act(t(3, 130), dual(130), 'gelu', bits=8)),
+            ('ffn x', lambda: ops.ffn_fp8(dual(3, 130), t(8, 130), None, t(5, 8))), ('ffn W', lambda: ops.ffn_fp8(t(3, 130), t(8, 130), None, dual(5, 8))),
+            ('ffn b', lambda: ops.ffn_fp8(t(3, 130), t(8, 130), dual(8), t(5, 8))),
+            ('linear3', lambda: ops.linear3_fp8(t(3, 130), t(8, 130), dual(8, 130), t(8, 130), None, None, None)),
+            ('linear3 bias', lambda: ops.linear3_fp8(t(3, 130), t(8, 130), t(8, 130), t(8, 130), t(8), t(8), dual(8)))]
+
+
+@pytest.mark.parametrize('grad', [True, False])
+def test_forward_mode_is_refused(grad):
+    """A tangent that no operator carries on is an error, never dropped; one that checkpoint8 need not touch stays."""
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        for name, call in tangent_calls('cpu'):
+            with pytest.raises(RuntimeError):
+                call()
+                pytest.fail(name)
+        x = forward_ad.make_dual(torch.ones(3, 130), torch.ones(3, 130))
+        if grad:
+            with pytest.raises(RuntimeError):
+                ops.checkpoint8(lambda t: t * 2, x)
+        else:
+            assert torch.equal(forward_ad.unpack_dual(ops.checkpoint8(lambda t: t * 2, x)).tangent, torch.full((3, 130), 2.0))

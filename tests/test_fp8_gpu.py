@@ -745,3 +745,14 @@ def test_e4m3_sums_lose_what_the_instruction_cuts(dev, M, K, N, spread):
     # fp32: K / 64 + 8 roundings to 2^-24 of a running sum, itself about the root of sum (a b)^2, twice that allowed
     var = torch.where(cut < step, cut ** 2, step ** 2 / 3).sum(1) + (K / 64 + 8) * 2.0 ** -46 * (w * a).square().sum(1)
     assert (err ** 2 / var).mean() <= 1.31 * (1 + 2.0 ** -7)
+
+
+@pytest.mark.parametrize('grad', [True, False])
+def test_forward_mode_is_refused(dev, grad):
+    from test_fp8_cpu import tangent_calls
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        for name, call in tangent_calls(dev):
+            with pytest.raises(RuntimeError):
+                call()
+                pytest.fail(name)
