@@ -27,6 +27,7 @@ import json
 import logging
 import math
 import os
+import threading
 
 import torch
 import torch.nn as nn
@@ -109,11 +110,28 @@ class BertConfig(object):
         return json.dumps(self.to_dict(), indent=2, sort_keys=True) + '\n'
 
 
-class LinearActivation(nn.Module):
+class _Codes(threading.local):
+    # {module: its weight's e4m3 codes} of the encoder forward that this thread is in.  Per thread: another
+    # thread's codes are made on that thread's stream, for that forward's gradients, and go with it
+    of = {}
+
+
+_CODES = _Codes()
+
+
+class _Fp8Part(object):
+    """A module of an encoder layer that holds a linear weight."""
+    fp8 = False     # set_compute_dtype(fp8=True): e4m3 products, 8-bit kept activations
+
+    @property
+    def codes(self):
+        """The weight's e4m3 codes while this thread is in its encoder's forward, else None."""
+        return _CODES.of.get(self)
+
+
+class LinearActivation(_Fp8Part, nn.Module):
     """Linear + activation; GELU/tanh with bias run as one fused epilogue kernel."""
     __constants__ = ['bias']
-    fp8 = False     # set_compute_dtype(fp8=True): e4m3 products, 8-bit kept activations (encoder layers)
-    codes = None    # the weight's e4m3 codes while its encoder's forward runs (BertEncoder)
 
     def __init__(self, in_features, out_features, act='gelu', bias=True):
         super().__init__()
@@ -190,9 +208,7 @@ class BertEmbeddings(nn.Module):
 _QKV_BIAS_EPILOGUE = os.environ.get('HX_QKV_BIAS_EPILOGUE', '1') != '0'
 
 
-class BertSelfAttention(nn.Module):
-    fp8, codes = False, None
-
+class BertSelfAttention(_Fp8Part, nn.Module):
     def __init__(self, config):
         super().__init__()
         if config.hidden_size % config.num_attention_heads != 0:
@@ -227,9 +243,7 @@ class BertSelfAttention(nn.Module):
                              bias=bias)
 
 
-class BertSelfOutput(nn.Module):
-    fp8, codes = False, None
-
+class BertSelfOutput(_Fp8Part, nn.Module):
     def __init__(self, config):
         super().__init__()
         self.dense = nn.Linear(config.hidden_size, config.hidden_size)
@@ -266,9 +280,7 @@ class BertIntermediate(nn.Module):
         return self.dense_act(hidden_states, res_grad)
 
 
-class BertOutput(nn.Module):
-    fp8, codes = False, None
-
+class BertOutput(_Fp8Part, nn.Module):
     def __init__(self, config):
         super().__init__()
         self.dense = nn.Linear(config.intermediate_size, config.hidden_size)
@@ -383,19 +395,18 @@ class BertEncoder(nn.Module):
     @contextlib.contextmanager
     def _weight_codes(self):
         """The e4m3 codes of every linear weight, made in one launch (or kept: ``keep_fp8_weights``) and
-        handed to the layers for this forward alone: a segment recomputed in the backward makes its
-        own."""
+        handed to the layers for this forward alone, in this thread: a segment recomputed in the backward
+        makes its own."""
         parts, grad = self._parts(), torch.is_grad_enabled()
         codes = None if grad else self.__dict__.get('_fp8_kept')
         if codes is None or len(codes) != len(parts):
             codes = self._fp8_codes(grad)
+        outer = _CODES.of
+        _CODES.of = {**outer, **dict(zip(parts, codes))}
         try:
-            for part, c in zip(parts, codes):
-                part.__dict__['codes'] = c
             yield
         finally:
-            for part in parts:
-                part.__dict__['codes'] = None
+            _CODES.of = outer
 
     def _forward(self, hidden_states, attention_mask_bias, output_all_encoded_layers, checkpoint_activations):
         all_encoder_layers = []

@@ -229,3 +229,50 @@ def test_kept_weights_serve_captured_and_alone(dev):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, enc(x, b, output_all_encoded_layers=False)[-1]), i
+
+
+def test_two_threads_two_streams_one_encoder(dev):
+    """One encoder in two threads with a stream each, a training pass beside serving forwards: each result is what
+    it is alone."""
+    import threading
+    enc = _encoder(layers=3)
+    for p in enc.parameters():
+        p.data = p.data.clone()
+    x, bias, d = _inputs(B=4, S=64)
+    xs = [x.detach().clone().requires_grad_(True), torch.randn(x.shape, generator=torch.Generator(device='cuda').manual_seed(9), device=dev).to(x.dtype)]
+
+    def train():
+        h = xs[0].detach().clone().requires_grad_(True)
+        out = enc(h, bias, output_all_encoded_layers=False)[-1]
+        return (out.detach(),) + torch.autograd.grad(out, [h] + list(enc.parameters()), d.to(out.dtype))
+
+    def serve():
+        with torch.no_grad():
+            return (enc(xs[1], bias, output_all_encoded_layers=False)[-1],)
+    jobs = [train, serve]
+    alone = [job() for job in jobs]
+    torch.cuda.synchronize()
+    gate, got, errors = threading.Barrier(2), [[], []], []
+
+    def loop(i):
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                for _ in range(12):
+                    gate.wait(30)
+                    got[i].append(jobs[i]())
+            st.synchronize()
+        except Exception as e:
+            errors.append(e)
+            gate.abort()
+    ts = [threading.Thread(target=loop, args=(i,)) for i in (0, 1)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join(60)
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for i in (0, 1):
+        assert len(got[i]) == 12
+        for k, run in enumerate(got[i]):
+            assert all(torch.equal(a, b) for a, b in zip(run, alone[i])), (i, k)
