@@ -20,6 +20,7 @@ Reference sites: hetseq/bert_modeling.py:334-336 (Q/K/V), :383 (attention output
 (MLM decoder), :1221 (NER classifier) and their backward products.
 """
 import os
+import threading
 
 import torch
 
@@ -28,8 +29,17 @@ from ._ext import C, use_kernels
 
 class _State(object):
     on = False
-    scope = None        # {(data_ptr, shape): (wf, wt, parts)} for the running forward
     min_rows = 1
+
+
+class _Scopes(threading.local):
+    # of the forward that this thread is in (another thread's operands are made on that thread's stream and
+    # freed when its forward ends)
+    pieces = None       # {(data_ptr, shape): (wf, wt, parts)}
+    b16 = None          # {(data_ptr, shape): W^T in bf16}
+
+
+_SCOPES = _Scopes()
 
 
 def set_enabled(flag):
@@ -183,7 +193,7 @@ class weight_scope(object):
         self.Ws = [W for W in Ws if W is not None]
 
     def __enter__(self):
-        self.prev = _State.scope
+        self.prev = _SCOPES.pieces
         Ws = [W for W in self.Ws if W.dim() == 2 and W.shape[0] % 64 == 0 and W.shape[1] % 64 == 0 and
               W.is_contiguous() and W.dtype == torch.float32 and W.is_cuda]
         if _State.on and Ws:
@@ -192,19 +202,19 @@ class weight_scope(object):
                 chunk = Ws[i:i + 64]
                 for W, o in zip(chunk, C().split_weight_f16(chunk)):
                     d[(W.data_ptr(), tuple(W.shape))] = tuple(o)
-            _State.scope = d
+            _SCOPES.pieces = d
         return self
 
     def __exit__(self, *exc):
-        _State.scope = self.prev
+        _SCOPES.pieces = self.prev
         return False
 
 
 def weight_pieces(W):
     """(wf [N, 2K], wt [K, 2N], rmax [N, 1], cmax [K, 1]) of W [N, K] (N, K multiples of 64): the
     pieces of W and of W^T, and the per-row scale sources of each (W's row / column maxima)."""
-    if _State.scope is not None:
-        e = _State.scope.get((W.data_ptr(), tuple(W.shape)))
+    if _SCOPES.pieces is not None:
+        e = _SCOPES.pieces.get((W.data_ptr(), tuple(W.shape)))
         if e is not None:
             return e
     return tuple(C().split_weight_f16([W.detach().contiguous()])[0])
@@ -279,10 +289,6 @@ def fit_cols(p):
 
 
 # ---------------------------------------------------------------- --precision bf16 (same kernel, one pass)
-class _B16(object):
-    scope = None        # {(data_ptr, shape): W^T in bf16} for the running forward
-
-
 def bf16_ok(x2, n_out, n_in):
     """--precision bf16 products on gemm_f16.hip's bf16 variant: bf16 GPU activations, 32-deep k
     steps, tile-able widths (the tiny heads stay on the library GEMM)."""
@@ -299,25 +305,25 @@ class bf16_scope(object):
                    W.shape[1] % 64 == 0 and W.is_contiguous() and W.dtype == torch.float32 and W.is_cuda]
 
     def __enter__(self):
-        self.prev = _B16.scope
+        self.prev = _SCOPES.b16
         if self.Ws:
             d = {}
             for i in range(0, len(self.Ws), 64):
                 chunk = self.Ws[i:i + 64]
                 for W, wt in zip(chunk, C().weight_bf16_t(chunk)):
                     d[(W.data_ptr(), tuple(W.shape))] = wt
-            _B16.scope = d
+            _SCOPES.b16 = d
         return self
 
     def __exit__(self, *exc):
-        _B16.scope = self.prev
+        _SCOPES.b16 = self.prev
         return False
 
 
 def bf16_wt(W):
     """W^T [K, N] in bf16 (the running forward's, or converted now)."""
-    if _B16.scope is not None:
-        e = _B16.scope.get((W.data_ptr(), tuple(W.shape)))
+    if _SCOPES.b16 is not None:
+        e = _SCOPES.b16.get((W.data_ptr(), tuple(W.shape)))
         if e is not None:
             return e
     return C().weight_bf16_t([W.detach().contiguous()])[0]

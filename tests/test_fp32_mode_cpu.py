@@ -149,3 +149,59 @@ def test_graph_train_step_modes():
     assert options.parse_training_args(base).graph_train_step == 'auto'
     assert options.parse_training_args(base + ['--graph-train-step']).graph_train_step == 'on'
     assert options.parse_training_args(base + ['--no-graph-train-step']).graph_train_step == 'off'
+
+
+@pytest.mark.parametrize('kind', ['fp16x3', 'bf16'])
+def test_a_forwards_weight_operands_belong_to_its_thread(monkeypatch, kind):
+    """Inside one thread's forward another thread makes its own operands of the same weight, and its forward's end
+    leaves the first one's in place."""
+    import threading
+
+    class Weight(object):   # what the scopes look at, on a "GPU"
+        shape, dtype, is_cuda = (64, 64), torch.float32, True
+
+        def dim(self):
+            return 2
+
+        def is_contiguous(self):
+            return True
+
+        def data_ptr(self):
+            return 4096
+
+        def detach(self):
+            return self
+
+        def contiguous(self):
+            return self
+
+    class Kernels(object):
+        def split_weight_f16(self, Ws):
+            return [(threading.get_ident(), object()) for _ in Ws]
+
+        def weight_bf16_t(self, Ws):
+            return [(threading.get_ident(), object()) for _ in Ws]
+    monkeypatch.setattr(gemm16, 'C', Kernels)
+    was = gemm16.enabled()
+    gemm16.set_enabled(True)
+    W, seen = Weight(), []
+    scope, get = (gemm16.weight_scope, gemm16.weight_pieces) if kind == 'fp16x3' else (gemm16.bf16_scope, gemm16.bf16_wt)
+
+    def other():
+        me = threading.get_ident()
+        seen.append(get(W)[0] == me)
+        with scope([W]):
+            first = get(W)
+            seen.append(first[0] == me and get(W) is first)
+    try:
+        with scope([W]):
+            mine = get(W)
+            assert get(W) is mine
+            t = threading.Thread(target=other)
+            t.start()
+            t.join(30)
+            assert seen == [True, True]
+            assert get(W) is mine
+        assert get(W) is not mine
+    finally:
+        gemm16.set_enabled(was)
