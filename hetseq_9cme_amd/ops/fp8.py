@@ -356,23 +356,23 @@ def linear3_fp8(x, wq, wk, wv, bq, bk, bv, res_grad=None, bias_grad=True, codes=
 class _BiasGelu8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, b):
-        ctx.b = b
-        if use_kernels(y):
+        ctx.b = b   # for its gradient slot; its values, which the slope is taken at, are saved: changed in place
+        if use_kernels(y):   # before the backward they are an error
             out, q, s = C().gelu8_fwd(y, b)
-            ctx.save_for_backward(q, s)
+            ctx.save_for_backward(q, s, b)
         else:
             u = y.float() if b is None else y.float() + b
             out = fused.gelu_ref(u).to(y.dtype)
-            ctx.save_for_backward(int8_ref(y), None)
+            ctx.save_for_backward(int8_ref(y), None, b)
         return out
 
     @staticmethod
     def backward(ctx, dout):
         _backward_checks('bias_act(bits=8)', dout)
-        q, s = ctx.saved_tensors
-        b, need_b = ctx.b, ctx.needs_input_grad[1]
+        q, s, b = ctx.saved_tensors
+        need_b = ctx.needs_input_grad[1]
         if use_kernels(dout):
-            dy, db = C().gelu8_bwd(dout.contiguous(), q, s, b, need_b, fused.grad_slot(b) if need_b else None)
+            dy, db = C().gelu8_bwd(dout.contiguous(), q, s, b, need_b, fused.grad_slot(ctx.b) if need_b else None)
             return dy, db
         dy = dout.float() * _gelu_grad_ref(q if b is None else q + b)
         return dy.to(dout.dtype), dy.reshape(-1, dy.shape[-1]).sum(0) if need_b else None
@@ -404,15 +404,15 @@ class _FfnFp8Fn(torch.autograd.Function):
         out = C().gemm_fp8(q, s, c2.q, c2.s, W2.shape[1], bf16)
         w1 = (c1.qt, c1.st) if need_x else (None, None)
         w2 = (c2.qt, c2.st) if need_u else (None, None)
-        ctx.save_for_backward(xt, xs, at, as_, kq, ks, *w1, *w2)
+        ctx.save_for_backward(xt, xs, at, as_, kq, ks, *w1, *w2, b1)   # (b1: the slope is taken at its values)
         return out.view(*x.shape[:-1], W2.shape[0])
 
     @staticmethod
     def backward(ctx, dy):
         _backward_checks('ffn_fp8', dy)
-        xt, xs, at, as_, kq, ks, w1, w1s, w2, w2s = ctx.saved_tensors
+        xt, xs, at, as_, kq, ks, w1, w1s, w2, w2s, b1 = ctx.saved_tensors
         need_x, _, _, _, need_1, need_b, need_2 = ctx.needs_input_grad
-        W1, b1, W2 = ctx.W1, ctx.b1, ctx.W2
+        W1, W2 = ctx.W1, ctx.W2
         dy2, bf16 = _rows2(dy), dy.dtype == torch.bfloat16
         M = dy2.shape[0]
         q, s, qt, st, _ = C().split8(dy2, ctx.need_u, need_2 and M > 0)
@@ -421,7 +421,7 @@ class _FfnFp8Fn(torch.autograd.Function):
         if ctx.need_u:
             da = C().gemm_fp8(q, s, w2, w2s, W2.shape[0], bf16)
             q, s, qt, st, db = C().gelu8_split_bwd(da, kq, ks, b1, need_x, need_1 and M > 0, need_b,
-                                                   fused.grad_slot(b1) if need_b else None)
+                                                   fused.grad_slot(ctx.b1) if need_b else None)
             g1 = _weight_grad(W1, qt, st, xt, xs, M) if need_1 else None
             if need_x:
                 dx = _input_grad(q, s, w1, w1s, W1.shape[0], M, ctx.xshape, bf16, ctx.mbox)

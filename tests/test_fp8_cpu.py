@@ -387,3 +387,21 @@ def test_two_threads_in_one_encoder(input_grad):
     assert torch.equal(got[0], alone)
     for n, g in want:
         assert torch.equal(enc.get_parameter(n).grad, g), n
+
+
+def changed_bias_calls(dev):
+    """GELU and feed-forward layers whose bias is changed between forward and backward: [(result, bias)]."""
+    t = lambda *s: torch.randn(*s, device=dev)
+    y, b = t(5, 64).requires_grad_(True), t(64).requires_grad_(True)
+    out = [(ops.bias_act(y, b, 'gelu', bits=8), b)]
+    b = t(64).requires_grad_(True)
+    out.append((ops.ffn_fp8(t(5, 32).requires_grad_(True), t(64, 32), b, t(16, 64)), b))
+    return out
+
+
+def test_a_bias_changed_before_the_backward_is_refused():
+    for out, b in changed_bias_calls('cpu'):
+        with torch.no_grad():
+            b.add_(1.0)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            out.sum().backward()

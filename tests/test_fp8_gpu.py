@@ -756,3 +756,24 @@ def test_forward_mode_is_refused(dev, grad):
             with pytest.raises(RuntimeError):
                 call()
                 pytest.fail(name)
+
+
+@pytest.mark.parametrize('flat', [False, True])
+def test_a_bias_changed_before_the_backward_is_refused(dev, flat):
+    from test_fp8_cpu import changed_bias_calls
+    for i in range(2):
+        if flat:   # parameters with flat gradient slots: the Python nodes
+            from hetseq_9cme_amd.parallel.flat_params import FlatParamSpace
+            m = torch.nn.Module()
+            m.b = torch.nn.Parameter(torch.randn(64, device=dev))
+            FlatParamSpace(m, dev).zero_grad()
+            x = torch.randn(5, 64, device=dev, requires_grad=True)
+            out = (ops.bias_act(x, m.b, 'gelu', bits=8) if i == 0 else
+                   ops.ffn_fp8(x, torch.randn(64, 64, device=dev), m.b, torch.randn(16, 64, device=dev)))
+            b = m.b
+        else:
+            out, b = changed_bias_calls(dev)[i]
+        with torch.no_grad():
+            b.add_(1.0)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            out.sum().backward()
