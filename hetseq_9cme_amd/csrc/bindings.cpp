@@ -1203,16 +1203,20 @@ inline std::pair<int64_t, int64_t> rows_cols8(const Tensor& x, const char* what)
   return {rows, x.size(-1)};
 }
 
-std::vector<Tensor> gelu8_fwd(Tensor y, OptT b) {
+// (gelu(y + b), y's int8 codes and scale bytes: undefined without `keep`)
+std::vector<OptT> gelu8_fwd(Tensor y, OptT b, bool keep) {
   const auto [rows, N] = rows_cols8(y, "gelu8_fwd y");
   check_bias8(b, N, y, "gelu8_fwd bias");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(y.device());
   Tensor out = torch::empty_like(y);
-  Tensor q = torch::empty({rows, blocks128(N), 128}, y.options().dtype(torch::kUInt8));
-  Tensor s = torch::empty({rows, blocks128(N)}, y.options().dtype(torch::kUInt8));
+  OptT q, s;
+  if (keep) {
+    q = torch::empty({rows, blocks128(N), 128}, y.options().dtype(torch::kUInt8));
+    s = torch::empty({rows, blocks128(N)}, y.options().dtype(torch::kUInt8));
+  }
   if (rows > 0)
-    hx_gelu8_fwd(act_bf16(y), y.data_ptr(), ptr_or_null<float>(b), out.data_ptr(), q.data_ptr<uint8_t>(),
-                 s.data_ptr<uint8_t>(), rows, (int)N, cur_stream(y));
+    hx_gelu8_fwd(act_bf16(y), y.data_ptr(), ptr_or_null<float>(b), out.data_ptr(), ptr_or_null<uint8_t>(q), ptr_or_null<uint8_t>(s), rows, (int)N,
+                 cur_stream(y));
   dbg_finite(out, "gelu8_fwd");
   return {out, q, s};
 }
@@ -1303,9 +1307,9 @@ std::vector<OptT> gelu8_split_bwd(Tensor dout, Tensor kq, Tensor ks, OptT b, boo
 // bias + GELU as one autograd node (see LinearFp8)
 struct BiasGelu8 : public torch::autograd::Function<BiasGelu8> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor y, OptT b) {
-    std::vector<Tensor> r = gelu8_fwd(y, b);
-    ctx->save_for_backward({r[1], r[2], has(b) ? *b : Tensor()});
-    return r[0];
+    std::vector<OptT> r = gelu8_fwd(y, b, true);
+    ctx->save_for_backward({*r[1], *r[2], has(b) ? *b : Tensor()});
+    return *r[0];
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
     refuse_second_derivative("bias_act(bits=8)");
@@ -1316,7 +1320,10 @@ struct BiasGelu8 : public torch::autograd::Function<BiasGelu8> {
     return {*r[0], need_b ? *r[1] : Tensor()};
   }
 };
-Tensor bias_gelu8(Tensor y, OptT b) { return BiasGelu8::apply(y.contiguous(), b); }
+Tensor bias_gelu8(Tensor y, OptT b) {
+  const bool wanted = at::GradMode::is_enabled() && (y.requires_grad() || (has(b) && b->requires_grad()));
+  return wanted ? BiasGelu8::apply(y.contiguous(), b) : *gelu8_fwd(y.contiguous(), b, false)[0];   // (no node, nothing kept)
+}
 
 std::vector<Tensor> pack8(Tensor x) {
   at::NoGradGuard no_grad;

@@ -307,9 +307,11 @@ __global__ __launch_bounds__(NT) void gelu8_fwd_k(const T* __restrict__ y, const
     const int c0 = (int)(i - r * nb) * 128 + 8 * l16, n = N - c0;
     Row8<T> x;
     x.load(y, r * N + c0, 0, n);
-    int e;
-    *reinterpret_cast<uint2*>(q + i * 128 + 8 * l16) = int8_block(x, 0, e);
-    if (l16 == 0) s[i] = (uint8_t)(e + 127);
+    if (q) {   // (null: no backward)
+      int e;
+      *reinterpret_cast<uint2*>(q + i * 128 + 8 * l16) = int8_block(x, 0, e);
+      if (l16 == 0) s[i] = (uint8_t)(e + 127);
+    }
     float v[8], bb[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) bb[k] = 0.f;

@@ -264,6 +264,15 @@ def _slots(params):
     return slots, slots[0] if len(slots) == 1 else fused._adjacent_view(slots)
 
 
+def _linear_nograd(x, w8, bias):
+    """The product alone: nothing is kept for a backward.  (Inside ``apply`` a parameter counts as needing its
+    gradient even under ``no_grad``.)"""
+    if use_kernels(x):
+        return C().linear_fp8_infer(x, w8.q, w8.s, w8.shape[1], bias)
+    y = e4m3_ref(_rows2(x)) @ w8.ref[0].t()
+    return (y if bias is None else y + bias).to(x.dtype).view(*x.shape[:-1], w8.shape[0])
+
+
 def _parts(g, params, slots, direct=False):
     """The stacked gradient ``g`` as one gradient per parameter (in its slot, where it has one)."""
     if g is None:
@@ -313,11 +322,13 @@ def linear_fp8(x, W, b=None, res_grad=None, codes=None):
     w8 = W if kept else codes
     if w8 is not None:
         _check_codes(w8, (N, K), W.device, grad and x.requires_grad, 'linear_fp8')
-    if use_kernels(x) and res_grad is None and (kept or not _flat(W)) and not _flat(b):
-        # autograd keeps the gradients: the whole layer is one node (bindings.cpp LinearFp8)
+    if use_kernels(x) and (not grad or res_grad is None and (kept or not _flat(W)) and not _flat(b)):
+        # autograd keeps the gradients, or there are none: the whole layer is one node (bindings.cpp LinearFp8)
         return C().linear_fp8(x, None if kept else W, b, [] if w8 is None else [w8.q, w8.s, w8.qt, w8.st], grad)
     if w8 is None:
         w8 = Fp8Weight(W, grad and x.requires_grad)
+    if not grad:
+        return _linear_nograd(x, w8, b)
     if kept:
         return _LinearFp8Fn.apply(x, w8, b, res_grad, True, 0, *(() if b is None else (b,)))
     return _LinearFp8Fn.apply(x, w8, b, res_grad, True, 1, W, *(() if b is None else (b,)))
@@ -349,20 +360,25 @@ def linear3_fp8(x, wq, wk, wv, bq, bk, bv, res_grad=None, bias_grad=True, codes=
     else:
         W = fused._adjacent_view([wq, wk, wv])
         codes = Fp8Weight(W if W is not None else torch.cat([wq.detach(), wk.detach(), wv.detach()], 0), need)
+    if not torch.is_grad_enabled():
+        return _linear_nograd(x, codes, bias)
     return _LinearFp8Fn.apply(x, codes, bias, res_grad, bool(bias_grad), 3, wq, wk, wv, *bs)
 
 
 # ---------------------------------------------------------------- bias + GELU with an int8 checkpoint
+def _bias_gelu_ref(y, b):
+    return fused.gelu_ref(y.float() if b is None else y.float() + b).to(y.dtype)
+
+
 class _BiasGelu8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, b):
         ctx.b = b   # for its gradient slot; its values, which the slope is taken at, are saved: changed in place
         if use_kernels(y):   # before the backward they are an error
-            out, q, s = C().gelu8_fwd(y, b)
+            out, q, s = C().gelu8_fwd(y, b, any(ctx.needs_input_grad))
             ctx.save_for_backward(q, s, b)
         else:
-            u = y.float() if b is None else y.float() + b
-            out = fused.gelu_ref(u).to(y.dtype)
+            out = _bias_gelu_ref(y, b)
             ctx.save_for_backward(int8_ref(y), None, b)
         return out
 
@@ -382,8 +398,11 @@ def bias_gelu8(y, b):
     """gelu(y + b); the backward reads y from int8 blocks (``bias_act(y, b, 'gelu', bits=8)``)."""
     _check_act(y, 'bias_act(bits=8)')
     _check_bias(b, y.shape[-1], y, 'bias_act(bits=8)')
-    if use_kernels(y) and not _flat(b):
+    grad = torch.is_grad_enabled()
+    if use_kernels(y) and not (grad and _flat(b)):
         return C().bias_gelu8(y, b)
+    if not grad:
+        return _bias_gelu_ref(y.contiguous(), b)
     return _BiasGelu8Fn.apply(y.contiguous(), b)
 
 
@@ -393,19 +412,25 @@ class _FfnFp8Fn(torch.autograd.Function):
     (quant8.hip gelu8_split_k): neither tensor is written."""
 
     @staticmethod
+    def products(x, c1, b1, c2, need_1, need_2, need_u):
+        """The forward, and what the weight gradients (need_1, need_2) and whatever is behind the GELU (need_u) read."""
+        x2, bf16 = _rows2(x), x.dtype == torch.bfloat16
+        q, s, xt, xs, _ = C().split8(x2, True, need_1)
+        y = C().gemm_fp8(q, s, c1.q, c1.s, c1.shape[1], bf16)
+        q, s, *kept = C().gelu8_split_fwd(y, b1, need_2, need_u)
+        out = C().gemm_fp8(q, s, c2.q, c2.s, c2.shape[1], bf16)
+        return (out.view(*x.shape[:-1], c2.shape[0]), xt, xs, *kept)
+
+    @staticmethod
     def forward(ctx, x, c1, c2, mbox, W1, b1, W2):
         need_x, _, _, _, need_1, need_b, need_2 = ctx.needs_input_grad
         ctx.xshape, ctx.mbox, ctx.W1, ctx.b1, ctx.W2 = x.shape, mbox, W1, b1, W2
         ctx.need_u = need_u = need_x or need_1 or need_b   # anything behind the GELU
-        x2, bf16 = _rows2(x), x.dtype == torch.bfloat16
-        q, s, xt, xs, _ = C().split8(x2, True, need_1)
-        y = C().gemm_fp8(q, s, c1.q, c1.s, W1.shape[1], bf16)
-        q, s, at, as_, kq, ks = C().gelu8_split_fwd(y, b1, need_2, need_u)
-        out = C().gemm_fp8(q, s, c2.q, c2.s, W2.shape[1], bf16)
+        out, xt, xs, at, as_, kq, ks = _FfnFp8Fn.products(x, c1, b1, c2, need_1, need_2, need_u)
         w1 = (c1.qt, c1.st) if need_x else (None, None)
         w2 = (c2.qt, c2.st) if need_u else (None, None)
         ctx.save_for_backward(xt, xs, at, as_, kq, ks, *w1, *w2, b1)   # (b1: the slope is taken at its values)
-        return out.view(*x.shape[:-1], W2.shape[0])
+        return out
 
     @staticmethod
     def backward(ctx, dy):
@@ -451,6 +476,8 @@ def ffn_fp8(x, W1, b1, W2, res_grad=None, codes=(None, None)):
         if given is not None:
             _check_codes(given, tuple(W.shape), W.device, need, 'ffn_fp8')
         c.append(given if given is not None else Fp8Weight(W, need))
+    if not grad:   # (see _linear_nograd)
+        return _FfnFp8Fn.products(x, c[0], b1, c[1], False, False, False)[0]
     return _FfnFp8Fn.apply(x, c[0], c[1], res_grad, W1, b1, W2)
 
 

@@ -405,3 +405,23 @@ def test_a_bias_changed_before_the_backward_is_refused():
             b.add_(1.0)
         with pytest.raises(RuntimeError, match='modified by an inplace operation'):
             out.sum().backward()
+
+
+def test_no_grad_forwards_make_no_transposed_codes(monkeypatch):
+    """Under no_grad, with parameters that need gradients, the results are the same and nothing of a backward is made."""
+    W, b, W2 = (torch.randn(*s, requires_grad=True) for s in ((64, 130), (64,), (16, 64)))
+    q = [torch.randn(64, 130, requires_grad=True) for _ in range(3)]
+    x = torch.randn(2, 5, 130)
+    h = torch.randn(5, 64)
+    w8, w28, q8 = ops.Fp8Weight(W), ops.Fp8Weight(W2), ops.Fp8Weight(torch.cat(q))
+    calls = [lambda: ops.linear_fp8(x, W, b, codes=w8), lambda: ops.linear3_fp8(x, *q, None, None, None, codes=q8),
+             lambda: ops.bias_act(h, b, 'gelu', bits=8), lambda: ops.ffn_fp8(x, W, b, W2, codes=(w8, w28))]
+    refs = [f().detach() for f in calls]
+    seen = []
+    e4m3_ref, int8_ref = fp8.e4m3_ref, fp8.int8_ref
+    monkeypatch.setattr(fp8, 'e4m3_ref', lambda t: seen.append(tuple(t.shape)) or e4m3_ref(t))
+    monkeypatch.setattr(fp8, 'int8_ref', lambda t: pytest.fail('kept codes'))
+    with torch.no_grad():
+        for f, r in zip(calls, refs):
+            assert torch.equal(f(), r)
+    assert all(s in ((10, 130), (10, 64)) for s in seen), seen

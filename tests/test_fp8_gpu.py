@@ -777,3 +777,89 @@ def test_a_bias_changed_before_the_backward_is_refused(dev, flat):
             b.add_(1.0)
         with pytest.raises(RuntimeError, match='modified by an inplace operation'):
             out.sum().backward()
+
+
+# ---------------------------------------------------------------- without gradients
+class Calls(object):
+    """The extension, its calls by name written down."""
+    def __init__(self):
+        self.seen = []
+
+    def __getattr__(self, name):
+        f = getattr(ops.C(), name)
+        return lambda *a, **kw: self.seen.append((name, a)) or f(*a, **kw)
+
+
+def recorded(monkeypatch, call):
+    from hetseq_9cme_amd.ops import fp8
+    calls = Calls()
+    with monkeypatch.context() as m:
+        m.setattr(fp8, 'C', lambda: calls)
+        out = call()
+    return out, calls.seen
+
+
+def peak(call):
+    torch.cuda.synchronize()
+    base = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = call()
+    torch.cuda.synchronize()
+    return torch.cuda.max_memory_allocated() - base, out
+
+
+def _params(dev, flat, **shapes):
+    """Parameters that need gradients, in a flat space (the engine's) or not."""
+    m = torch.nn.Module()
+    for i, (n, s) in enumerate(shapes.items()):
+        m.register_parameter(n, torch.nn.Parameter(rand(s, torch.float32, 60 + i) * 0.05))
+    if flat:
+        from hetseq_9cme_amd.parallel.flat_params import FlatParamSpace
+        FlatParamSpace(m, dev).zero_grad()
+    return [getattr(m, n) for n in shapes]
+
+
+@pytest.mark.parametrize('flat', [False, True])
+def test_no_grad_forward_keeps_nothing(dev, monkeypatch, flat):
+    """Under no_grad, with parameters that need gradients: no transposed copies, no kept codes, and the one-launch
+    product for few rows; the results are those of a forward that keeps them."""
+    W, W2, b, bo = _params(dev, flat, W=(512, 256), W2=(256, 512), b=(512,), bo=(256,))
+    q = _params(dev, flat, q=(256, 256), k=(256, 256), v=(256, 256), bq=(256,), bk=(256,), bv=(256,))
+    w8, w3 = ops.Fp8Weight(W), ops.Fp8Weight(torch.cat([t.detach() for t in q[:3]]))
+    for M in (3000, 20):
+        x = rand((M, 256), torch.bfloat16, M)
+        h = rand((M, 512), torch.bfloat16, M + 1)
+        calls = {'linear': lambda: ops.linear_fp8(x, W, b, codes=w8), 'own': lambda: ops.linear_fp8(x, W, b),
+                 'mailbox': lambda: ops.linear_fp8(x, W, b, res_grad=ops.ResidualGrad(), codes=w8),
+                 'linear3': lambda: ops.linear3_fp8(x, *q, bias_grad=False, codes=w3),
+                 'gelu': lambda: ops.bias_act(h, b, 'gelu', bits=8), 'gelu alone': lambda: ops.bias_act(h, None, 'gelu', bits=8),
+                 'ffn': lambda: ops.ffn_fp8(x, W, b, W2, codes=(w8, ops.Fp8Weight(W2)))}
+        for name, call in calls.items():
+            ref = call().detach()
+            with torch.no_grad():
+                out, seen = recorded(monkeypatch, call)
+            assert not out.requires_grad
+            names = [n for n, _ in seen]
+            for n, a in seen:
+                if n == 'split8' and name != 'own' and a[0].shape[0] == M:
+                    assert not a[2], (name, 'transposed codes')
+                if n == 'gelu8_split_fwd':
+                    assert not a[2] and not a[3], name
+                assert n not in ('linear_fp8_fwd', 'gelu8_fwd'), (name, names)
+            if M == 3000 or name in ('own', 'gelu', 'gelu alone', 'ffn'):
+                assert torch.equal(out, ref), (name, M)
+            else:   # few rows: exact products
+                Wq, bias = (torch.cat(q[:3]), torch.cat(q[3:])) if name == 'linear3' else (W, b)
+                assert_product(out, e4m3(x), e4m3(Wq.detach()), bias=bias.detach())
+
+
+def test_no_grad_memory(dev):
+    b = torch.nn.Parameter(rand((512,), torch.float32, 2))
+    y = rand((4096, 512), torch.bfloat16, 1)
+    with torch.no_grad():
+        assert peak(lambda: ops.bias_act(y, b, 'gelu', bits=8))[0] <= y.numel() * 2 + 1024      # its result alone
+    assert peak(lambda: ops.bias_act(y, b.detach(), 'gelu', bits=8))[0] <= y.numel() * 2 + 1024
+    W = torch.nn.Parameter(rand((512, 512), torch.float32, 2) * 0.05)
+    w8 = ops.Fp8Weight(W)
+    with torch.no_grad():   # the result, x's codes and scale words
+        assert peak(lambda: ops.linear_fp8(y, W, codes=w8))[0] <= y.numel() * 2 + y.numel() + 4096 * 4 + 4096
