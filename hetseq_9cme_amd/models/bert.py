@@ -389,8 +389,27 @@ class BertEncoder(nn.Module):
     def keep_fp8_weights(self, keep=True):
         """For serving at fp8: the layers' weights are brought to 8 bits now, and every forward without
         gradients reads those until the next call (``keep=False``: codes once per forward again).  A
-        forward with gradients always takes the weights as they are."""
-        self.__dict__['_fp8_kept'] = self._fp8_codes(False) if keep else None
+        forward with gradients always takes the weights as they are.
+
+        A captured forward reads the codes' memory: a further call writes the new codes into the same memory
+        (ordered like any write to a weight), so that replays serve the new weights, and ``keep=False`` leaves the
+        memory to them.  Layers of other shapes or on another device take memory of their own: capture again.
+        The call waits for its codes, so forwards on any stream may follow it."""
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('keep_fp8_weights: not inside a graph capture (its codes would be those of the replays only)')
+        kept = self.__dict__.get('_fp8_kept')
+        self.__dict__['_fp8_serving'] = bool(keep)
+        if not keep:
+            return
+        codes = self._fp8_codes(False)
+        if kept is not None and len(kept) == len(codes) and all(a.holds(b) for a, b in zip(kept, codes)):
+            for a, b in zip(kept, codes):
+                a.assign(b)
+        else:
+            self.__dict__['_fp8_kept'] = kept = codes
+        dev = kept[0].device if kept else None
+        if dev is not None and dev.type == 'cuda':
+            torch.cuda.current_stream(dev).synchronize()
 
     @contextlib.contextmanager
     def _weight_codes(self):
@@ -398,7 +417,7 @@ class BertEncoder(nn.Module):
         handed to the layers for this forward alone, in this thread: a segment recomputed in the backward
         makes its own."""
         parts, grad = self._parts(), torch.is_grad_enabled()
-        codes = None if grad else self.__dict__.get('_fp8_kept')
+        codes = self.__dict__.get('_fp8_kept') if self.__dict__.get('_fp8_serving') and not grad else None
         if codes is None or len(codes) != len(parts):
             codes = self._fp8_codes(grad)
         outer = _CODES.of

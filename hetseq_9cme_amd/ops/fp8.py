@@ -133,6 +133,21 @@ class Fp8Weight(object):
     def is_cuda(self):
         return self.device.type == 'cuda'
 
+    def holds(self, other):
+        """Whether this one's memory fits ``other``'s codes."""
+        return (self.shape == other.shape and self.device == other.device and (self.ref is None) == (other.ref is None) and
+                self.has_grad == other.has_grad)
+
+    def assign(self, other):
+        """``other``'s codes into this one's memory, which captured forwards read."""
+        if self.ref is not None:
+            self.ref = other.ref
+            return
+        with torch.inference_mode():   # (codes made in inference mode may be written in it only)
+            for a, b in ((self.q, other.q), (self.s, other.s), (self.qt, other.qt), (self.st, other.st)):
+                if a is not None:
+                    a.copy_(b)
+
     @property
     def has_grad(self):
         return self.qt is not None or (self.ref is not None and self.ref[1] is not None)

@@ -425,3 +425,30 @@ def test_no_grad_forwards_make_no_transposed_codes(monkeypatch):
         for f, r in zip(calls, refs):
             assert torch.equal(f(), r)
     assert all(s in ((10, 130), (10, 64)) for s in seen), seen
+
+
+def test_keeping_again_writes_the_same_codes():
+    """keep_fp8_weights again: the codes that a captured forward reads take the new values; keep=False leaves them."""
+    enc = _fp8_encoder()
+    x, mask = torch.randn(2, 7, 64), torch.zeros(2, 7)
+    run = lambda: enc(x, mask, output_all_encoded_layers=False)[-1]
+    seen = []
+    linear3 = ops.linear3_fp8
+    with torch.no_grad(), pytest.MonkeyPatch.context() as m:
+        m.setattr(ops, 'linear3_fp8', lambda *a, **kw: seen.append(kw['codes']) or linear3(*a, **kw))
+        enc.keep_fp8_weights()
+        first = run()
+        for layer in enc.layer:
+            layer.output.dense.weight.mul_(1.5)
+            layer.attention.self.query.weight.mul_(1.5)
+        own = list(seen)
+        with torch.inference_mode():
+            enc.keep_fp8_weights()
+        second = run()
+        assert not torch.equal(first, second)
+        enc.keep_fp8_weights(False)
+        assert torch.equal(run(), second)
+        enc.keep_fp8_weights()
+        assert torch.equal(run(), second)
+    assert len(own) == 2 and [id(c) for c in own] == [id(c) for c in seen[2:4]] == [id(c) for c in seen[6:8]]
+    assert not {id(c) for c in own} & {id(c) for c in seen[4:6]}

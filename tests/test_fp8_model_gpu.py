@@ -276,3 +276,42 @@ def test_two_threads_two_streams_one_encoder(dev):
         assert len(got[i]) == 12
         for k, run in enumerate(got[i]):
             assert all(torch.equal(a, b) for a, b in zip(run, alone[i])), (i, k)
+
+
+def test_captured_forwards_serve_the_weights_kept_last(dev):
+    """A forward captured on kept weights, replayed after the weights changed and were kept again, with other
+    tensors allocated in between: the new weights' results, without a new capture; after keep=False the last ones."""
+    enc = _encoder().eval()
+    x, b = _inputs()[:2]
+    with torch.no_grad():
+        enc.keep_fp8_weights()
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            enc(x, b, output_all_encoded_layers=False)
+        torch.cuda.current_stream().wait_stream(st)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = enc(x, b, output_all_encoded_layers=False)[-1]
+        last, others = None, []
+        for i in range(3):
+            for p in enc.parameters():
+                if p.dim() == 2:
+                    p.add_(0.02 * torch.randn(p.shape, generator=torch.Generator(device='cuda').manual_seed(i), device=dev))
+            with torch.inference_mode(i == 1):
+                enc.keep_fp8_weights()
+            others += [torch.full((n,), 255, dtype=torch.uint8, device=dev) for n in (128 * 128, 128 * 384, 384 * 128, 512) for _ in range(16)]
+            graph.replay()
+            torch.cuda.synchronize()
+            ref = enc(x, b, output_all_encoded_layers=False)[-1]
+            assert torch.equal(out, ref) and (last is None or not torch.equal(ref, last)), i
+            last = ref
+        enc.keep_fp8_weights(False)
+        others += [torch.full((n,), 255, dtype=torch.uint8, device=dev) for n in (128 * 128, 128 * 384, 384 * 128, 512) for _ in range(16)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, last)
+        graph2 = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match='not inside a graph capture'):
+            with torch.cuda.graph(graph2):
+                enc.keep_fp8_weights()
