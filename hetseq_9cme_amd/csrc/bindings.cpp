@@ -749,9 +749,10 @@ inline void check_rows8(const Tensor& x, const char* what) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.stride(1) == 1 || x.size(1) == 1) && (x.stride(0) >= x.size(1) || x.size(0) <= 1),
               what, ": a 2-D GPU tensor with unit column stride");
   act_bf16(x);
+  // (a launch has fewer than 2^32 threads, 512 of them to a tile of 128 x 128)
   TORCH_CHECK(x.size(0) < (1LL << 31) - 128 && x.size(1) >= 1 && x.size(1) <= (1LL << 22) &&
-                  blocks128(x.size(0)) * blocks128(x.size(1)) < (1LL << 31),
-              what, ": fewer than 2^31 rows of 1 .. 2^22 columns");
+                  blocks128(x.size(0)) * blocks128(x.size(1)) < (1LL << 22),
+              what, ": fewer than 2^31 rows of 1 .. 2^22 columns, and fewer than 2^22 blocks of 128 x 128");
 }
 inline Tensor scale_words(int64_t rows, int64_t cols, const Tensor& like) {
   // one byte per row and block of 128; four blocks of a row to a word, rows rounded up to 4
@@ -841,7 +842,7 @@ std::vector<std::vector<OptT>> split8_weights(std::vector<Tensor> Ws, bool by_co
     d.C[i] = (int)K;
     d.start[i] = (int)tiles;
     tiles += blocks128(N) * blocks128(K);
-    TORCH_CHECK(tiles < (1LL << 31), "split8_weights: too many tiles");
+    TORCH_CHECK(tiles < (1LL << 23), "split8_weights: too many tiles");
   }
   d.start[d.n] = (int)tiles;
   hx_split8_many(d, cur_stream(Ws[0]));
@@ -1203,10 +1204,15 @@ inline std::pair<int64_t, int64_t> rows_cols8(const Tensor& x, const char* what)
   return {rows, x.size(-1)};
 }
 
+// what the backward launches: 256 threads to 128 columns of a chunk of rows
+inline void check_gelu8_grid(int64_t rows, int64_t N) {
+  TORCH_CHECK(blocks128(N) * hx_gelu8_chunks(rows) < (1LL << 24), "bias_act(bits=8): ", rows, " rows of ", N, " are too many");
+}
 // (gelu(y + b), y's int8 codes and scale bytes: undefined without `keep`)
 std::vector<OptT> gelu8_fwd(Tensor y, OptT b, bool keep) {
   const auto [rows, N] = rows_cols8(y, "gelu8_fwd y");
   check_bias8(b, N, y, "gelu8_fwd bias");
+  if (keep) check_gelu8_grid(rows, N);
   c10::hip::HIPGuardMasqueradingAsCUDA guard(y.device());
   Tensor out = torch::empty_like(y);
   OptT q, s;
@@ -1225,6 +1231,7 @@ std::vector<OptT> gelu8_bwd(Tensor dout, Tensor q, Tensor s, OptT b, bool want_d
   const auto [rows, N] = rows_cols8(dout, "gelu8_bwd dout");
   check_kept(q, s, dout, rows, N, "gelu8_bwd");
   check_bias8(b, N, dout, "gelu8_bwd bias");
+  check_gelu8_grid(rows, N);
   c10::hip::HIPGuardMasqueradingAsCUDA guard(dout.device());
   auto f32 = dout.options().dtype(torch::kFloat32);
   Tensor dy = torch::empty_like(dout);

@@ -863,3 +863,19 @@ def test_no_grad_memory(dev):
     w8 = ops.Fp8Weight(W)
     with torch.no_grad():   # the result, x's codes and scale words
         assert peak(lambda: ops.linear_fp8(y, W, codes=w8))[0] <= y.numel() * 2 + y.numel() + 4096 * 4 + 4096
+
+
+def test_more_rows_than_a_launch_holds_are_refused(dev):
+    """A launch has fewer than 2^32 threads: what would need more is an error before anything is allocated."""
+    y = torch.zeros(2 ** 30 + 64, 1, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(RuntimeError, match='too many'):
+        ops.bias_act(y.requires_grad_(True), None, 'gelu', bits=8)
+    y = y.detach()
+    assert not ops.bias_act(y, None, 'gelu', bits=8).any()      # forward alone: any number
+    w8 = ops.Fp8Weight(torch.ones(1, 1, device=dev))
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match='fewer than 2\\^22 blocks'):
+            ops.linear_fp8(y, w8)
+        assert torch.equal(ops.linear_fp8(y[:2 ** 20] + 1.0, w8), y[:2 ** 20] + 1.0)
+    with pytest.raises(RuntimeError, match='fewer than 2\\^22 blocks'):
+        ops.linear_fp8(y, torch.ones(1, 1, device=dev, requires_grad=True))
