@@ -345,7 +345,7 @@ class BertEncoder(nn.Module):
 
     def forward(self, hidden_states, attention_mask_bias, output_all_encoded_layers=True,
                 checkpoint_activations=False):
-        fp8 = len(self.layer) > 0 and self.layer[0].output.fp8
+        fp8 = any(getattr(getattr(layer, 'output', None), 'fp8', False) for layer in self.layer)
         with (self._weight_codes() if fp8 else ops.weight_pieces_scope(self._piece_weights(), hidden_states)):
             return self._forward(hidden_states, attention_mask_bias, output_all_encoded_layers,
                                  checkpoint_activations)
@@ -366,12 +366,12 @@ class BertEncoder(nn.Module):
         return [ops.qkv_weight_view(*p) if isinstance(p, tuple) else p for p in ps]
 
     def _parts(self):
-        """The layers' modules that hold a linear weight, in order."""
-        parts = self.__dict__.get('_fp8_parts')
-        if parts is None or len(parts) != 4 * len(self.layer):
-            parts = self.__dict__['_fp8_parts'] = [
-                part for layer in self.layer for part in (layer.attention.self, layer.attention.output,
-                                                          layer.intermediate.dense_act, layer.output)]
+        """The modules that hold a linear weight of the layers that are BertLayers, in order."""
+        count, parts = self.__dict__.get('_fp8_parts', (None, None))
+        if count != len(self.layer):
+            parts = [part for layer in self.layer if isinstance(layer, BertLayer)
+                     for part in (layer.attention.self, layer.attention.output, layer.intermediate.dense_act, layer.output)]
+            self.__dict__['_fp8_parts'] = (len(self.layer), parts)
         return parts
 
     def _fp8_codes(self, grad):

@@ -452,3 +452,25 @@ def test_keeping_again_writes_the_same_codes():
         assert torch.equal(run(), second)
     assert len(own) == 2 and [id(c) for c in own] == [id(c) for c in seen[2:4]] == [id(c) for c in seen[6:8]]
     assert not {id(c) for c in own} & {id(c) for c in seen[4:6]}
+
+
+@pytest.mark.parametrize('on', [False, True])
+def test_a_layer_of_another_kind_in_an_encoder(on):
+    """An encoder whose first layer is replaced by a module without BertLayer's parts, between two forwards or (fp8)
+    before the first."""
+    class Halve(torch.nn.Module):
+        def forward(self, x, mask):
+            return x * 0.5
+    x, mask = torch.randn(2, 7, 64), torch.zeros(2, 7)
+    outs = []
+    for before in (False, True) if on else (False,):
+        enc = _fp8_encoder()
+        for m in enc.modules():
+            if getattr(m, 'fp8', False):
+                m.fp8 = on
+        if not before:
+            enc(x, mask)
+        enc.layer[0] = Halve()
+        outs.append(enc(x, mask, output_all_encoded_layers=False)[-1])
+        assert torch.equal(outs[-1], enc.layer[1](x * 0.5, mask))
+    assert torch.equal(outs[0], outs[-1])
