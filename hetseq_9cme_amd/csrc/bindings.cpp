@@ -745,6 +745,12 @@ inline void check_bias8(const OptT& b, int64_t N, const Tensor& like, const char
   check_f32(*b, what);
   TORCH_CHECK(b->numel() == N && b->device() == like.device(), what, ": fp32 [N] on the tensor's device");
 }
+// a bias of any stride, one after the other
+inline OptT bias8(const OptT& b, int64_t N, const Tensor& like, const char* what) {
+  const OptT d = has(b) && !b->is_contiguous() ? OptT(b->contiguous()) : b;
+  check_bias8(d, N, like, what);
+  return d;
+}
 inline void check_rows8(const Tensor& x, const char* what) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.stride(1) == 1 || x.size(1) == 1) && (x.stride(0) >= x.size(1) || x.size(0) <= 1),
               what, ": a 2-D GPU tensor with unit column stride");
@@ -929,7 +935,7 @@ Tensor gemm_fp8(Tensor a, Tensor as, Tensor b, Tensor bs, int64_t K, bool out_bf
   TORCH_CHECK(K >= 1, "gemm_fp8: an empty reduction");
   operand(a, as, "gemm_fp8 a");
   operand(b, bs, "gemm_fp8 b");
-  check_bias8(bias, N, a, "gemm_fp8 bias");
+  bias = bias8(bias, N, a, "gemm_fp8 bias");
   TORCH_CHECK(!beta || has(out_), "gemm_fp8: beta needs an output to accumulate into");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
   const auto dt = out_bf16 ? torch::kBFloat16 : torch::kFloat32;
@@ -958,13 +964,13 @@ struct Codes8 {
 
 // x [M, K] W^T (+ bias) from W's codes; with `keep`, also x's codes blocked along the rows (the weight
 // gradient's operand).  Small products that need no such copy go through one launch (fp8_rows_k).
-static Tensor linear_fp8_y(const Tensor& x2, const Tensor& wq, const Tensor& ws, const OptT& bias, bool keep, OptT* qt, OptT* st) {
+static Tensor linear_fp8_y(const Tensor& x2, const Tensor& wq, const Tensor& ws, const OptT& b, bool keep, OptT* qt, OptT* st) {
   const int64_t M = x2.size(0), K = x2.size(1), N = wq.size(0);
   if (!keep && M > 0) {
     check_rows8(x2, "linear_fp8");
     TORCH_CHECK(wq.is_cuda() && wq.device() == x2.device() && wq.size(1) == blocks128(K) * 128 && wq.is_contiguous() && aligned16(wq.data_ptr()) &&
                     ws.numel() == (blocks128(K) + 3) / 4 * ((N + 3) / 4 * 4) * 4, "linear_fp8: the weight's codes do not fit x");
-    check_bias8(bias, N, x2, "linear_fp8 bias");
+    const OptT bias = bias8(b, N, x2, "linear_fp8 bias");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(x2.device());
     const int bf16 = act_bf16(x2);
     Tensor y = torch::empty({M, N}, x2.options());
@@ -999,7 +1005,7 @@ static Tensor linear_fp8_y(const Tensor& x2, const Tensor& wq, const Tensor& ws,
     *qt = c[2];
     *st = c[3];
   }
-  return gemm_fp8(*c[0], *c[1], wq, ws, K, x2.scalar_type() == torch::kBFloat16, c10::nullopt, false, bias);
+  return gemm_fp8(*c[0], *c[1], wq, ws, K, x2.scalar_type() == torch::kBFloat16, c10::nullopt, false, b);
 }
 // [.., K] -> [rows, K] with unit column stride (a contiguous copy if it has none)
 static Tensor as_rows8(const Tensor& x) {
@@ -1050,7 +1056,7 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
     Tensor x2 = as_rows8(x);
     const int64_t M = x2.size(0);
     const bool keep = grad && has(W) && W->requires_grad(), wt = grad && x.requires_grad();
-    const OptT& bias = b;   // (no gradient is recorded here: apply() turns it off)
+    const OptT bias = bias8(b, N, x2, "linear_fp8 bias");   // (no gradient is recorded here: apply() turns it off)
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = N;
     Tensor y, kept, wtq, wts;   // what the backward needs: x's codes; the codes of W^T and their scales
@@ -1062,7 +1068,6 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
       y = linear_fp8_y(x2, *wq, *ws, bias, false, nullptr, nullptr);
     } else {
       check_rows8(x2, "linear_fp8");
-      check_bias8(bias, N, x2, "linear_fp8 bias");
       Tensor W2 = own ? as_rows8(*W) : Tensor();
       if (own) check_rows8(W2, "linear_fp8 weight");
       TORCH_CHECK(!keep || M <= (1LL << 22), "linear_fp8: at most 2^22 rows in a training step");
@@ -1211,7 +1216,7 @@ inline void check_gelu8_grid(int64_t rows, int64_t N) {
 // (gelu(y + b), y's int8 codes and scale bytes: undefined without `keep`)
 std::vector<OptT> gelu8_fwd(Tensor y, OptT b, bool keep) {
   const auto [rows, N] = rows_cols8(y, "gelu8_fwd y");
-  check_bias8(b, N, y, "gelu8_fwd bias");
+  b = bias8(b, N, y, "gelu8_fwd bias");
   if (keep) check_gelu8_grid(rows, N);
   c10::hip::HIPGuardMasqueradingAsCUDA guard(y.device());
   Tensor out = torch::empty_like(y);
@@ -1230,7 +1235,7 @@ std::vector<OptT> gelu8_fwd(Tensor y, OptT b, bool keep) {
 std::vector<OptT> gelu8_bwd(Tensor dout, Tensor q, Tensor s, OptT b, bool want_db, OptT db_out) {
   const auto [rows, N] = rows_cols8(dout, "gelu8_bwd dout");
   check_kept(q, s, dout, rows, N, "gelu8_bwd");
-  check_bias8(b, N, dout, "gelu8_bwd bias");
+  b = bias8(b, N, dout, "gelu8_bwd bias");
   check_gelu8_grid(rows, N);
   c10::hip::HIPGuardMasqueradingAsCUDA guard(dout.device());
   auto f32 = dout.options().dtype(torch::kFloat32);
@@ -1256,7 +1261,7 @@ std::vector<OptT> gelu8_bwd(Tensor dout, Tensor q, Tensor s, OptT b, bool want_d
 std::vector<OptT> gelu8_split_fwd(Tensor y, OptT b, bool by_cols, bool keep) {
   check_rows8(y, "gelu8_split_fwd");
   const int64_t R = y.size(0), C = y.size(1);
-  check_bias8(b, C, y, "gelu8_split_fwd bias");
+  b = bias8(b, C, y, "gelu8_split_fwd bias");
   TORCH_CHECK(!by_cols || R <= (1LL << 22), "gelu8_split_fwd: at most 2^22 rows blocked along the rows");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(y.device());
   auto u8 = y.options().dtype(torch::kUInt8);
@@ -1282,7 +1287,7 @@ std::vector<OptT> gelu8_split_bwd(Tensor dout, Tensor kq, Tensor ks, OptT b, boo
   check_rows8(dout, "gelu8_split_bwd");
   const int64_t R = dout.size(0), C = dout.size(1);
   check_kept(kq, ks, dout, R, C, "gelu8_split_bwd");
-  check_bias8(b, C, dout, "gelu8_split_bwd bias");
+  b = bias8(b, C, dout, "gelu8_split_bwd bias");
   TORCH_CHECK(!by_cols || R <= (1LL << 22), "gelu8_split_bwd: at most 2^22 rows blocked along the rows");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(dout.device());
   auto u8 = dout.options().dtype(torch::kUInt8);

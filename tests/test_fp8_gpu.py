@@ -879,3 +879,28 @@ def test_more_rows_than_a_launch_holds_are_refused(dev):
         assert torch.equal(ops.linear_fp8(y[:2 ** 20] + 1.0, w8), y[:2 ** 20] + 1.0)
     with pytest.raises(RuntimeError, match='fewer than 2\\^22 blocks'):
         ops.linear_fp8(y, torch.ones(1, 1, device=dev, requires_grad=True))
+
+
+@pytest.mark.parametrize('kind', ['strided', 'broadcast'])
+def test_bias_of_any_stride(dev, kind):
+    """Every second element of a buffer, one element for all features: as a dense copy, its gradient that of the view's base."""
+    base = rand((1200,) if kind == 'strided' else (1,), torch.float32, 3).requires_grad_(True)
+    view = (lambda n: base[:2 * n:2]) if kind == 'strided' else (lambda n: base.expand(n))
+    W, W2 = rand((600, 130), torch.float32, 1) * 0.02, rand((96, 600), torch.float32, 2) * 0.02
+    w8 = ops.Fp8Weight(W)
+    for M in (3, 900):
+        x, d, d2 = rand((M, 130), torch.bfloat16, M), rand((M, 600), torch.bfloat16, 5), rand((M, 96), torch.bfloat16, 6)
+        y = rand((M, 600), torch.bfloat16, 7)
+        for f, g in ((lambda b: ops.linear_fp8(x, W, b), d), (lambda b: ops.linear_fp8(x, w8, b), d),
+                     (lambda b: ops.bias_act(y, b, 'gelu', bits=8), d), (lambda b: ops.ffn_fp8(x, W, b, W2), d2)):
+            out, dense = f(view(600)), view(600).detach().clone().requires_grad_(True)
+            ref = f(dense)
+            assert torch.equal(out, ref)
+            gb, = torch.autograd.grad(out, base, g)
+            rb, = torch.autograd.grad(ref, dense, g)
+            if kind == 'strided':
+                assert torch.equal(gb[:1200:2], rb) and not gb[1::2].any()
+            else:
+                assert (gb - rb.sum()).abs() <= 700 * 2.0 ** -24 * rb.abs().sum()
+            with torch.no_grad():
+                assert torch.equal(f(view(600)), f(view(600).clone()))
