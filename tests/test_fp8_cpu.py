@@ -474,3 +474,21 @@ def test_a_layer_of_another_kind_in_an_encoder(on):
         outs.append(enc(x, mask, output_all_encoded_layers=False)[-1])
         assert torch.equal(outs[-1], enc.layer[1](x * 0.5, mask))
     assert torch.equal(outs[0], outs[-1])
+
+
+def inference_mode_calls(dev):
+    t = lambda *s: torch.randn(*s, device=dev)
+    x, W, b, W2, q = t(2, 5, 130), t(64, 130).requires_grad_(True), t(64).requires_grad_(True), t(16, 64), [t(64, 130).requires_grad_(True) for _ in range(3)]
+    w8 = ops.Fp8Weight(W)
+    y = t(5, 64)
+    return [lambda: ops.linear_fp8(x, W, b), lambda: ops.linear_fp8(x, w8, b), lambda: ops.linear3_fp8(x, *q, None, None, None),
+            lambda: ops.linear_fp8(x, W, b, codes=ops.fp8_weights([W])[0]), lambda: ops.bias_act(y, b, 'gelu', bits=8),
+            lambda: ops.ffn_fp8(x, W, b, W2), lambda: ops.unpack8(ops.pack8(x)), lambda: ops.checkpoint8(lambda v: v * 2, x)]
+
+
+def test_inference_mode():
+    for i, call in enumerate(inference_mode_calls('cpu')):
+        with torch.no_grad():
+            ref = call()
+        with torch.inference_mode():
+            assert torch.equal(call(), ref), i

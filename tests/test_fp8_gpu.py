@@ -904,3 +904,12 @@ def test_bias_of_any_stride(dev, kind):
                 assert (gb - rb.sum()).abs() <= 700 * 2.0 ** -24 * rb.abs().sum()
             with torch.no_grad():
                 assert torch.equal(f(view(600)), f(view(600).clone()))
+
+
+def test_inference_mode(dev):
+    from test_fp8_cpu import inference_mode_calls
+    for i, call in enumerate(inference_mode_calls(dev)):
+        with torch.no_grad():
+            ref = call()
+        with torch.inference_mode():
+            assert torch.equal(call(), ref), i
