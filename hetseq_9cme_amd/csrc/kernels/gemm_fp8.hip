@@ -19,10 +19,10 @@
 //    whose result is kept in fp32 (weight gradients, fp32 activations).  Half the matrix rate, and a
 //    decoding instruction (half rate itself) for every 4 codes of a fragment.
 //
-// Measured (M x K x N, us, TFLOP/s): 16384 x 4096 x 1024 57, 2410; 16384 x 1024 x 4096 74, 1860 and 8192 x 1024
-// x 4096 39, 1760 (134 and 67 MB of results); 16384 x 2304 x 768 31, 1880; exact, with its slab sums: 1024 x
-// 16384 x 4096 121, 1140; 2304 x 16384 x 768 66, 880; 1312 x 768 x 768 5.7.  The library's e4m3 and bf16
-// products of 8192^3 run at 2600 and 1150.
+// Measured alone, calls back to back (M x K x N, us, TFLOP/s): 16384 x 4096 x 1024 56, 2440; 16384 x 1024 x 4096 77,
+// 1780 and 8192 x 1024 x 4096 41, 1690 (134 and 67 MB of results); 16384 x 2304 x 768 31, 1855; exact: 8192 x 1024
+// x 4096 75, 920; with its slab sums 1024 x 16384 x 4096 119 .. 124, 1110 .. 1156 and 2304 x 16384 x 768 65 .. 67, 860 .. 900;
+// 1312 x 768 x 768 5.8.  The library's e4m3 and bf16 products of 8192^3 run at 2600 and 1150.
 #include <algorithm>
 #include <atomic>
 
@@ -64,6 +64,11 @@ __device__ __forceinline__ bf16x8v decode8(int w0, int w1, float s) {
 // per stage, two stages of LDS.  Persistent: a workgroup takes the tiles (and slabs) of its XCD's share
 // in turn, and its streams of stages, scale words and biases run on from one tile into the next, so the
 // first loads of a tile are under way while the one before it is stored.
+//
+// The 256 x 256 tile's 128 accumulators and fragments leave it short of registers: 8 (bf16 results), 6 (fp32 slabs) and
+// 33 (exact) are spilled, outside the main loop, and read back in the epilogue.  Where result rows are not 16-B aligned (g.vec = 0)
+// those reads lie between the stores and each waits for the stores before it, and a store's 16 B may cross lines: 8192 x
+// 1024 x 4097 takes 72 us (exact 92) where x 4096 takes 41 (75), 16384 x 4096 x 1023 66 where x 1024 takes 56.
 //
 // A k block is two 64-deep halves: while the MFMAs of one run on fragments in registers, the fragments
 // of the next are read.  A stage is opened (`open`) by a counted vmcnt and one raw barrier, which also
@@ -455,7 +460,7 @@ __global__ __launch_bounds__(256) void fp8_finish_k(HxFinish f) {
 // blocks dealt over its waves.  A wave reads its W codes straight into registers (32 B of a row per lane: a
 // whole 128-B line per row), rounds its 32 x values per lane to e4m3 (the block's maximum is 4 lanes), runs
 // both through exact bf16 MFMAs, and the waves' sums are added in LDS in wave order.  Bound by latency (one
-// token through 768 x 2304: 1.8 MB of codes, 3.5 us; 41 rows through 1024 x 1024: 3.7) and, as rows are
+// token through 768 x 2304: 1.8 MB of codes, 4.0 us; 41 rows through 1024 x 1024: 4.2) and, as rows are
 // added, by the rounding, which every workgroup does for itself: groups of rows in one workgroup share the W
 // codes but leave CUs idle (41 rows, 64 workgroups of 16 waves: 6.9 us).  Splitting the reduction inside
 // the workgroup keeps up to 16 waves of loads in flight where a tile per wave would leave one.

@@ -277,8 +277,8 @@ __global__ __launch_bounds__(SNT) void split8_many_k(HxSplit8Batch d) {
 // gelu(u) = u Phi(u), Phi(u) = (1 + erf(z)) / 2 with z = u / 1.41421 (the model's truncated constant).
 // erfc by Abramowitz & Stegun 7.1.26 (a degree-5 polynomial in 1 / (1 + p |z|) times exp(-z^2), error at
 // most 1.5e-7), its constants taken with u: the exponential is the derivative's too.  Both directions move
-// 5 bytes per bf16 element; 16384 x 4096 takes 68 us forward (4.9 TB/s; a large copy runs at 5.1) and 74
-// us back (4.5: the derivative's arithmetic on what int8 decodes to takes what is left), 41 x 4096 3.0 and 5.1.
+// 5 bytes per bf16 element; 16384 x 4096 takes 69 us forward (4.9 TB/s; a large copy runs at 5.1) and 74
+// us back (4.5: the derivative's arithmetic on what int8 decodes to takes what is left), 41 x 4096 3.2 and 5.2.
 // Back, a workgroup takes 128 columns of kRowChunk rows: 512 columns at a time left 41 rows with 8
 // workgroups (11 us); every row loaded before the first is used took 87 us (registers).
 struct Gelu {
@@ -372,8 +372,10 @@ __global__ __launch_bounds__(NT) void gelu8_bwd_k(const T* __restrict__ dout, co
 // its input's gradient by the first one's gradient products only: they go straight to e4m3 codes (both
 // blockings, as split8) and the tensors themselves are never written.  Same arithmetic, and the same
 // rounding to T in between, as gelu8 and split8 one after the other: equal bits.  5 bytes per bf16 element
-// each way where those move 9; 16384 x 4096 takes 85 us forward and 105 back (118 and 125 one after the
-// other), bound by the vector arithmetic of both.  64 registers for a fourth workgroup per CU spill (91, 122).
+// each way where those move 9; 16384 x 4096 takes 91 us forward and 109 back in the layer (76 and 94 at best; fp32 100 and
+// 141; bytes alone 66).  Vector instructions issue in 96 % of the forward's cycles (counted) and in 75 % of the backward's, whose
+// waves wait for their two loads for half of their time; 64 registers for a fourth workgroup per CU spill and cost more (91 / 122
+// where it was 87 / 114).
 struct GeluStep {   // y -> gelu(y + b), y's int8 blocks kept (q null: not kept)
   static constexpr bool sums = false;
   const float* b;
@@ -449,8 +451,8 @@ __global__ __launch_bounds__(SNT) void gelu8_split_k(HxSplit8 a, Step step) {
 }
 
 // ---------------------------------------------------------------- pack8 / unpack8
-// One pass, 16 lanes to a block; bound by memory: 16384 x 1024 fp32 (84 MB) 16 us each way (5.3 TB/s, part
-// of it from the last level cache), 1312 x 768 bf16 2.5 us.
+// One pass, 16 lanes to a block; bound by memory: 16384 x 1024 fp32 (84 MB) 15 us in and 16 back (5.2 - 5.8 TB/s, part
+// of it from the last level cache), 1312 x 768 bf16 2.8 us.
 template <typename T>
 __global__ __launch_bounds__(NT) void pack8_k(const T* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ s,
                                             int64_t nblk, int nb, int N) {
