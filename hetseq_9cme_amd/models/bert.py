@@ -367,11 +367,11 @@ class BertEncoder(nn.Module):
 
     def _parts(self):
         """The modules that hold a linear weight of the layers that are BertLayers, in order."""
-        count, parts = self.__dict__.get('_fp8_parts', (None, None))
+        count, parts = self.__dict__.get('_fp8_layer_parts', (None, None))
         if count != len(self.layer):
             parts = [part for layer in self.layer if isinstance(layer, BertLayer)
                      for part in (layer.attention.self, layer.attention.output, layer.intermediate.dense_act, layer.output)]
-            self.__dict__['_fp8_parts'] = (len(self.layer), parts)
+            self.__dict__['_fp8_layer_parts'] = (len(self.layer), parts)
         return parts
 
     def _fp8_codes(self, grad):
@@ -401,6 +401,7 @@ class BertEncoder(nn.Module):
         self.__dict__['_fp8_serving'] = bool(keep)
         if not keep:
             return
+        self.__dict__.pop('_fp8_layer_parts', None)   # the layers as they are now
         codes = self._fp8_codes(False)
         if kept is not None and len(kept) == len(codes) and all(a.holds(b) for a, b in zip(kept, codes)):
             for a, b in zip(kept, codes):

@@ -492,3 +492,20 @@ def test_inference_mode():
             ref = call()
         with torch.inference_mode():
             assert torch.equal(call(), ref), i
+
+
+def test_kept_weights_of_a_layer_put_in_later():
+    """keep_fp8_weights after a layer was replaced keeps the new layer's weights: until the next call it serves those."""
+    enc = _fp8_encoder()
+    x, mask = torch.randn(2, 7, 64), torch.zeros(2, 7)
+    run = lambda: enc(x, mask, output_all_encoded_layers=False)[-1]
+    with torch.no_grad():
+        enc.keep_fp8_weights()
+        run()
+        enc.layer[1] = _fp8_encoder(1).layer[0]
+        enc.keep_fp8_weights()
+        first = run()
+        enc.layer[1].output.dense.weight.mul_(2.0)
+        assert torch.equal(run(), first)
+        enc.keep_fp8_weights()
+        assert not torch.equal(run(), first)
