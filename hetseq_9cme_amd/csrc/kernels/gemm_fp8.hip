@@ -85,7 +85,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) *
   // in tile i - 1, of up to 4 k blocks before that tile's first barrier, when a slower wave may still be
   // reading the bias of tile i - 2 in its epilogue: two slots would give it tile i's.  The slot's tile before,
   // i - 3, was read by every wave before the barriers of tile i - 2.
-  constexpr int STAGE = (BM + BN) * 128, SCALES = 2 * STAGE, BIAS = SCALES + 4096, SPARE = BIAS + 3072;
+  constexpr int STAGE = (BM + BN) * 128, SCALES = 2 * STAGE, BIAS = SCALES + 4096, SPARE = BIAS + 3 * 1024;
   constexpr int STORES = MB * NB * (OB ? 2 : 4);   // of a lane in the epilogue
   static_assert(STORES < 63, "counted by vmcnt");
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -575,7 +575,7 @@ __global__ __launch_bounds__(1024) void fp8_rows_k(HxRows8 g) {
 template <int BM, int BN, int WM, int WN, int WGS, bool EXACT, bool OB>
 int launch(const HxGemm8& g, hipStream_t s) {
   constexpr int NT = (BM / WM) * (BN / WN) * 64;
-  constexpr int LDS = 2 * (BM + BN) * 128 + 4096 + 3072 + 1024;   // stages, scale words, biases, spare
+  constexpr int LDS = 2 * (BM + BN) * 128 + 4096 + 3 * 1024 + 1024;   // stages, scale words, biases, spare
   auto k = gemm_fp8_k<BM, BN, WM, WN, WGS, EXACT, OB>;
   static std::atomic<uint64_t> allowed{0};   // devices on which the kernel may take this much LDS
   int dev = 0;
