@@ -318,7 +318,9 @@ def linear_fp8(x, W, b=None, res_grad=None, codes=None):
     ``Fp8Weight`` (then it gets no gradient: inference, frozen layers); ``b`` fp32 [N].
     ``codes``: the parameter's ``Fp8Weight``, where the caller has made it for this forward
     (``fp8_weights``).  ``res_grad``: see ``ResidualGrad``.  First derivatives only; at most 2^22
-    features in or out, and in a training step 2^22 rows."""
+    features in or out, fewer than 2^22 blocks of 128 x 128 of x, and in a training step 2^22 rows.
+    Without gradients, few rows and a weight in 8 bits are one launch of exact products: a bf16 result may
+    then be the other neighbour of the training forward's."""
     kept = isinstance(W, Fp8Weight)
     if kept and codes is None and torch.is_tensor(x) and use_kernels(x) and W.q is not None and not torch.is_grad_enabled():
         return C().linear_fp8_infer(x, W.q, W.s, W.shape[1], b)   # (checks its arguments as below)
